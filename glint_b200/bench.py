@@ -320,7 +320,7 @@ def run_cli_bench(args):
     need = max(need, args.prompt_len + 64)
     llm = open_llm(shape, args.dtype, args.device, args.layers, args.context, cache_tokens=need,
                    max_active=max(max(batches), args.requests if "serve" in modes else 1),
-                   max_step_tokens=max(2048, min(args.prompt_len, 8192)))
+                   max_step_tokens=max(2048, min(args.prompt_len, 8192)), cache_dtype=args.cache_dtype)
     engine, model = llm.engine, llm.model
     rows = []
     if "prefill" in modes:

@@ -104,7 +104,42 @@ class PagedKVNeed(PagedNeed):
         return 2 * self.num_kv_heads * self.head_dim * element_size
 
     def readable_by(self, other):
-        return (getattr(other, "num_kv_heads", None), getattr(other, "head_dim", None)) == (self.num_kv_heads, self.head_dim)
+        return (isinstance(other, CodedKVNeed) == isinstance(self, CodedKVNeed)
+                and (getattr(other, "num_kv_heads", None), getattr(other, "head_dim", None)) == (self.num_kv_heads, self.head_dim))
+
+
+@dataclass(frozen=True)
+class CodedKVNeed(PagedKVNeed):
+    """Keys and values in codes of 8 bits with a scale per page and kv head (csrc/cache8.cu), in the same places as
+    ``PagedKVNeed``'s.  A group also keeps one layer's worth of wide pages in the engine's dtype, which the
+    attention of prompt portions reads (all layers take turns: a step's kernels run in order on one stream)."""
+
+    def group_key(self):
+        return ("coded",) + super().group_key()
+
+    def group_name(self):
+        return super().group_name() + "/int8"
+
+    def allocate(self, layers, num_pages, page_size, dtype, device):
+        one = (num_pages, self.num_kv_heads, page_size, self.head_dim)
+        codes = [torch.zeros((layers,) + one, dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.zeros((layers,) + one[:2], dtype=torch.float32, device=device) for _ in range(2)]
+        wide = [torch.zeros(one, dtype=dtype, device=device) for _ in range(2)]
+        return (*codes, *scales, *wide)
+
+    def view(self, storage, layer):
+        v = LayerView()
+        v.k, v.v, v.k_scale, v.v_scale = (t[layer] for t in storage[:4])
+        v.k_wide, v.v_wide = storage[4:]
+        return v
+
+    def bytes_per_token(self, element_size):
+        """Codes; a scale serves a page, counted as one of 16 tokens."""
+        return 2 * self.num_kv_heads * self.head_dim + (8 * self.num_kv_heads + 15) // 16
+
+    def shared_bytes_per_token(self, element_size):
+        """Of the wide pages, which the group has once."""
+        return 2 * self.num_kv_heads * self.head_dim * element_size
 
 
 @dataclass(frozen=True)
@@ -124,8 +159,11 @@ def is_paged(need):
 
 
 def cache_bytes_per_token(needs, cache_of, element_size):
-    """Bytes one token takes in all layers that keep pages of their own."""
-    return sum(n.bytes_per_token(element_size) for n, of in zip(needs, cache_of) if is_paged(n) and of is None)
+    """Bytes one token takes in all layers that keep pages of their own, and in what their groups have once."""
+    own = [n for n, of in zip(needs, cache_of) if is_paged(n) and of is None]
+    groups = {n.group_key(): n for n in own}
+    return (sum(n.bytes_per_token(element_size) for n in own)
+            + sum(n.shared_bytes_per_token(element_size) for n in groups.values() if hasattr(n, "shared_bytes_per_token")))
 
 
 class PagePool:
@@ -217,7 +255,7 @@ class PagedGroup:
         self.end_live = core.as_array(lib.glint_cache_end_live(handle, index), (num_slots,))       # one past the last page held
 
     def bytes_per_token(self):
-        return len(self.members) * self.need.bytes_per_token(self.element_size)
+        return cache_bytes_per_token([self.need] * len(self.members), [None] * len(self.members), self.element_size)
 
     def owned_pages(self, slot):
         return [int(p) for p in self.table[slot] if p >= 0]

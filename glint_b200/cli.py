@@ -26,6 +26,8 @@ def _add_engine_options(p):
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"],
                    help="bfloat16: serving kernels; float32: everything in true 32-bit")
     p.add_argument("--device", default="cuda:0")
+    p.add_argument("--cache-dtype", default="auto", choices=["auto", "int8"],
+                   help="keys and values: auto = as --dtype; int8 = codes of 8 bits with a scale per page and head")
 
 
 def build_parser():
@@ -114,7 +116,8 @@ def cmd_inspect(args):
 def cmd_run(args):
     from .engine.api import LLM
     prompt = _ids(args.prompt)
-    llm = LLM(args.file, dtype=args.dtype, device=args.device, max_active=1)      # one prompt: a cache of four contexts
+    llm = LLM(args.file, dtype=args.dtype, device=args.device, max_active=1,      # one prompt: a cache of four contexts
+              cache_dtype=args.cache_dtype)
     print(f"Prompt: {prompt}")
     t0 = time.time()
     out = llm.generate(prompt, max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k,
@@ -128,7 +131,8 @@ def cmd_run(args):
 def cmd_generate(args):
     from .engine.api import LLM
     prompt = _ids(args.tokens)
-    llm = LLM(args.file, dtype=args.dtype, device=args.device, max_active=1)      # one prompt: a cache of four contexts
+    llm = LLM(args.file, dtype=args.dtype, device=args.device, max_active=1,      # one prompt: a cache of four contexts
+              cache_dtype=args.cache_dtype)
     out = llm.generate(prompt, max_tokens=args.max_tokens, temperature=0.0)
     print(f"Generated token ids: {prompt + out}")
     return 0

@@ -31,7 +31,7 @@ NVCC_FLAGS = ARCH_FLAGS + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPI
 NVCC_FLAGS += os.environ.get("GLINT_NVCC_EXTRA", "").split()
 
 LIBRARIES = {
-    "core": ["elementwise.cu", "gemm_plain.cu", "attention_plain.cu", "sampling.cu", "sample_noalloc.cu", "runtime.cu"],
+    "core": ["elementwise.cu", "cache8.cu", "gemm_plain.cu", "attention_plain.cu", "sampling.cu", "sample_noalloc.cu", "runtime.cu"],
     "tensor": ["gemm_tcgen05.cu", "gemm_skinny.cu", "attention_decode.cu", "attention_prefill.cu", "attention_tcgen05.cu"],
     "host": ["host/cache_core.cpp"],
 }

@@ -19,6 +19,14 @@ int glint_rope_kv_write(const float* qkv, const int* positions, const int* token
                         int max_pages, const float* inv_freq, float factor, int rot, void* q_out, void* k_pool,
                         void* v_pool, int dtype, int T, int nh, int nkv, int hd, int page_size, int num_pages,
                         int* status, cudaStream_t stream);
+int glint_rope_append(const float* qkv, const int* positions, const int* token_seq, const int* block_table,
+                      int max_pages, const double* turns, int rot, int interleaved, float amplitude, void* q_out,
+                      int dtype, void* k_pool, void* v_pool, float* k_scale, float* v_scale, int T, int nh, int nkv,
+                      int hd, int page_size, int num_pages, int* status, cudaStream_t stream);
+int glint_cache8_unpack(const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
+                        const int* seq_start, const int* cu_seqlens, const int* block_table, int max_pages,
+                        void* k_out, void* v_out, int dtype, int n_seqs, int most_pages, int window, int nkv, int hd,
+                        int page_size, int num_pages, int* status, cudaStream_t stream);
 int glint_gated_act(const float* gu, void* out, int dtype, int T, int I, int act, cudaStream_t stream);
 int glint_gemm_plain(const void* A, const void* W, int dtype, float* out, int M, int N, int K, float cap,
                      cudaStream_t stream);
@@ -161,12 +169,46 @@ extern "C" int glint_op_rope_store(const GlintRuntime* rt, const GlintStep* step
                              step->num_tokens, nh, nkv, hd, view->page_size, view->num_pages, rt->status, stream));
 }
 
+extern "C" int glint_op_rope_append(const GlintRuntime* rt, const GlintStep* step, const float* qkv, void* q_out,
+                                    const GlintView* view, int nh, int nkv, int hd, const GlintRope* rope,
+                                    cudaStream_t stream) {
+  const int g = view->group;
+  return counted(glint_rope_append(qkv, step->positions, step->token_seq, step->block_table[g], step->max_pages[g],
+                                   rope->turns, rope->rotary_dim, rope->interleaved, rope->amplitude, q_out, rt->dtype,
+                                   view->writes ? view->k : nullptr, view->writes ? view->v : nullptr,
+                                   view->writes ? view->k_scale : nullptr, view->writes ? view->v_scale : nullptr,
+                                   step->num_tokens, nh, nkv, hd, view->page_size, view->num_pages, rt->status, stream));
+}
+
+extern "C" int glint_op_cache8_unpack(const GlintRuntime* rt, const GlintStep* step, const GlintView* view, int nkv,
+                                      int hd, int window, cudaStream_t stream) {
+  if (!view->k_scale || !view->v_scale || !view->k_wide || !view->v_wide) return GLINT_ERR_BAD_ARG;
+  const int g = view->group, page = view->page_size;
+  // pages of the longest range: up to the whole context, or what a portion and the window before it can touch
+  long long most = ((long long)step->max_context + page - 1) / page;
+  if (window > 0) {
+    const long long reach = ((long long)window + step->max_seq_len + page - 1) / page + 1;
+    if (reach < most) most = reach;
+  }
+  if (most > step->max_pages[g]) most = step->max_pages[g];
+  return counted(glint_cache8_unpack((const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale,
+                                     step->seq_start, step->cu_seqlens, step->block_table[g], step->max_pages[g],
+                                     view->k_wide, view->v_wide, rt->dtype, step->num_seqs, (int)most, window, nkv, hd, page,
+                                     view->num_pages, rt->status, stream));
+}
+
 extern "C" int glint_op_qkv_rope(const GlintRuntime* rt, const GlintStep* step, const void* x, const void* w,
                                  void* q_out, float* qkv_tmp, const GlintView* view, int nh, int nkv, int hd, int K,
                                  const float* inv_freq, float factor, int rotary_dim, GlintTrigTable* trig,
-                                 cudaStream_t stream) {
+                                 const GlintRope* rope, cudaStream_t stream) {
   const int M = step->num_tokens;
   if (M <= 0) return GLINT_OK;
+  if (view->k_scale || (rope && rope->only)) {   // coded pages, or a rotary form that the epilogues below do not have
+    if (!qkv_tmp || !rope) return GLINT_ERR_BAD_ARG;
+    const int rc = glint_op_linear(rt, x, w, qkv_tmp, 0, M, (nh + 2 * nkv) * hd, K, 0.f, 0, 0, nullptr, stream);
+    if (rc != GLINT_OK) return rc;
+    return glint_op_rope_append(rt, step, qkv_tmp, q_out, view, nh, nkv, hd, rope, stream);
+  }
   const int g = view->group;
   void* k = view->writes ? view->k : nullptr;
   void* v = view->writes ? view->v : nullptr;
@@ -255,6 +297,15 @@ extern "C" int glint_op_attention(const GlintRuntime* rt, const GlintStep* step,
                                   cudaStream_t stream) {
   const int T = step->num_tokens;
   if (T <= 0) return GLINT_OK;
+  if (view->k_scale) {
+    const int rc = glint_op_cache8_unpack(rt, step, view, nkv, hd, window, stream);
+    if (rc != GLINT_OK) return rc;
+    GlintView wide = *view;
+    wide.k = view->k_wide;
+    wide.v = view->v_wide;
+    wide.k_scale = wide.v_scale = nullptr;
+    return glint_op_attention(rt, step, q, &wide, out, nh, nkv, hd, multiplier, cap, window, stream);
+  }
   const int g = view->group;
   const int* table = step->block_table[g];
   const int max_pages = step->max_pages[g];
@@ -335,7 +386,7 @@ extern "C" int glint_program_size(const GlintProgram* prog) { return prog ? (int
 //   RMSNORM      p: x, weight, out        i: out dtype, H                             f: eps, offset
 //   ADD_RMSNORM  p: x, y, w_a, out, w_b   i: out dtype, H                             f: eps_a, offset_a, eps_b, offset_b
 //   LINEAR       p: a, w, out, tmp        i: out bf16, N, K, gated, activation        f: cap
-//   QKV_ROPE     p: x, w, q_out, tmp, view, inv_freq, trig   i: nh, nkv, hd, K, rotary dim    f: factor
+//   QKV_ROPE     p: x, w, q_out, tmp, view, inv_freq, trig, rope   i: nh, nkv, hd, K, rotary dim    f: factor
 //   ROPE_STORE   p: qkv, q_out, view, inv_freq               i: nh, nkv, hd, rotary dim       f: factor
 //   ATTENTION    p: q, view, out          i: nh, nkv, hd, window                      f: multiplier, cap
 //   HOST         nothing: the place of a step that the host language runs between two native stretches
@@ -369,7 +420,7 @@ extern "C" int glint_program_run(GlintProgram* prog, const GlintStep* step, int 
       case GLINT_OP_QKV_ROPE:
         rc = glint_op_qkv_rope(rt, step, op.p[0], op.p[1], op.p[2], (float*)op.p[3], (const GlintView*)op.p[4],
                                (int)op.i[0], (int)op.i[1], (int)op.i[2], (int)op.i[3], (const float*)op.p[5], op.f[0],
-                               (int)op.i[4], (GlintTrigTable*)op.p[6], stream);
+                               (int)op.i[4], (GlintTrigTable*)op.p[6], (const GlintRope*)op.p[7], stream);
         break;
       case GLINT_OP_ROPE_STORE:
         rc = glint_op_rope_store(rt, step, (const float*)op.p[0], op.p[1], (const GlintView*)op.p[2], (int)op.i[0],

@@ -90,11 +90,25 @@ struct GlintRuntime {
   GlintTensorEntries tensor;
 };
 
-// A cache view as the attention operations see it.
+// A cache view as the attention operations see it.  With scales the pages hold codes of 8 bits (cache8.cu); the wide
+// pools are then scratch of one layer in the activations' type, with the same places, for the attention of portions.
 struct GlintView {
   void* k;
   void* v;
   int page_size, num_pages, group, writes;
+  float* k_scale;               // [pages][kv heads], null: pages of the activations' type
+  float* v_scale;
+  void* k_wide;
+  void* v_wide;
+};
+
+// A rotary encoding that the kernel of cache8.cu applies.
+struct GlintRope {
+  const double* turns;          // [rotary_dim / 2] turns per position
+  int rotary_dim;
+  int interleaved;              // pairs (2 j, 2 j + 1) instead of (j, j + rotary_dim / 2)
+  float amplitude;              // of the rotated dims
+  int only;                     // 1: always this kernel (interleaved pairs or an amplitude: no other takes them)
 };
 
 // The table of rotation angles of one rotary encoding: filled at most once per step.
@@ -112,7 +126,13 @@ int glint_op_linear(const GlintRuntime* rt, const void* a, const void* w, void* 
 // q, k, v = x w^T, rotary encoding of q and k, q to q_out, k and v into the pages of `view`.
 int glint_op_qkv_rope(const GlintRuntime* rt, const GlintStep* step, const void* x, const void* w, void* q_out,
                       float* qkv_tmp, const GlintView* view, int nh, int nkv, int hd, int K, const float* inv_freq,
-                      float factor, int rotary_dim, GlintTrigTable* trig, cudaStream_t stream);
+                      float factor, int rotary_dim, GlintTrigTable* trig, const GlintRope* rope, cudaStream_t stream);
+// The same for a finished product, with the kernel that takes every rotary form and either kind of pages.
+int glint_op_rope_append(const GlintRuntime* rt, const GlintStep* step, const float* qkv, void* q_out,
+                         const GlintView* view, int nh, int nkv, int hd, const GlintRope* rope, cudaStream_t stream);
+// Widens the pages of `view` that the step's tokens can reach through `window` (0: all before them) into its wide pools.
+int glint_op_cache8_unpack(const GlintRuntime* rt, const GlintStep* step, const GlintView* view, int nkv, int hd, int window,
+                           cudaStream_t stream);
 // Rotary encoding of a finished q/k/v product and the cache write (the second half of the two-kernel path).
 int glint_op_rope_store(const GlintRuntime* rt, const GlintStep* step, const float* qkv, void* q_out,
                         const GlintView* view, int nh, int nkv, int hd, const float* inv_freq, float factor,

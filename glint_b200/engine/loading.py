@@ -14,19 +14,20 @@ from .model import CausalLM
 from .step import Engine
 
 
-def load_model(model_dir, dtype="bfloat16", device="cuda:0", kernels="auto"):
+def load_model(model_dir, dtype="bfloat16", device="cuda:0", kernels="auto", cache_dtype=None):
     config = load_config(model_dir)
-    rt = Runtime(device, dtype, kernels)
+    rt = Runtime(device, dtype, kernels, cache_dtype)
     model = CausalLM(config.model_spec(), rt)
     model.config = config
     return load_weights(model, model_dir)
 
 
-def random_model(config, seed=0, std=0.02, norm_std=0.1, dtype="bfloat16", device="cuda:0", kernels="auto"):
+def random_model(config, seed=0, std=0.02, norm_std=0.1, dtype="bfloat16", device="cuda:0", kernels="auto",
+                 cache_dtype=None):
     """A model of ``config`` (typed, or a config.json dict) with random weights made on the device."""
     if isinstance(config, dict):
         config = config_from_dict(config)
-    rt = Runtime(device, dtype, kernels)
+    rt = Runtime(device, dtype, kernels, cache_dtype)
     model = CausalLM(config.model_spec(), rt)
     model.config = config
     return fill_random(model, seed, std, norm_std)

@@ -59,7 +59,19 @@ class RuntimeStruct(Structure):
 
 class ViewStruct(Structure):
     _fields_ = [("k", c_void_p), ("v", c_void_p), ("page_size", c_int), ("num_pages", c_int), ("group", c_int),
-                ("writes", c_int)]
+                ("writes", c_int), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_wide", c_void_p),
+                ("v_wide", c_void_p)]
+
+
+class RopeStruct(Structure):
+    """``GlintRope`` of csrc/runtime.h."""
+    _fields_ = [("turns", c_void_p), ("rotary_dim", c_int), ("interleaved", c_int), ("amplitude", c_float),
+                ("only", c_int)]
+
+
+def rope_struct(turns, interleaved=False, amplitude=1.0, only=False):
+    """A rotary encoding for the kernel that takes every form: ``turns`` float64 [rotary_dim / 2] on the device."""
+    return RopeStruct(turns.data_ptr(), 2 * turns.numel(), 1 if interleaved else 0, float(amplitude), 1 if only else 0)
 
 
 class TrigStruct(Structure):
@@ -230,6 +242,9 @@ class Program:
             s.page_size, s.num_pages = view.page_size, view.num_pages
             s.group = next(i for i, g in enumerate(self.groups) if g is view.group)
             s.writes = 1 if view.writes else 0
+            if getattr(view, "k_scale", None) is not None:       # pages of codes, with scratch for one wide layer
+                s.k_scale, s.v_scale = view.k_scale.data_ptr(), view.v_scale.data_ptr()
+                s.k_wide, s.v_wide = view.k_wide.data_ptr(), view.v_wide.data_ptr()
             self._views[id(view)] = s
             self._keep.append((s, view))
         return ctypes.addressof(s)
@@ -291,11 +306,13 @@ class Program:
                   (1 if out.dtype == torch.bfloat16 else 0, N, w.shape[1], 1 if gated else 0,
                    ops.ACTIVATIONS[gated] if gated else 0), (cap or 0.0,))
 
-    def qkv_rope(self, x, w_qkv, q_out, tmp, view, nh, nkv, hd, inv_freq, factor, rotary_dim, trig):
-        self._keep.append(trig)
+    def qkv_rope(self, x, w_qkv, q_out, tmp, view, nh, nkv, hd, inv_freq, factor, rotary_dim, trig, rope=None):
+        """``rope`` (a ``RopeStruct``): what coded pages, interleaved pairs and an amplitude are encoded with."""
+        self._keep.append((trig, rope))
         self._add(OP_QKV_ROPE, 0, (x.ptr, w_qkv.data_ptr(), q_out.ptr, tmp.ptr if tmp is not None else 0,
                                    self.view_struct(view), inv_freq.data_ptr(),
-                                   ctypes.addressof(trig.struct) if trig is not None else 0),
+                                   ctypes.addressof(trig.struct) if trig is not None else 0,
+                                   ctypes.addressof(rope) if rope is not None else 0),
                   (nh, nkv, hd, w_qkv.shape[1], rotary_dim), (factor,))
 
     def rope_store(self, qkv, q_out, view, nh, nkv, hd, inv_freq, factor, rotary_dim):

@@ -57,6 +57,7 @@ _CORE_SIGNATURES = {
     "glint_add_rmsnorm": [_P, _P, _P, _F, _F, _P, _I, _P, _F, _F, _I, _I, _P],
     "glint_rope_table": [_P, _P, _F, _P, _I, _I, _P],
     "glint_rope_kv_write": [_P, _P, _P, _P, _I, _P, _F, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "glint_rope_append": [_P, _P, _P, _P, _I, _P, _I, _I, _F, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
     "glint_gated_act": [_P, _P, _I, _I, _I, _I, _P],
     "glint_softcap": [_P, _L, _F, _P],
     "glint_place_tokens": [_P, _P, _P, _P, _I, _P],
@@ -174,6 +175,28 @@ def rope_kv_write(qkv, positions, token_slot, block_table, inv_freq, factor, rot
                                      block_table.shape[1], ptr(inv_freq), factor, rot, ptr(q_out), ptr(k_pool),
                                      ptr(v_pool), dtype_code(q_out.dtype), T, nh, nkv, hd, page_size, num_pages,
                                      ptr(status), stream()), "rope_kv_write")
+
+
+def rope_append(qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_pool, nh, nkv, hd, page_size, num_pages,
+                status, k_scale=None, v_scale=None, interleaved=False, amplitude=1.0):
+    """``rope_kv_write`` for every rotary form and either kind of pages: the first ``2 * len(turns)`` dims of a head are
+    turned by ``positions * turns`` (float64) of a full turn, in pairs (j, j + half) or, ``interleaved``, (2j, 2j + 1),
+    and scaled by ``amplitude``; with scales the pools are uint8 and the pages coded (``ops_cache8``), else they
+    are of ``q_out``'s dtype.  ``k_pool`` None: q only."""
+    T = qkv.shape[0]
+    require(qkv, torch.float32, "qkv"); require(positions, torch.int32, "positions")
+    require(token_seq, torch.int32, "token_seq"); require(block_table, torch.int32, "block_table")
+    require(turns, torch.float64, "turns"); require(q_out, None, "q_out")
+    pool = torch.uint8 if k_scale is not None else q_out.dtype
+    require(k_pool, pool, "k_pool"); require(v_pool, pool, "v_pool")
+    require(k_scale, torch.float32, "k_scale"); require(v_scale, torch.float32, "v_scale")
+    if qkv.shape[1] != (nh + 2 * nkv) * hd or 2 * turns.numel() > hd or q_out.numel() != T * nh * hd:
+        raise KernelError(f"rope_append shapes do not fit: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)}, "
+                          f"{turns.numel()} pairs, heads {nh}/{nkv} x {hd}")
+    check(core().glint_rope_append(ptr(qkv), ptr(positions), ptr(token_seq), ptr(block_table), block_table.shape[1],
+                                   ptr(turns), 2 * turns.numel(), int(bool(interleaved)), amplitude, ptr(q_out),
+                                   dtype_code(q_out.dtype), ptr(k_pool), ptr(v_pool), ptr(k_scale), ptr(v_scale), T, nh,
+                                   nkv, hd, page_size, num_pages, ptr(status), stream()), "rope_append")
 
 
 def rope_table(positions, inv_freq, factor, out):

@@ -1,0 +1,212 @@
+"""Python face of the key/value cache held in 8 bits (csrc/cache8.cu): rotate and append, widen, attend.
+
+A page holds ``page_size`` tokens of one kv head as codes of 8 bits with one scale ``s`` (a power of two), for keys
+and for values each: code ``c`` stands for ``(c - 127.5) * s`` and is made by ``floor(x / s) + 128``.  A page's scale
+is the smallest that holds its largest magnitude below ``128 s``; when a later token needs a larger one, the codes
+before it are shifted, which gives exactly the codes they would have got at once.  So a page depends on its tokens
+only, not on how they were cut into steps; a value is off by at most half a step, and is exact in bfloat16.
+
+The calls launch on the current stream of the runtime's device, with the kernels the runtime chooses.  ``Cache8`` and
+``StepArrays`` are made once for a layer's pages and a step's arrays and only point at them: what the arrays hold is
+read by the kernels.  The wide pools of a ``Cache8`` are scratch for the attention of portions: two streams
+must not use one ``Cache8`` at the same time.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import POINTER, byref, c_float, c_int, c_void_p
+from dataclasses import dataclass
+
+import torch
+
+from . import native, ops
+from .errors import KernelError
+
+LAYOUTS = {"half": False, "interleaved": True}
+
+_routed = None
+
+
+def _lib():
+    """The core library with the routed operations of the coded cache typed."""
+    global _routed
+    if _routed is None:
+        lib = native.lib()
+        step, view, rope = POINTER(native.StepStruct), POINTER(native.ViewStruct), POINTER(native.RopeStruct)
+        lib.glint_op_rope_append.argtypes = [c_void_p, step, c_void_p, c_void_p, view, c_int, c_int, c_int, rope, c_void_p]
+        lib.glint_op_cache8_unpack.argtypes = [c_void_p, step, view, c_int, c_int, c_int, c_void_p]
+        lib.glint_op_attention.argtypes = [c_void_p, step, c_void_p, view, c_void_p, c_int, c_int, c_int, c_float, c_float,
+                                           c_int, c_void_p]
+        for f in (lib.glint_op_rope_append, lib.glint_op_cache8_unpack, lib.glint_op_attention):
+            f.restype = c_int
+        _routed = lib
+    return _routed
+
+
+@dataclass
+class Cache8:
+    """One layer's pages: ``k``, ``v`` uint8 [pages, kv heads, page size, head size], ``k_scale``, ``v_scale`` float32
+    [pages, kv heads], and ``k_wide``, ``v_wide``, scratch of the codes' shape in the runtime's dtype.  The wide pools
+    have to be finite when the cache is made (zeros)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    k_wide: torch.Tensor
+    v_wide: torch.Tensor
+
+    def __post_init__(self):
+        for name in ("k", "v"):
+            ops.require(getattr(self, name), torch.uint8, name)
+            ops.require(getattr(self, name + "_scale"), torch.float32, name + "_scale")
+            ops.require(getattr(self, name + "_wide"), self.k_wide.dtype, name + "_wide")
+        if self.k.dim() != 4 or min(self.k.shape) < 1:
+            raise KernelError(f"a coded cache is [pages, kv heads, page size, head size], not {tuple(self.k.shape)}")
+        self.num_pages, self.nkv, self.page_size, self.hd = self.k.shape
+        for name, shape in (("v", self.k.shape), ("k_scale", self.k.shape[:2]), ("v_scale", self.k.shape[:2]),
+                            ("k_wide", self.k.shape), ("v_wide", self.k.shape)):
+            if tuple(getattr(self, name).shape) != tuple(shape):
+                raise KernelError(f"{name} {tuple(getattr(self, name).shape)} does not fit codes {tuple(self.k.shape)}")
+        if self.hd % 2:
+            raise KernelError(f"a coded cache takes even head sizes, not {self.hd}")
+        if any(t.device != self.k.device for t in (self.v, self.k_scale, self.v_scale, self.k_wide, self.v_wide)):
+            raise KernelError("the tensors of a coded cache belong to one device")
+        self.struct = native.ViewStruct(self.k.data_ptr(), self.v.data_ptr(), self.page_size, self.num_pages, 0, 1,
+                                        self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.k_wide.data_ptr(),
+                                        self.v_wide.data_ptr())
+
+    @classmethod
+    def empty(cls, num_pages, num_kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda:0"):
+        """A cache that holds nothing yet."""
+        shape = (num_pages, num_kv_heads, page_size, head_dim)
+        made = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2)]
+        made += [torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)]
+        made += [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
+        return cls(*made)
+
+
+class StepArrays:
+    """The arrays of a step (int32, on the device) for calls that bring their own: ``positions`` and ``token_seq`` per
+    token (a request's tokens stand together, in ascending positions; requests in the order of their rows), ``seq_start``
+    (tokens cached before the step) and ``cu_seqlens`` (token offsets, one more) per request, ``block_table``
+    [requests, pages].  ``max_seq_len`` is the most tokens of a request, ``max_context`` at least the largest position
+    plus one; ``contexts``: the contexts of the requests in front that bring a single token, for planning launches.
+    ``begin()`` starts a new step: the arrays may hold other values, and what was planned for the old ones is not used."""
+
+    def __init__(self, positions, token_seq, seq_start, cu_seqlens, block_table, max_seq_len, max_context, contexts=()):
+        from .engine.step import _uneven
+        named = {"positions": positions, "token_seq": token_seq, "seq_start": seq_start, "cu_seqlens": cu_seqlens,
+                 "block_table": block_table}
+        for name, t in named.items():
+            ops.require(t, torch.int32, name)
+            if t.device != positions.device:
+                raise KernelError(f"{name} belongs to another device than positions")
+        T, R = positions.numel(), seq_start.numel()
+        if block_table.dim() != 2 or block_table.shape[0] != R or cu_seqlens.numel() != R + 1 or token_seq.numel() != T:
+            raise KernelError(f"step arrays do not fit: {T} positions, {token_seq.numel()} token rows, {R} requests, "
+                              f"{cu_seqlens.numel()} offsets, block table {tuple(block_table.shape)}")
+        if T and not (1 <= max_seq_len <= T and max_context >= max_seq_len and R >= 1):
+            raise KernelError(f"max_seq_len {max_seq_len} and max_context {max_context} do not fit {T} tokens")
+        if len(contexts) > R:
+            raise KernelError(f"{len(contexts)} contexts for {R} requests")
+        self.tensors, self.num_tokens, self.device = named, T, positions.device
+        contexts = [int(c) for c in contexts]
+        s = self.struct = native.StepStruct()
+        s.num_tokens, s.num_seqs, s.max_seq_len, s.max_context = T, R, int(max_seq_len), int(max_context)
+        s.leading_single, s.leading_single_context = (R if max_seq_len == 1 else len(contexts)), max(contexts or [0])
+        s.uneven = _uneven(contexts)
+        s.num_groups = 1
+        s.positions, s.token_seq = positions.data_ptr(), token_seq.data_ptr()
+        s.seq_start, s.cu_seqlens = seq_start.data_ptr(), cu_seqlens.data_ptr()
+        s.block_table[0], s.max_pages[0] = block_table.data_ptr(), block_table.shape[1]
+        self.begin()
+
+    def begin(self):
+        self.struct.id = native.next_step_id()
+
+
+def _check(rt, cache, step, window=0):
+    if cache.k_wide.dtype != rt.dtype:
+        raise KernelError(f"the wide pools are {cache.k_wide.dtype}, the runtime is {rt.dtype}")
+    if cache.k.device != rt.device or step.device != rt.device:
+        raise KernelError(f"the cache ({cache.k.device}), the step ({step.device}) and the runtime ({rt.device}) belong to "
+                          f"one device")
+    if window < 0:
+        raise KernelError(f"a window of {window} tokens")
+    if step.struct.max_context > step.struct.max_pages[0] * cache.page_size:
+        raise KernelError(f"a context of {step.struct.max_context} exceeds the block table of {step.struct.max_pages[0]} "
+                          f"pages of {cache.page_size}")
+
+
+def _rows(t, rows, width, dtype, name):
+    ops.require(t, dtype, name)
+    if t.dim() != 2 or tuple(t.shape) != (rows, width):
+        raise KernelError(f"{name} {tuple(t.shape)} is not [{rows}, {width}]")
+
+
+def _run(rc, what):
+    if rc != 0:
+        raise KernelError(f"{what}: {ops.error_string(rc)} (code {rc})")
+
+
+def _heads(num_heads, cache):
+    if num_heads < 1 or num_heads % cache.nkv:
+        raise KernelError(f"{num_heads} query heads do not share {cache.nkv} kv heads evenly")
+
+
+def append(rt, cache, step, qkv, turns, num_heads, q_out=None, layout="half", amplitude=1.0):
+    """Rotate the queries and keys of a finished product ``qkv`` float32 [tokens, (heads + 2 kv heads) * head size], write
+    the queries to ``q_out`` (made here in the runtime's dtype unless given; returned) and code keys and values into
+    their pages.  ``turns`` float64 [pairs]: turns per position of the first ``2 pairs`` dims of a head, which are
+    paired (j, j + pairs) in the layout "half" and (2j, 2j + 1) in the layout "interleaved"; the angles are computed
+    in 64 bits.  ``amplitude`` scales the turned dims.  A key or value that is not finite makes its page's scale NaN."""
+    _check(rt, cache, step)
+    _heads(num_heads, cache)
+    if layout not in LAYOUTS:
+        raise KernelError(f"rotary layout {layout!r} is none of {sorted(LAYOUTS)}")
+    T, hd = step.num_tokens, cache.hd
+    _rows(qkv, T, (num_heads + 2 * cache.nkv) * hd, torch.float32, "qkv")
+    ops.require(turns, torch.float64, "turns")
+    if turns.dim() != 1 or 2 * turns.numel() > hd:
+        raise KernelError(f"turns {tuple(turns.shape)} do not fit heads of {hd}")
+    if q_out is None:
+        q_out = torch.empty((T, num_heads * hd), dtype=rt.dtype, device=rt.device)
+    _rows(q_out, T, num_heads * hd, rt.dtype, "q_out")
+    if qkv.device != rt.device or q_out.device != rt.device or turns.device != rt.device:
+        raise KernelError(f"qkv, turns and q_out belong to the runtime's device {rt.device}")
+    rope = native.rope_struct(turns, LAYOUTS[layout], amplitude)
+    with torch.cuda.device(rt.device):
+        _run(_lib().glint_op_rope_append(ctypes.addressof(rt.native), byref(step.struct), ops.ptr(qkv), ops.ptr(q_out),
+                                         byref(cache.struct), num_heads, cache.nkv, hd, byref(rope), ops.stream()),
+             "cache8 append")
+    return q_out
+
+
+def unpack(rt, cache, step, window=0):
+    """The values of every page that the step's tokens can reach (through ``window``, or all before them), at the same
+    places of the wide pools (returned); other places are left as they were."""
+    _check(rt, cache, step, window or 0)
+    with torch.cuda.device(rt.device):
+        _run(_lib().glint_op_cache8_unpack(ctypes.addressof(rt.native), byref(step.struct), byref(cache.struct), cache.nkv,
+                                           cache.hd, int(window or 0), ops.stream()), "cache8 unpack")
+    return cache.k_wide, cache.v_wide
+
+
+def attention(rt, cache, step, q, num_heads, multiplier, softcap=0.0, window=0, out=None):
+    """Attention of the step's queries ``q`` [tokens, heads * head size] (the runtime's dtype) over the coded pages, keys
+    and values of the step among them: scores times ``multiplier``, soft cap, keys of the last ``window`` positions (0:
+    all).  Returns ``out`` [tokens, heads * head size]."""
+    _check(rt, cache, step, window or 0)
+    _heads(num_heads, cache)
+    T, hd = step.num_tokens, cache.hd
+    _rows(q, T, num_heads * hd, rt.dtype, "q")
+    if out is None:
+        out = torch.empty_like(q)
+    _rows(out, T, num_heads * hd, rt.dtype, "out")
+    if q.device != rt.device or out.device != rt.device:
+        raise KernelError(f"q and out belong to the runtime's device {rt.device}")
+    with torch.cuda.device(rt.device):
+        _run(_lib().glint_op_attention(ctypes.addressof(rt.native), byref(step.struct), ops.ptr(q), byref(cache.struct),
+                                       ops.ptr(out), num_heads, cache.nkv, hd, multiplier, softcap or 0.0, int(window or 0),
+                                       ops.stream()), "cache8 attention")
+    return out

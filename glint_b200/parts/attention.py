@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from ..cache import PagedKVNeed
+from ..cache import CodedKVNeed, PagedKVNeed
 from .base import Part, TensorNeed, run_lowered
 from .registry import build_part, register_part
 
@@ -40,7 +40,8 @@ class Attention(Part):
         return self.num_kv_heads * self.head_dim
 
     def cache_need(self):
-        return PagedKVNeed(self.num_kv_heads, self.head_dim, self.window)
+        kind = CodedKVNeed if getattr(self.rt, "cache_dtype", None) == "int8" else PagedKVNeed
+        return kind(self.num_kv_heads, self.head_dim, self.window)
 
     def needs(self):
         n = self.names
@@ -99,7 +100,7 @@ class Attention(Part):
         return 4 * self.num_heads * self.head_dim * self.keys_read(start, n)
 
     def cache_read_bytes(self, position, element_size):
-        return self.keys_read(position, 1) * 2 * self.num_kv_heads * self.head_dim * element_size
+        return self.keys_read(position, 1) * self.cache_need().bytes_per_token(element_size)
 
 
 register_part("mixer", "attention", Attention)

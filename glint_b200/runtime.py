@@ -12,7 +12,8 @@ DTYPES = {"float32": torch.float32, "fp32": torch.float32, "f32": torch.float32,
 _STATUS_TEXT = {1: "a token id lies outside the embedding table",
                 2: "a token's position has no page in its block table (cache write)",
                 3: "a key's position has no page in its block table (attention read)",
-                4: "a bounded device-side wait ran out"}
+                4: "a bounded device-side wait ran out",
+                5: "a request's tokens do not stand together in ascending positions (cache write)"}
 
 
 def parse_dtype(dtype):
@@ -26,13 +27,23 @@ def parse_dtype(dtype):
         raise KernelError(f"unknown dtype '{dtype}' (known: float32, bfloat16)") from None
 
 
+def parse_cache_dtype(cache_dtype):
+    if cache_dtype in (None, "auto"):
+        return None
+    if cache_dtype == "int8":
+        return "int8"
+    raise KernelError(f"unknown cache dtype '{cache_dtype}' (known: auto, int8)")
+
+
 class Runtime:
     """``dtype`` float32 means the true 32-bit path: CUDA-core products, no tensor cores.
-    ``kernels`` is 'auto' (tensor-core kernels where they exist, for bfloat16) or 'plain'."""
+    ``kernels`` is 'auto' (tensor-core kernels where they exist, for bfloat16) or 'plain'.  ``cache_dtype`` is what
+    attention keeps keys and values in: None (``dtype``) or 'int8' (codes of 8 bits, see ``ops_cache8``)."""
 
-    def __init__(self, device="cuda:0", dtype=torch.bfloat16, kernels="auto"):
+    def __init__(self, device="cuda:0", dtype=torch.bfloat16, kernels="auto", cache_dtype=None):
         self.device = torch.device(device)
         self.dtype = parse_dtype(dtype)
+        self.cache_dtype = parse_cache_dtype(cache_dtype)
         if kernels not in ("auto", "plain"):
             raise KernelError(f"kernels must be 'auto' or 'plain', not '{kernels}'")
         self.kernels = kernels
