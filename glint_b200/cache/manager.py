@@ -112,7 +112,8 @@ class PagedKVNeed(PagedNeed):
 class CodedKVNeed(PagedKVNeed):
     """Keys and values in codes of 8 bits with a scale per page and kv head (csrc/cache8.cu), in the same places as
     ``PagedKVNeed``'s.  A group also keeps one layer's worth of wide pages in the engine's dtype, which the
-    attention of prompt portions reads (all layers take turns: a step's kernels run in order on one stream)."""
+    attention of prompt portions reads, and scratch for single tokens (all layers take turns: a step's kernels run
+    in order on one stream)."""
 
     def group_key(self):
         return ("coded",) + super().group_key()
@@ -125,12 +126,13 @@ class CodedKVNeed(PagedKVNeed):
         codes = [torch.zeros((layers,) + one, dtype=torch.uint8, device=device) for _ in range(2)]
         scales = [torch.zeros((layers,) + one[:2], dtype=torch.float32, device=device) for _ in range(2)]
         wide = [torch.zeros(one, dtype=dtype, device=device) for _ in range(2)]
-        return (*codes, *scales, *wide)
+        from ..native import cache8_scratch
+        return (*codes, *scales, *wide, cache8_scratch(self.num_kv_heads, self.head_dim, device))
 
     def view(self, storage, layer):
         v = LayerView()
         v.k, v.v, v.k_scale, v.v_scale = (t[layer] for t in storage[:4])
-        v.k_wide, v.v_wide = storage[4:]
+        v.k_wide, v.v_wide, v.scratch = storage[4:]
         return v
 
     def bytes_per_token(self, element_size):

@@ -292,20 +292,45 @@ static int decode_attention(const GlintRuntime* rt, const GlintStep* step, const
                                     stream));
 }
 
+// Attention over coded pages.  Single tokens (all, or those in front of portions) read the codes; portions read wide
+// pages, which a kernel in front writes once for all their query tiles: inside the tiled kernel every block of 128 query
+// rows would widen the same keys again.  Sizes that no tensor-core kernel takes are widened whole.
+static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const void* q, const GlintView* view, void* out,
+                           int nh, int nkv, int hd, float multiplier, float cap, int window, cudaStream_t stream) {
+  const GlintTensorEntries& t = rt->tensor;
+  const int page = view->page_size, g = view->group, blocks = 2 * rt->sms;
+  const bool single = rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_decode8 && view->partials && view->arrive &&
+                      t.attention_decode8_supported(nh, nkv, hd, page) &&
+                      t.attention_decode8_workspace(blocks, nh, nkv, hd) <= view->partial_floats;
+  const int lead = !single ? 0 : step->max_seq_len == 1 ? step->num_tokens : step->leading_single;
+  if (lead > 0) {
+    const int rc = counted(t.attention_decode8(
+        q, (const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale, step->positions, step->token_seq,
+        step->block_table[g], step->max_pages[g], out, lead, nh, nkv, hd, page, view->num_pages, multiplier, cap, window,
+        step->max_context, blocks, view->partials, view->arrive, view->arrive_ints, rt->status, stream));
+    if (rc != GLINT_OK || lead == step->num_tokens) return rc;
+  }
+  GlintStep rest = *step;                        // the requests behind; their tokens keep their absolute offsets
+  rest.num_seqs -= lead;
+  rest.cu_seqlens += lead;
+  rest.seq_start += lead;
+  rest.block_table[g] += (size_t)lead * step->max_pages[g];
+  rest.leading_single = rest.leading_single_context = rest.uneven = 0;
+  const int rc = glint_op_cache8_unpack(rt, &rest, view, nkv, hd, window, stream);
+  if (rc != GLINT_OK) return rc;
+  GlintView wide = *view;
+  wide.k = view->k_wide;
+  wide.v = view->v_wide;
+  wide.k_scale = wide.v_scale = nullptr;
+  return glint_op_attention(rt, lead ? &rest : step, q, &wide, out, nh, nkv, hd, multiplier, cap, window, stream);
+}
+
 extern "C" int glint_op_attention(const GlintRuntime* rt, const GlintStep* step, const void* q, const GlintView* view,
                                   void* out, int nh, int nkv, int hd, float multiplier, float cap, int window,
                                   cudaStream_t stream) {
   const int T = step->num_tokens;
   if (T <= 0) return GLINT_OK;
-  if (view->k_scale) {
-    const int rc = glint_op_cache8_unpack(rt, step, view, nkv, hd, window, stream);
-    if (rc != GLINT_OK) return rc;
-    GlintView wide = *view;
-    wide.k = view->k_wide;
-    wide.v = view->v_wide;
-    wide.k_scale = wide.v_scale = nullptr;
-    return glint_op_attention(rt, step, q, &wide, out, nh, nkv, hd, multiplier, cap, window, stream);
-  }
+  if (view->k_scale) return coded_attention(rt, step, q, view, out, nh, nkv, hd, multiplier, cap, window, stream);
   const int g = view->group;
   const int* table = step->block_table[g];
   const int max_pages = step->max_pages[g];

@@ -51,6 +51,11 @@ struct GlintTensorEntries {
   int (*attention_decode_stream)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*,
                                  int, int, int, int, int, int, float, float, int, int, const void*, float*, int*, int,
                                  int*, cudaStream_t);
+  int (*attention_decode8)(const void*, const uint8_t*, const uint8_t*, const float*, const float*, const int*, const int*,
+                           const int*, int, void*, int, int, int, int, int, int, float, float, int, int, int, float*, int*,
+                           int, int*, cudaStream_t);
+  int (*attention_decode8_supported)(int, int, int, int);
+  long long (*attention_decode8_workspace)(int, int, int, int);
   int (*attention_prefill)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int,
                            int, int, int, int, int, int, float, float, int, int*, cudaStream_t);
   int (*attention_tcgen05)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int,
@@ -100,6 +105,10 @@ struct GlintView {
   float* v_scale;
   void* k_wide;
   void* v_wide;
+  float* partials;              // scratch of the single-token attention over codes: partial results, and counters that are
+  long long partial_floats;     // zero between launches
+  int* arrive;
+  int arrive_ints;
 };
 
 // A rotary encoding that the kernel of cache8.cu applies.

@@ -36,7 +36,9 @@ class StepStruct(Structure):
 class TensorEntries(Structure):
     _fields_ = [(name, c_void_p) for name in ("gemm_tcgen05", "gemm_skinny", "gemm_tcgen05_rope", "gemm_skinny_rope",
                                               "attention_decode", "attention_decode_stream_plan",
-                                              "attention_decode_stream", "attention_prefill", "attention_tcgen05")]
+                                              "attention_decode_stream", "attention_decode8",
+                                              "attention_decode8_supported", "attention_decode8_workspace",
+                                              "attention_prefill", "attention_tcgen05")]
 
 
 ATTN_PLANS = 8
@@ -60,7 +62,20 @@ class RuntimeStruct(Structure):
 class ViewStruct(Structure):
     _fields_ = [("k", c_void_p), ("v", c_void_p), ("page_size", c_int), ("num_pages", c_int), ("group", c_int),
                 ("writes", c_int), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_wide", c_void_p),
-                ("v_wide", c_void_p)]
+                ("v_wide", c_void_p), ("partials", c_void_p), ("partial_floats", c_longlong), ("arrive", c_void_p),
+                ("arrive_ints", c_int)]
+
+
+CACHE8_ARRIVE = 65536        # pairs of a token and a kv head that one launch of the single-token attention over codes takes
+
+
+def cache8_scratch(num_kv_heads, head_dim, device):
+    """Scratch of the single-token attention over coded pages, for up to 8 query heads a pair and two blocks per SM:
+    (partial results float32, arrival counters int32, zero between launches).  It belongs to one cache, like the wide pages:
+    launches on one stream share it."""
+    blocks = 2 * torch.cuda.get_device_properties(device).multi_processor_count if torch.device(device).type == "cuda" else 1
+    return (torch.empty(blocks * 2 * 8 * (head_dim + 4), dtype=torch.float32, device=device),
+            torch.zeros(CACHE8_ARRIVE, dtype=torch.int32, device=device))
 
 
 class RopeStruct(Structure):
@@ -245,6 +260,9 @@ class Program:
             if getattr(view, "k_scale", None) is not None:       # pages of codes, with scratch for one wide layer
                 s.k_scale, s.v_scale = view.k_scale.data_ptr(), view.v_scale.data_ptr()
                 s.k_wide, s.v_wide = view.k_wide.data_ptr(), view.v_wide.data_ptr()
+                partials, arrive = view.scratch
+                s.partials, s.partial_floats = partials.data_ptr(), partials.numel()
+                s.arrive, s.arrive_ints = arrive.data_ptr(), arrive.numel()
             self._views[id(view)] = s
             self._keep.append((s, view))
         return ctypes.addressof(s)

@@ -8,8 +8,8 @@ only, not on how they were cut into steps; a value is off by at most half a step
 
 The calls launch on the current stream of the runtime's device, with the kernels the runtime chooses.  ``Cache8`` and
 ``StepArrays`` are made once for a layer's pages and a step's arrays and only point at them: what the arrays hold is
-read by the kernels.  The wide pools of a ``Cache8`` are scratch for the attention of portions: two streams
-must not use one ``Cache8`` at the same time.
+read by the kernels.  A ``Cache8`` holds scratch (the wide pools for portions, partial results for single tokens): calls on
+one ``Cache8`` belong on one stream, or on streams that wait for each other, graphs among them.
 """
 from __future__ import annotations
 
@@ -71,9 +71,11 @@ class Cache8:
             raise KernelError(f"a coded cache takes even head sizes, not {self.hd}")
         if any(t.device != self.k.device for t in (self.v, self.k_scale, self.v_scale, self.k_wide, self.v_wide)):
             raise KernelError("the tensors of a coded cache belong to one device")
+        self.scratch = partials, arrive = native.cache8_scratch(self.nkv, self.hd, self.k.device)
         self.struct = native.ViewStruct(self.k.data_ptr(), self.v.data_ptr(), self.page_size, self.num_pages, 0, 1,
                                         self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.k_wide.data_ptr(),
-                                        self.v_wide.data_ptr())
+                                        self.v_wide.data_ptr(), partials.data_ptr(), partials.numel(), arrive.data_ptr(),
+                                        arrive.numel())
 
     @classmethod
     def empty(cls, num_pages, num_kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda:0"):

@@ -219,6 +219,12 @@ def test_what_is_not_finite_reaches_its_own_request_only(rts, bad, place):
         q = torch.randn(60, nh * hd, generator=torch.Generator().manual_seed(1)).to(DEV, torch.bfloat16)
         s.step.begin()
         outs.append(ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.125).float().cpu().view(60, nh, hd))
+        # the same as single tokens: the last token of each request
+        one = ops_cache8.StepArrays(*[torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([19, 39], [0, 1], [19, 39], [0, 1, 2])],
+                                    s.step.tensors["block_table"], 1, 40, contexts=[20, 40])
+        single = ops_cache8.attention(rt, s.cache, one, q[[19, 59]].contiguous(), nh, 0.125).float().cpu().view(2, nh, hd)
+        assert bool(torch.isnan(single[0, 2:]).all()) == poison and torch.isfinite(single[0, :2]).all()
+        assert torch.isfinite(single[1]).all()
         if poison:
             again = Setup(rt, [4], [16], nkv, hd, 16, seed=2)
             step = ops_cache8.StepArrays(*[again.step.tensors[n] for n in ("positions", "token_seq", "seq_start", "cu_seqlens")],
