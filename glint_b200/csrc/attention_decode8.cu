@@ -4,19 +4,21 @@
 // The pages of all pairs, in order, are one sequence; block b of two per SM takes units [b W, (b + 1) W) of it,
 // whatever pairs they belong to (a unit is a page; every pair is preceded by `pair_cost` empty units that stand for
 // what a pair costs a block beside its pages).  Every block finds W and where it begins by itself, from the
-// positions: no launch goes before this one.  A producer warp streams the pages into a ring of shared-memory stages
-// (TMA boxes with the 128-byte swizzle, completion on an mbarrier) with each page's two scales beside them; the
-// consumer warps take the pages in turn.  A pair that lies inside one block is finished there; of a shared pair every
-// block leaves a partial result in a workspace and the last one to arrive adds them up, in block order.
+// positions: no launch goes before this one.  The warps take the block's pages in turn; each fills its own stages of a
+// ring in shared memory (TMA boxes with the 128-byte swizzle, completion on an mbarrier) as soon as it has read them:
+// one producer warp for all cannot issue pages of 4 KB fast enough.  A pair that lies inside one block is finished
+// there; of a shared pair every block leaves a partial result in a workspace and the last one to arrive adds them up,
+// in block order.
 //
-// Per 16 keys: scores^T = K q^T and out^T += V^T p^T with mma.sync m16n8k16 tiles in half precision, in which N
-// (8) holds the query heads of the group.  Codes become half-precision integers c - 128 by one byte permutation (the
-// byte under an exponent of 2^10) and one subtraction, both exact; the half that a code's middle lies above c - 128
-// enters through the accumulators: 0.5 sum(q) for the scores and 0.5 sum(p) for the values.  Queries are scaled by a
-// power of two so that their largest element lies in [2^8, 2^9): bfloat16 queries are then exact down to 2^-24 of
-// it.  A page's key scale multiplies its scores; its value scale goes into the probabilities (times 2^10, rounded to the
-// 11 bits of a half) as its ratio to a reference scale, which the accumulators follow when the ratio leaves
-// [2^-5, 2^5].  Scores, soft cap, maxima, sums and accumulators are 32-bit.
+// Per 16 keys: scores^T = K q^T with mma.sync m16n8k32 over the codes themselves, in which N (8) holds the query heads of
+// the group.  Queries become 16-bit integers (a power of two brings the largest element below 2^15: a bfloat16 query
+// is then exact down to 2^-7 of it, and off by at most 2^-15 of it below), whose upper and lower bytes are two B operands;
+// the products are exact integers, -127.5 sum(q) brings the codes' middle in, and the result becomes 32-bit float.
+// out^T += V^T p^T with m16n8k16 in half precision: a byte permutation puts a code under an exponent of 2^10 and one
+// subtraction gives c - 128, both exact; the half that a code stands above c - 128 enters at the end as 0.5 sum(p).
+// A page's key scale multiplies its scores; its value scale goes into the probabilities (times 64, rounded to the 11
+// bits of a half) as its ratio to a reference scale, which the accumulators follow when the ratio leaves [1/8, 8].
+// Scores, soft cap, maxima, sums and accumulators are 32-bit.
 // Score = (q.k) * multiplier, then cap * tanh(score / cap); keys from max(0, pos - window + 1) to pos.
 //
 // No key is masked by zeroing values: codes are finite whatever bytes an unwritten row holds, and so is what
@@ -28,13 +30,15 @@
 
 namespace glint {
 
-constexpr int D8_WARPS = 4;                       // consumer warps; one more warp is the producer
-constexpr int D8_THREADS = D8_WARPS * 32 + 32;
-constexpr int D8_MAX_STAGES = 12;                 // a multiple of the consumer warps (see the kernel)
+constexpr int D8_WARPS = 6;
+constexpr int D8_THREADS = D8_WARPS * 32;
+constexpr int D8_MAX_STAGES = 24;                 // a multiple of the warps (see the kernel)
+constexpr int D8_CHUNK = 128;                     // pages looked up at a time
+constexpr int D8_BLOCK_SMEM = 113 * 1024;         // of an SM's 228 KB: two blocks with 1 KB each of the system's
 constexpr int D8_HEADS = 8;                       // query heads of a pair (the MMA's N); larger groups are several pairs
 constexpr int D8_ROW = 128;                       // bytes of a swizzled row
 constexpr int D8_MAX_TOKENS = 1024;               // of a launch
-constexpr float D8_P_BASE = 1024.f;               // probabilities are multiplied by this before they become halves
+constexpr float D8_P_BASE = 64.f;                 // probabilities are multiplied by this before they become halves
 
 struct Decode8Params {
   const __nv_bfloat16* q;       // [T][nh][hd]
@@ -48,21 +52,21 @@ struct Decode8Params {
   int* arrive;                  // [pairs]: blocks that have left their part; back at 0 after the launch
   int* status;
   float multiplier, cap;
-  int T, nh, nkv, hd, groups, page_size, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units;
+  int T, nh, nkv, hd, groups, page_size, splits, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units;
+};
+
+// Rows that a block reads: the first of them in the pools (-1: none), their scales.
+struct Decode8Entry {
+  int row;
+  float ks, vs;
 };
 
 struct Decode8Shared {
   uint64_t full[D8_MAX_STAGES];
-  uint64_t empty[D8_MAX_STAGES];
-  float2 scale[D8_MAX_STAGES];  // of the page in the stage: keys, values
-  long long warp_sum[D8_THREADS / 32];
-  long long total, W;
-  int start_token, start_inside;
+  Decode8Entry entry[2][D8_CHUNK];
   int abort_flag;
   int last_one;
 };
-
-__device__ __forceinline__ void d8_consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(D8_WARPS * 32) : "memory"); }
 
 __device__ __forceinline__ void d8_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -70,6 +74,31 @@ __device__ __forceinline__ void d8_mma(float* c, uint32_t a0, uint32_t a1, uint3
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// codes times the upper (signed) and lower (unsigned) bytes of 16-bit queries
+__device__ __forceinline__ void d8_mma_hi(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void d8_mma_lo(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void d8_ldsm(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void d8_ldsm_trans(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
 }
 __device__ __forceinline__ uint32_t d8_transpose(uint32_t v) {
   uint32_t r;
@@ -80,7 +109,7 @@ __device__ __forceinline__ uint32_t d8_pack(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Bytes b0, b1 of w (0..3) as the halves c - 128: 0x6400 | c is 1024 + c.
+// Bytes B0, B1 (0..3) of w as the halves c - 128: 0x6400 | c is 1024 + c.
 template <int B0, int B1>
 __device__ __forceinline__ uint32_t d8_halves(uint32_t w) {
   const uint32_t raised = __byte_perm(w, 0x64646464u, B0 | (4 << 4) | (B1 << 8) | (4 << 12));
@@ -97,18 +126,7 @@ __device__ __forceinline__ float d8_rcp(float x) {
   asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint4 d8_lds16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint2 d8_lds8(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-// Byte offset of a 16-byte chunk of a row in a tile of 128-byte rows with the 128-byte swizzle.
-__device__ __forceinline__ uint32_t d8_swz(int row, int chunk) { return (uint32_t)(row * D8_ROW + ((chunk ^ (row & 7)) << 4)); }
+__device__ __forceinline__ float d8_inverse(float power_of_two) { return __int_as_float((254 << 23) - __float_as_int(power_of_two)); }
 
 struct Decode8Segment {
   int first, page_lo, pages;    // of a token: first key, first page, pages
@@ -125,26 +143,33 @@ __device__ __forceinline__ Decode8Segment d8_segment(int pos, int window, int pa
 template <int HD>
 struct Decode8State {
   float o[HD / 16][4];          // sums of (c - 128) p'' in units of `ref`
-  float m[2], l[2], lp[2];      // heads 2 tq, 2 tq + 1: maximum (log2), sum of p, sum of p'' (this thread's keys only)
-  float ref;                    // value scale that o counts in (0: nothing yet)
+  float m[2], l[2], lp[2];      // heads 2 tq, 2 tq + 1: reference of the exponents (log2; within 4 of the maximum), sums of
+                                // p and of p'' (this thread's keys only)
+  float ref;                    // 1 / the value scale that o counts in (0: nothing yet)
 };
 
-// One page of a stage.  Row g of a score tile is key kappa(g) = g / 2 + 4 (g mod 2) of the 16, row g + 8 is
-// key kappa(g) + 8: the eight lanes that a 16-byte shared-memory load serves at a time then hit different banks, for
-// keys (chunks tq of rows p and p + 4) and for values (chunks kappa(g) of rows tq) alike.
+// A pair's queries as this thread's part of the B operand: per 32 dims, the upper and lower bytes of dims
+// 4 tq .. 4 tq + 3 and 16 + 4 tq .. of head g.
 template <int HD>
-__device__ __forceinline__ void d8_page(Decode8State<HD>& st, const uint32_t (&qb)[HD / 16][2], const float (&bias)[2],
-                                        const float (&qscale)[2], uint32_t kbase, uint32_t vbase, float ks, float vs, int page_key0,
-                                        int pos, int first, int page_size, int hd, uint32_t sub_bytes, float cap2, int lane) {
-  constexpr int VW = HD == 64 ? 2 : 4;                         // words of a row of values that a lane holds
-  const int g = lane >> 2, tq = lane & 3;
-  const int kappa = (g >> 1) + 4 * (g & 1);
+struct Decode8Query {
+  uint32_t hi[HD / 32][2], lo[HD / 32][2];
+  int start[2];                 // heads 2 tq, 2 tq + 1: -128 sum(q)
+  float half[2];                // sum(q) / 2
+  float scale[2];               // of a score, without the page's scale
+};
+
+// One page of a stage; kaddr, vaddr: where this lane's rows of 16-byte chunks for ldmatrix begin.
+template <int HD, bool FULL>
+__device__ __forceinline__ void d8_page(Decode8State<HD>& st, const Decode8Query<HD>& qy, uint32_t kaddr, uint32_t vaddr,
+                                        float ks, float vs, int page_key0, int pos, int first, int page_size, int hd,
+                                        uint32_t sub_bytes, float cap2, int lane) {
+  const int g = lane >> 2;
   // The page's value scale against the one that o counts in (the same in all lanes).  Upwards o follows all the way;
-  // downwards by 2^64 at most, so that it cannot overflow: what a page 2^69 smaller still adds is nothing.
-  if (st.ref == 0.f) st.ref = vs;
-  float ratio = vs * (1.f / st.ref);
-  for (int i = 0; ratio > 32.f || (i == 0 && ratio < 0.03125f); ++i) {
-    const int d = max(-64, min(64, ((__float_as_int(st.ref) >> 23) & 255) - ((__float_as_int(vs) >> 23) & 255)));
+  // downwards by 2^64 at most, so that it cannot overflow: what a page 2^67 smaller still adds is nothing.
+  if (st.ref == 0.f) st.ref = d8_inverse(vs);
+  float ratio = vs * st.ref;
+  for (int i = 0; ratio > 8.f || (i == 0 && ratio < 0.125f); ++i) {
+    const int d = max(-64, min(64, 254 - ((__float_as_int(st.ref) >> 23) & 255) - ((__float_as_int(vs) >> 23) & 255)));
     const float f = __int_as_float((127 + d) << 23);
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) {
@@ -153,302 +178,295 @@ __device__ __forceinline__ void d8_page(Decode8State<HD>& st, const uint32_t (&q
     }
     st.lp[0] *= f;
     st.lp[1] *= f;
-    st.ref *= __int_as_float((127 - d) << 23);
-    ratio = vs * (1.f / st.ref);
+    st.ref *= f;
+    ratio = vs * st.ref;
   }
   const float pscale = D8_P_BASE * ratio;
-  for (int tile = 0; tile * 16 < page_size; ++tile) {
-    const int key0 = page_key0 + tile * 16;
+  const float f0 = qy.scale[0] * ks, f1 = qy.scale[1] * ks;
+  for (int key0 = page_key0; key0 < page_key0 + page_size; key0 += 16, kaddr += 16 * D8_ROW, vaddr += 16 * D8_ROW) {
     if (key0 > pos || key0 + 15 < first) continue;             // the whole tile is masked
-    float sc[4] = {bias[0], bias[1], bias[0], bias[1]};
-    const uint32_t krow = kbase + (uint32_t)(tile * 16) * D8_ROW;
+    int hi[4] = {0, 0, 0, 0}, lo[4] = {qy.start[0], qy.start[1], qy.start[0], qy.start[1]};
 #pragma unroll
-    for (int u = 0; u < HD / 64; ++u) {                        // 64 dims: a lane's 16 bytes of rows g and g + 8
-      if (u * 64 < hd) {
-        const uint32_t at = krow + (u >> 1) * sub_bytes + d8_swz(kappa, (u & 1) * 4 + tq);
-        const uint4 a = d8_lds16(at), b = d8_lds16(at + 8 * D8_ROW);
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          d8_mma(sc, d8_halves<0, 1>(aw[j]), d8_halves<0, 1>(bw[j]), d8_halves<2, 3>(aw[j]), d8_halves<2, 3>(bw[j]),
-                 qb[4 * u + j][0], qb[4 * u + j][1]);
+    for (int s = 0; s < HD / 32; ++s) {
+      if (FULL || s * 32 < hd) {
+        uint32_t a[4];
+        d8_ldsm(a, (kaddr + (s >> 2) * sub_bytes) ^ ((s & 3) << 5));
+        d8_mma_hi(hi, a, qy.hi[s][0], qy.hi[s][1]);
+        d8_mma_lo(lo, a, qy.lo[s][0], qy.lo[s][1]);
       }
     }
-    // sc[h]: key kappa, head 2 tq + h;  sc[2 + h]: key kappa + 8
-    const bool inside = key0 >= first && key0 + 15 <= pos;
-    const bool va = inside || (key0 + kappa >= first && key0 + kappa <= pos);
-    const bool vb = inside || (key0 + kappa + 8 >= first && key0 + kappa + 8 <= pos);
-    float corr[2], pp[4];
+    // [h]: key g, head 2 tq + h;  [2 + h]: key g + 8.  In log2 units; with a cap the scale holds 2 log2(e) / cap, and
+    // tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e)).
+    float x[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // log2 units; with a cap, qscale holds 2 log2(e) / cap and tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e))
-      const float f = qscale[h] * ks;
-      float xa = sc[h] * f, xb = sc[2 + h] * f;
-      if (cap2 > 0.f) {
-        xa = cap2 - 2.f * cap2 * d8_rcp(1.f + d8_exp2(xa));
-        xb = cap2 - 2.f * cap2 * d8_rcp(1.f + d8_exp2(xb));
-      }
-      xa = va ? xa : -INFINITY;
-      xb = vb ? xb : -INFINITY;
-      float mx = fmaxf(xa, xb);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float m_new = fmaxf(st.m[h], mx);
-      const float base = m_new == -INFINITY ? 0.f : m_new;
-      corr[h] = d8_exp2(st.m[h] - base);
-      const float pa = d8_exp2(xa - base), pb = d8_exp2(xb - base);
-      st.l[h] = st.l[h] * corr[h] + pa + pb;
-      st.m[h] = m_new;
-      pp[h] = pa * pscale;
-      pp[2 + h] = pb * pscale;
-      st.lp[h] = st.lp[h] * corr[h] + pp[h] + pp[2 + h];
+    for (int i = 0; i < 4; ++i) {
+      x[i] = ((float)(hi[i] * 256 + lo[i]) + qy.half[i & 1]) * ((i & 1) ? f1 : f0);
+      if (cap2 > 0.f) x[i] = fmaf(-2.f * cap2, d8_rcp(1.f + d8_exp2(x[i])), cap2);
     }
-    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+    if (key0 < first || key0 + 15 > pos) {
+      const bool va = key0 + g >= first && key0 + g <= pos, vb = key0 + g + 8 >= first && key0 + g + 8 <= pos;
+      x[0] = va ? x[0] : -INFINITY;
+      x[1] = va ? x[1] : -INFINITY;
+      x[2] = vb ? x[2] : -INFINITY;
+      x[3] = vb ? x[3] : -INFINITY;
+    }
+    // the exponents' reference follows the maximum only when that has grown by more than 4 (p is then at most 16)
+    float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
+    if (__any_sync(0xffffffffu, t0 > st.m[0] + 4.f || t1 > st.m[1] + 4.f)) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+      }
+      const float n0 = fmaxf(st.m[0], t0), n1 = fmaxf(st.m[1], t1);
+      const float c0 = st.m[0] == -INFINITY ? 0.f : d8_exp2(st.m[0] - n0), c1 = st.m[1] == -INFINITY ? 0.f : d8_exp2(st.m[1] - n1);
+      st.m[0] = n0;
+      st.m[1] = n1;
+      st.l[0] *= c0; st.l[1] *= c1;
+      st.lp[0] *= c0; st.lp[1] *= c1;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        st.o[i][0] *= corr[0];
-        st.o[i][1] *= corr[1];
-        st.o[i][2] *= corr[0];
-        st.o[i][3] *= corr[1];
+        st.o[i][0] *= c0;
+        st.o[i][1] *= c1;
+        st.o[i][2] *= c0;
+        st.o[i][3] *= c1;
       }
     }
-    // p^T as the B operand: keys (tq, tq + 4) and (tq + 8, tq + 12) of head g
-    const uint32_t b0 = d8_transpose(d8_pack(pp[0], pp[1])), b1 = d8_transpose(d8_pack(pp[2], pp[3]));
-    const uint32_t vrow = vbase + (uint32_t)(tile * 16) * D8_ROW;
+    const float base0 = st.m[0] == -INFINITY ? 0.f : st.m[0], base1 = st.m[1] == -INFINITY ? 0.f : st.m[1];
+    const float p0 = d8_exp2(x[0] - base0), p1 = d8_exp2(x[1] - base1), p2 = d8_exp2(x[2] - base0), p3 = d8_exp2(x[3] - base1);
+    st.l[0] += p0 + p2;
+    st.l[1] += p1 + p3;
+    st.lp[0] = fmaf(p0 + p2, pscale, st.lp[0]);
+    st.lp[1] = fmaf(p1 + p3, pscale, st.lp[1]);
+    // p''^T as the B operand: keys 2 tq, 2 tq + 1 (and + 8) of head g, by an 8x8 transpose in the warp
+    const uint32_t b0 = d8_transpose(d8_pack(p0 * pscale, p1 * pscale)), b1 = d8_transpose(d8_pack(p2 * pscale, p3 * pscale));
+    // values: the transposed load of 16-bit units gives dims (2 g, 2 g + 1) of keys 2 tq, 2 tq + 1; rows g and g + 8 of
+    // the tile over a chunk of 16 dims are its dims 2 g and 2 g + 1
 #pragma unroll
-    for (int s = 0; s < (HD + 127) / 128; ++s) {
-      if (s * 128 < hd) {
-        // this lane's 16 dims (8 of the 64 when heads are that small) of keys tq, tq + 4, tq + 8, tq + 12
-        uint32_t w[4][VW];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = tq + 4 * k;
-          const uint32_t at = vrow + s * sub_bytes;
-          if (VW == 4) {
-            const uint4 v = d8_lds16(at + d8_swz(row, kappa));
-            w[k][0] = v.x; w[k][1] = v.y; w[k][VW == 4 ? 2 : 0] = v.z; w[k][VW == 4 ? 3 : 1] = v.w;
-          } else {
-            const uint2 v = d8_lds8(at + d8_swz(row, g >> 1) + (g & 1) * 8);
-            w[k][0] = v.x; w[k][1] = v.y;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < VW; ++c) {                         // 4 dims: two tiles of (dim, dim + 1)
-          const uint32_t lo0 = __byte_perm(w[0][c], w[1][c], 0x5140), hi0 = __byte_perm(w[0][c], w[1][c], 0x7362);
-          const uint32_t lo1 = __byte_perm(w[2][c], w[3][c], 0x5140), hi1 = __byte_perm(w[2][c], w[3][c], 0x7362);
-          d8_mma(st.o[s * 8 + 2 * c], d8_halves<0, 1>(lo0), d8_halves<2, 3>(lo0), d8_halves<0, 1>(lo1), d8_halves<2, 3>(lo1), b0, b1);
-          d8_mma(st.o[s * 8 + 2 * c + 1], d8_halves<0, 1>(hi0), d8_halves<2, 3>(hi0), d8_halves<0, 1>(hi1), d8_halves<2, 3>(hi1), b0, b1);
-        }
+    for (int s = 0; s < HD / 32; ++s) {
+      if (FULL || s * 32 < hd) {
+        uint32_t a[4];
+        d8_ldsm_trans(a, (vaddr + (s >> 2) * sub_bytes) ^ ((s & 3) << 5));
+        d8_mma(st.o[2 * s], d8_halves<0, 2>(a[0]), d8_halves<1, 3>(a[0]), d8_halves<0, 2>(a[1]), d8_halves<1, 3>(a[1]), b0, b1);
+        d8_mma(st.o[2 * s + 1], d8_halves<0, 2>(a[2]), d8_halves<1, 3>(a[2]), d8_halves<0, 2>(a[3]), d8_halves<1, 3>(a[3]), b0, b1);
       }
     }
   }
 }
 
+// Four output elements: sums over the sum of the probabilities.
+__device__ __forceinline__ void d8_store(__nv_bfloat16* out, float4 acc, float L) {
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
 // HD: register capacity (head_dim <= HD; head_dim and page_size are multiples of 16).
-template <int HD>
+// FULL: head_dim is HD.
+template <int HD, bool FULL>
 __global__ void __launch_bounds__(D8_THREADS, 2)
 attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                          const Decode8Params p) {
   extern __shared__ uint8_t d8_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(d8_raw) + 1023) & ~(uintptr_t)1023);
-  const int hd = p.hd, G = p.nh / p.nkv;
+  const int hd = FULL ? HD : p.hd, G = p.nh / p.nkv;
   const int pairs = p.nkv * p.groups;                          // pairs of a token: (kv head, up to 8 query heads)
   const int nsub = (hd + 127) >> 7;
   const uint32_t sub_bytes = (uint32_t)p.page_size * D8_ROW;
   const uint32_t page_bytes = nsub * sub_bytes;
-  const int stride_f = hd + 2, pstride = hd + 4;
+  const int stride_f = hd + 4;                                 // floats of a partial result: values, maximum, sum
   const int HP = G < D8_HEADS ? G : D8_HEADS;
-  float* merge = reinterpret_cast<float*>(ring + (size_t)p.stages * 2 * page_bytes);      // [warps][HP][hd + 2]
-  Decode8Shared* sh = reinterpret_cast<Decode8Shared*>(merge + (((size_t)D8_WARPS * HP * stride_f + 3) & ~(size_t)3));
+  float* merge = reinterpret_cast<float*>(ring + (size_t)p.stages * 2 * page_bytes);      // [warps][HP][hd + 4]
+  Decode8Shared* sh = reinterpret_cast<Decode8Shared*>(merge + (size_t)D8_WARPS * HP * stride_f);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &sh->abort_flag;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      tc::mbar_init(&sh->full[s], 1);
-      tc::mbar_init(&sh->empty[s], 1);
-    }
+    for (int s = 0; s < p.stages; ++s) tc::mbar_init(&sh->full[s], 1);
     sh->abort_flag = 0;
-    sh->last_one = 0;
-    sh->start_token = -1;
     tc::fence_barrier_init();
     tc::tma_prefetch_desc(&map_k);
     tc::tma_prefetch_desc(&map_v);
   }
   pdl_wait_release();
-  // ---- where this block begins: a scan over the tokens' units, some tokens per thread ---------------------------
-  const int per = (p.T + D8_THREADS - 1) / D8_THREADS;
-  const int r0 = min((int)threadIdx.x * per, p.T), r1 = min(r0 + per, p.T);
-  long long mine = 0;
-  for (int r = r0; r < r1; ++r) mine += (long long)(p.pair_cost + d8_segment(p.positions[r], p.window, p.page_size).pages) * pairs;
-  long long incl = mine;
+  // ---- where this block begins: every warp scans the tokens' units for itself, some consecutive tokens per lane -----
+  const int per = (p.T + 31) >> 5;
+  const int r0 = min(lane * per, p.T), r1 = min(r0 + per, p.T);
+  int mine = 0, row_first = 0;
+  if (r0 < r1) row_first = p.token_seq[r0];
+  for (int r = r0; r < r1; ++r) mine += (p.pair_cost + d8_segment(p.positions[r], p.window, p.page_size).pages) * pairs;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
-  if (lane == 31) sh->warp_sum[warp] = incl;
-  __syncthreads();
-  long long before = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < D8_THREADS / 32; ++w) {
-    if (w < warp) before += sh->warp_sum[w];
-    total += sh->warp_sum[w];
-  }
-  const long long share = (total + gridDim.x - 1) / gridDim.x;
-  const long long W = share > p.min_units ? share : p.min_units;
+  const int total = __shfl_sync(0xffffffffu, incl, 31);
+  const int W = max(p.min_units, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const long long begin = (long long)blockIdx.x * W;
   if (begin >= total) return;                                  // fewer units than blocks (the same for all threads)
-  if (begin >= before && begin < before + mine) {
-    int r = r0;
-    long long inside = begin - before;
-    for (; r < r1; ++r) {
-      const long long u = (long long)(p.pair_cost + d8_segment(p.positions[r], p.window, p.page_size).pages) * pairs;
+  int t = 0, pos = 0, row = 0, inside = (int)begin - (incl - mine);
+  const bool owner = inside >= 0 && inside < mine;             // one lane of the warp
+  if (owner) {
+    t = r0;
+    row = row_first;
+    for (;; ++t) {
+      pos = p.positions[t];
+      const int u = (p.pair_cost + d8_segment(pos, p.window, p.page_size).pages) * pairs;
       if (inside < u) break;
       inside -= u;
     }
-    sh->start_token = r;
-    sh->start_inside = (int)inside;
+    if (t > r0) row = p.token_seq[t];
   }
-  __syncthreads();
-  int t = sh->start_token;
-  int remaining = (int)min(W, total - begin);                  // units
-  int pos = p.positions[t];
+  const int who = __ffs(__ballot_sync(0xffffffffu, owner)) - 1;
+  t = __shfl_sync(0xffffffffu, t, who);
+  pos = __shfl_sync(0xffffffffu, pos, who);
+  row = __shfl_sync(0xffffffffu, row, who);
+  inside = __shfl_sync(0xffffffffu, inside, who);
+  int remaining = min(W, total - (int)begin);                  // units
   Decode8Segment sg = d8_segment(pos, p.window, p.page_size);
-  int pair = sh->start_inside / (p.pair_cost + sg.pages);
-  int voff = sh->start_inside - pair * (p.pair_cost + sg.pages);
-  int it0 = 0;
-  volatile int* abort_flag = &sh->abort_flag;
+  int pair = inside / (p.pair_cost + sg.pages);
+  int voff = inside - pair * (p.pair_cost + sg.pages);
 
-  if (warp == D8_WARPS) {
-    // ---- producer warp: 32 page lookups at a time with the pages' scales, one lane starts the copies --------------
-    int row = p.token_seq[t];
-    while (remaining > 0 && t < p.T) {
-      const int units = min(remaining, p.pair_cost + sg.pages - voff);    // of this pair in this block
-      const int off = max(voff, p.pair_cost) - p.pair_cost;               // first page
-      const int n = max(0, voff + units - p.pair_cost - off);             // pages
-      const int kvh = pair / p.groups;
-      const int* table = p.block_table + (size_t)row * p.max_pages + sg.page_lo + off;
-      for (int base = 0; base < n; base += 32) {
-        int page = 0;
-        float ks = 0.f, vs = 1.f;
-        if (base + lane < n) {
-          page = sg.page_lo + off + base + lane < p.max_pages ? table[base + lane] : -1;
-          if (page < 0 || page >= p.num_pages) {               // never read outside the pool; report it
-            atomicExch(p.status, 3);
-            page = 0;
-          }
-          ks = p.k_scale[(size_t)page * p.nkv + kvh];
-          vs = p.v_scale[(size_t)page * p.nkv + kvh];
-          if (!(fabsf(vs) <= 3.4e38f)) {                       // not finite: the keys say so, the values stay finite
-            ks = __int_as_float(0x7fc00000);
-            vs = 1.f;
-          }
-          if (vs == 0.f) vs = 7.5231638e-37f;                  // 2^-120: a page that nothing was written to
+  // ---- the block's pages are looked up 128 at a time, one by a thread, into one of two halves of `entry`: chunk c + 1
+  // when the block comes to chunk c.  The walk over the pairs goes on where the last lookup ended. ----------------------
+  int wt = t, wpos = pos, wrow = row, wpair = pair, woff = voff, wleft = remaining;
+  auto look_up = [&](int half) -> int {                        // place of this thread's page in the scales, -1: none
+    int at = -1, first_row = -1;
+    const int i = threadIdx.x;
+    for (int i0 = 0; i0 < D8_CHUNK && wleft > 0 && wt < p.T;) {           // the same walk in all threads, pair by pair
+      const Decode8Segment ws = d8_segment(wpos, p.window, p.page_size);
+      const int skipped = max(woff, p.pair_cost) - woff;       // empty units
+      const int off = woff + skipped - p.pair_cost;            // first page of this pair here
+      const int n = max(0, min(D8_CHUNK - i0, min(wleft - skipped, ws.pages - off)));
+      if (i >= i0 && i < i0 + n) {
+        const int unit = ws.page_lo + off + i - i0, place = unit / p.splits;
+        int page = place < p.max_pages ? p.block_table[(size_t)wrow * p.max_pages + place] : -1;
+        if (page < 0 || page >= p.num_pages) {                 // never read outside the pool; report it
+          atomicExch(p.status, 3);
+          page = 0;
         }
-        for (int j = 0; j < 32 && base + j < n; ++j) {
-          const int it = it0 + base + j;
-          const int pg = __shfl_sync(0xffffffffu, page, j);
-          const float pks = __shfl_sync(0xffffffffu, ks, j), pvs = __shfl_sync(0xffffffffu, vs, j);
-          if (tc::elect_one()) {
-            const int s = it % p.stages;
-            bool ok = true;
-            if (it >= p.stages) ok = tc::mbar_wait(&sh->empty[s], ((it / p.stages) - 1) & 1, abort_flag);
-            if (ok) {
-              uint8_t* kdst = ring + (size_t)s * 2 * page_bytes;
-              const int at = (pg * p.nkv + kvh) * p.page_size;
-              sh->scale[s] = make_float2(pks, pvs);            // before the arrival that completes with the copies
-              tc::mbar_expect_tx(&sh->full[s], 2 * page_bytes);
-              if (p.whole_page) {
-                tc::tma_load_3d(kdst, &map_k, &sh->full[s], 0, at, 0);
-                tc::tma_load_3d(kdst + page_bytes, &map_v, &sh->full[s], 0, at, 0);
-              } else {
-                for (int sub = 0; sub < nsub; ++sub) {
-                  tc::tma_load_2d(kdst + sub * sub_bytes, &map_k, &sh->full[s], sub * 128, at);
-                  tc::tma_load_2d(kdst + page_bytes + sub * sub_bytes, &map_v, &sh->full[s], sub * 128, at);
-                }
-              }
-            }
-          }
-        }
+        at = page * p.nkv + wpair / p.groups;
+        first_row = at * (p.page_size * p.splits) + (unit - place * p.splits) * p.page_size;
       }
-      remaining -= units;
-      it0 += n;
-      voff = 0;
-      if (++pair == pairs) {
-        pair = 0;
-        if (++t < p.T && remaining > 0) {
-          sg = d8_segment(p.positions[t], p.window, p.page_size);
-          row = p.token_seq[t];
+      i0 += n;
+      wleft -= skipped + n;
+      woff += skipped + n;
+      if (woff >= p.pair_cost + ws.pages) {
+        woff = 0;
+        if (++wpair == pairs) {
+          wpair = 0;
+          if (++wt < p.T && wleft > 0) {
+            wpos = p.positions[wt];
+            wrow = p.token_seq[wt];
+          }
         }
       }
     }
-    return;
-  }
+    if (i < D8_CHUNK) sh->entry[half][i].row = first_row;
+    return at;
+  };
+  auto scales = [&](int half, int at) {
+    if (at < 0) return;
+    sh->entry[half][threadIdx.x].ks = p.k_scale[at];
+    sh->entry[half][threadIdx.x].vs = p.v_scale[at];
+  };
+  // Copies page i of the block into stage s: called by the warp whose page it is, which has read what was there before.
+  auto fetch = [&](int i, int s) {
+    const int first_row = sh->entry[(i / D8_CHUNK) & 1][i & (D8_CHUNK - 1)].row;
+    if (first_row >= 0 && tc::elect_one()) {
+      uint8_t* kdst = ring + (size_t)s * 2 * page_bytes;
+      tc::mbar_expect_tx(&sh->full[s], 2 * page_bytes);
+      if (p.whole_page) {
+        tc::tma_load_3d(kdst, &map_k, &sh->full[s], 0, first_row, 0);
+        tc::tma_load_3d(kdst + page_bytes, &map_v, &sh->full[s], 0, first_row, 0);
+      } else {
+        for (int sub = 0; sub < nsub; ++sub) {
+          tc::tma_load_2d(kdst + sub * sub_bytes, &map_k, &sh->full[s], sub * 128, first_row);
+          tc::tma_load_2d(kdst + page_bytes + sub * sub_bytes, &map_v, &sh->full[s], sub * 128, first_row);
+        }
+      }
+    }
+  };
+  // The first pages are on their way before anything else is waited for.
+  const int at0 = look_up(0);
+  __syncthreads();
+  for (int s = warp; s < p.stages; s += D8_WARPS) fetch(s, s);            // a stage is always the same warp's
+  scales(0, at0);
+  scales(1, look_up(1));
+  bool looked_up = false;                                      // by all threads: a barrier away
 
-  // ---- consumer warps ------------------------------------------------------------------------------------------
   const int g = lane >> 2, tq = lane & 3;
   const float LOG2E = 1.4426950408889634f;
   const float cap2 = p.cap > 0.f ? p.cap * LOG2E : 0.f;
   const float score_scale = p.cap > 0.f ? 2.f * LOG2E * p.multiplier / p.cap : p.multiplier * LOG2E;
-  const uint32_t ring_addr = tc::smem_u32(ring);
-  long long cursor = begin;
+  // for ldmatrix, lane 8 i + r gives row r + 8 (i mod 2) of 16 keys and chunk i / 2 of 32 dims; further chunks are an
+  // exclusive or away (128-byte swizzle: chunk c of row r sits at c ^ (r mod 8))
+  const uint32_t lane_addr = tc::smem_u32(ring) + (uint32_t)((lane & 7) + ((lane >> 3) & 1) * 8) * D8_ROW +
+                             (uint32_t)(((lane >> 4) ^ (lane & 7)) << 4);
+  int it = warp, stage = warp, phase = 0, it0 = 0;              // this warp's next page of the block; the pair's first
+  int cursor = (int)begin;
   while (remaining > 0 && t < p.T) {
     const int units = min(remaining, p.pair_cost + sg.pages - voff);
     const int off = max(voff, p.pair_cost) - p.pair_cost;
     const int n = max(0, voff + units - p.pair_cost - off);
-    const long long pair_begin = cursor - voff + p.pair_cost;   // the pair's first page in the launch's sequence
+    const int pair_begin = cursor - voff + p.pair_cost;         // the pair's first page in the launch's sequence
     cursor += units;
     remaining -= units;
     voff = 0;
-    const int kvh = pair / p.groups, h0 = (pair - kvh * p.groups) * D8_HEADS;     // of the group: first head
-    const int H = min(G - h0, D8_HEADS);
     if (n > 0) {
+      const int kvh = pair / p.groups, h0 = (pair - kvh * p.groups) * D8_HEADS;   // of the group: first head
+      const int H = min(G - h0, D8_HEADS);
       const bool begins = off == 0, ends = off + n == sg.pages;
-      // q^T as the B operand: this thread holds, per 64 dims, dims 16 tq .. 16 tq + 15 of head g, four to a tile
-      uint32_t qb[HD / 16][2];
-      float qscale[2], bias[2];
+      Decode8Query<HD> qy;
       {
         const __nv_bfloat16* qrow = p.q + ((size_t)t * p.nh + kvh * G + h0 + (g < H ? g : 0)) * hd;
+        uint2 raw[HD / 32][2];
         unsigned top = 0;
-        uint32_t raw[HD / 16][2];
 #pragma unroll
-        for (int u = 0; u < HD / 64; ++u) {
-          const bool in = u * 64 + tq * 16 < hd && g < H;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (in) v = *reinterpret_cast<const uint4*>(qrow + u * 64 + tq * 16 + half * 8);
-            raw[4 * u + 2 * half][0] = v.x; raw[4 * u + 2 * half][1] = v.y;
-            raw[4 * u + 2 * half + 1][0] = v.z; raw[4 * u + 2 * half + 1][1] = v.w;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) top = max(top, max(raw[i][j] & 0x7fffu, (raw[i][j] >> 16) & 0x7fffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^-e brings the largest element to [2^8, 2^9); e is held where both powers are normal
-        const int e = max(-100, min(118, (int)(top >> 7) - 127 - 8));
-        const float down = __int_as_float((127 - e) << 23);
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
+        for (int s = 0; s < HD / 32; ++s)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float lo = __uint_as_float(raw[i][j] << 16) * down, hi = __uint_as_float(raw[i][j] & 0xffff0000u) * down;
-            const __half2 hv = __floats2half2_rn(lo, hi);
-            qb[i][j] = *reinterpret_cast<const uint32_t*>(&hv);
-            sum += __low2float(hv) + __high2float(hv);
+            raw[s][j] = make_uint2(0, 0);
+            if (s * 32 + j * 16 < hd && g < H) raw[s][j] = *reinterpret_cast<const uint2*>(qrow + s * 32 + j * 16 + tq * 4);
+            top = __vmaxu2(top, __vmaxu2(raw[s][j].x & 0x7fff7fffu, raw[s][j].y & 0x7fff7fffu));
           }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const float up = __int_as_float((127 + e) << 23);
+        top = max(top & 0xffffu, top >> 16);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^-e brings the largest element below 2^15; e is held where both powers are normal numbers
+        const int e = max(-100, min(113, (int)(top >> 7) - 127 - 14));
+        const float down = __int_as_float((127 - e) << 23);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {                           // from the lanes of head 2 tq + h
-          bias[h] = 0.5f * __shfl_sync(0xffffffffu, sum, (2 * tq + h) * 4);
-          qscale[h] = score_scale * __shfl_sync(0xffffffffu, up, (2 * tq + h) * 4);
+        for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            // x + 1.5 * 2^23 holds the rounded integer in its low bits
+            const float magic = 12582912.f;
+            const uint32_t v0 = __float_as_uint(fmaf(__uint_as_float(raw[s][j].x << 16), down, magic));
+            const uint32_t v1 = __float_as_uint(fmaf(__uint_as_float(raw[s][j].x & 0xffff0000u), down, magic));
+            const uint32_t v2 = __float_as_uint(fmaf(__uint_as_float(raw[s][j].y << 16), down, magic));
+            const uint32_t v3 = __float_as_uint(fmaf(__uint_as_float(raw[s][j].y & 0xffff0000u), down, magic));
+            const uint32_t w01 = __byte_perm(v0, v1, 0x5410), w23 = __byte_perm(v2, v3, 0x5410);
+            qy.lo[s][j] = __byte_perm(w01, w23, 0x6420);
+            qy.hi[s][j] = __byte_perm(w01, w23, 0x7531);
+          }
+        // sum(q) of every head, by a product with rows of ones: it arrives in the lanes that need it
+        const uint32_t ones[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
+        int sh_[4] = {0, 0, 0, 0}, sl_[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) {
+          d8_mma_hi(sh_, ones, qy.hi[s][0], qy.hi[s][1]);
+          d8_mma_lo(sl_, ones, qy.lo[s][0], qy.lo[s][1]);
+        }
+        // a query that is not finite makes its scores NaN
+        const float up = top < 0x7f80u ? __int_as_float((127 + e) << 23) : __int_as_float(0x7fc00000);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int sum = sh_[h] * 256 + sl_[h];
+          qy.start[h] = -128 * sum;
+          qy.half[h] = 0.5f * (float)sum;
+          qy.scale[h] = score_scale * __shfl_sync(0xffffffffu, up, (2 * tq + h) * 4);
         }
       }
       Decode8State<HD> st;
@@ -460,21 +478,45 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         st.l[h] = st.lp[h] = 0.f;
       }
       st.ref = 0.f;
-      // Page `it` of the block belongs to warp it % warps and stage it % stages (a multiple of them: a stage is always
-      // read by the same warp, which therefore sees every phase of the stage's barrier).
-      for (int it = it0 + ((warp - it0) % D8_WARPS + D8_WARPS) % D8_WARPS; it < it0 + n; it += D8_WARPS) {
-        const int s = it % p.stages;
-        const bool ok = tc::mbar_wait(&sh->full[s], (it / p.stages) & 1, abort_flag);
-        const uint32_t kbase = ring_addr + (uint32_t)s * 2 * page_bytes;
-        if (ok) {
-          const float2 scale = sh->scale[s];
-          d8_page<HD>(st, qb, bias, qscale, kbase, kbase + page_bytes, scale.x, scale.y, (sg.page_lo + off + it - it0) * p.page_size,
-                      pos, sg.first, p.page_size, hd, sub_bytes, cap2, lane);
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh->empty[s]);
+      if (!looked_up) {
+        __syncthreads();
+        looked_up = true;
       }
+      // Page `it` of the block belongs to warp it % warps and stage it % stages (a multiple of them: a stage is always
+      // filled and read by the same warp, which therefore sees every phase of the stage's barrier).
+      for (int done = it0; done < it0 + n;) {
+        if (done > 0 && (done & (D8_CHUNK - 1)) == 0) {        // all warps have left the chunk before
+          __syncthreads();
+          const int half = (done / D8_CHUNK + 1) & 1;
+          scales(half, look_up(half));
+          __syncthreads();
+        }
+        done = min(it0 + n, (done & ~(D8_CHUNK - 1)) + D8_CHUNK);
+        for (; it < done; it += D8_WARPS) {
+          const Decode8Entry& en = sh->entry[(it / D8_CHUNK) & 1][it & (D8_CHUNK - 1)];
+          float ks = en.ks, vs = en.vs;
+          if (!(fabsf(vs) <= 3.4e38f)) {                        // not finite: the keys say so, the values stay finite
+            ks = __int_as_float(0x7fc00000);
+            vs = 1.f;
+          }
+          if (vs == 0.f) vs = 7.5231638e-37f;                   // 2^-120: a page that nothing was written to
+          if (tc::mbar_wait(&sh->full[stage], phase, abort_flag)) {
+            const uint32_t kaddr = lane_addr + (uint32_t)stage * 2 * page_bytes;
+            d8_page<HD, FULL>(st, qy, kaddr, kaddr + page_bytes, ks, vs, (sg.page_lo + off + it - it0) * p.page_size, pos, sg.first,
+                              p.page_size, hd, sub_bytes, cap2, lane);
+            __syncwarp();
+            fetch(it + p.stages, stage);
+          }
+          stage += D8_WARPS;
+          if (stage >= p.stages) {
+            stage -= p.stages;
+            phase ^= 1;
+          }
+        }
+      }
+      it0 += n;
       // ---- this warp's totals; the warps are merged in shared memory, in warp order ------------------------------
+      const float unit = st.ref == 0.f ? 0.f : d8_inverse(st.ref) * (1.f / D8_P_BASE);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -485,58 +527,69 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         const int head = 2 * tq + h;
         if (head < H) {
           float* dst = merge + ((size_t)warp * HP + head) * stride_f;
-          const float unit = st.ref * (1.f / D8_P_BASE), half = 0.5f * st.lp[h];
+          const float half = 0.5f * st.lp[h];
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i) {
-            // tile i: dims (d, d + 1) of this lane's 16 (or 8) of the 128 (or 64)
-            const int d = HD == 64 ? g * 8 + 2 * i : (i >> 3) * 128 + ((g >> 1) + 4 * (g & 1)) * 16 + 2 * (i & 7);
-            if (d < hd) *reinterpret_cast<float2*>(dst + d) = make_float2((st.o[i][h] + half) * unit, (st.o[i][2 + h] + half) * unit);
+            const int d = i * 16 + 2 * g;
+            if (FULL || d < hd) *reinterpret_cast<float2*>(dst + d) = make_float2((st.o[i][h] + half) * unit, (st.o[i][2 + h] + half) * unit);
           }
           if (g == 0) *reinterpret_cast<float2*>(dst + hd) = make_float2(st.m[h], st.l[h]);
         }
       }
-      d8_consumer_sync();
+      __syncthreads();
       const bool whole = begins && ends;
-      float* partial = p.partials + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HP * pstride;
+      float* partial = p.partials + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HP * stride_f;
       __nv_bfloat16* out = p.out + ((size_t)t * p.nh + kvh * G + h0) * hd;
-      for (int j = 0; j < H; ++j) {
+      const int quads = hd >> 2;
+      for (int e = threadIdx.x; e < H * quads; e += D8_THREADS) {
+        const int j = e / quads, d = (e - j * quads) * 4;
+        const float* part = merge + (size_t)j * stride_f;
+        float2 ml[D8_WARPS];
         float M = -INFINITY;
 #pragma unroll
-        for (int wv = 0; wv < D8_WARPS; ++wv) M = fmaxf(M, merge[((size_t)wv * HP + j) * stride_f + hd]);
-        float L = 0.f, w[D8_WARPS];
+        for (int wv = 0; wv < D8_WARPS; ++wv) {
+          ml[wv] = *reinterpret_cast<const float2*>(part + (size_t)wv * HP * stride_f + hd);
+          M = fmaxf(M, ml[wv].x);
+        }
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int wv = 0; wv < D8_WARPS; ++wv) {
-          const float2 ml = *reinterpret_cast<const float2*>(merge + ((size_t)wv * HP + j) * stride_f + hd);
-          // a warp without pages has l = 0; one whose scores were all NaN has the maximum -inf and l = NaN
-          w[wv] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : d8_exp2(ml.x - M);
-          L += ml.y * w[wv];
+          // a warp without pages has l = 0; one whose scores were all NaN has no maximum and l = NaN
+          const float w = ml[wv].x == -INFINITY ? (ml[wv].y == 0.f ? 0.f : ml[wv].y) : d8_exp2(ml[wv].x - M);
+          const float4 v = *reinterpret_cast<const float4*>(part + (size_t)wv * HP * stride_f + d);
+          L += ml[wv].y * w;
+          acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
         }
-        for (int d = threadIdx.x; d < hd; d += D8_WARPS * 32) {
-          float ov = 0.f;
-#pragma unroll
-          for (int wv = 0; wv < D8_WARPS; ++wv) ov += merge[((size_t)wv * HP + j) * stride_f + d] * w[wv];
-          if (whole) out[(size_t)j * hd + d] = __float2bfloat16_rn(L == 0.f ? 0.f : ov / L);
-          else partial[(size_t)j * pstride + d] = ov;
+        if (whole) {
+          d8_store(out + (size_t)j * hd + d, acc, L);
+        } else {
+          *reinterpret_cast<float4*>(partial + (size_t)j * stride_f + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(partial + (size_t)j * stride_f + hd) = make_float2(M, L);
         }
-        if (!whole && threadIdx.x == 0) *reinterpret_cast<float2*>(partial + (size_t)j * pstride + hd) = make_float2(M, L);
       }
+      __syncthreads();                                          // the merge area is free, every part of the partial is written
       if (!whole) {
-        // ---- the pair is shared: the block that leaves its part last adds the parts up, in block order --------------
-        const int b_first = (int)(pair_begin / W), b_last = (int)((pair_begin + sg.pages - 1) / W);
-        d8_consumer_sync();                                     // every thread's share of the partial result is written
-        if (threadIdx.x == 0) {
-          __threadfence();                                      // and visible before this block is counted
-          int* counter = p.arrive + (size_t)t * pairs + pair;
-          const int last = atomicAdd(counter, 1) == b_last - b_first;
-          if (last) *counter = 0;                               // for the next launch
-          __threadfence();
-          sh->last_one = last;
-        }
-        d8_consumer_sync();
-        if (sh->last_one) {
-          const int parts = b_last - b_first + 1;
-          const int quads = hd >> 2;
-          for (int e = threadIdx.x; e < H * quads; e += D8_WARPS * 32) {
+        // ---- the pair is shared: the block that leaves its part last adds the parts up, in block order.  With pages left
+        // to do that is warp 0's work (the block whose last pair it is usually arrives later), else all warps'. -----------
+        const int b_first = pair_begin / W, parts = (pair_begin + sg.pages - 1) / W - b_first + 1;
+        const bool all = remaining <= 0;
+        if (all || warp == 0) {
+          int last = 0;
+          if (threadIdx.x == 0) {
+            // counted after this block's part is visible, and the others' parts are visible to the one that counts last
+            int* counter = p.arrive + (size_t)t * pairs + pair;
+            int seen;
+            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(seen) : "l"(counter) : "memory");
+            last = seen == parts - 1;
+            if (last) *counter = 0;                             // for the next launch
+            if (all) sh->last_one = last;
+          }
+          if (all) __syncthreads();
+          last = all ? sh->last_one : __shfl_sync(0xffffffffu, last, 0);
+          __syncwarp();
+          const int step = all ? D8_THREADS : 32;
+          for (int e = threadIdx.x; last && e < H * quads; e += step) {
             const int j = e / quads, d = (e - j * quads) * 4;
             float M = -INFINITY, L = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -549,7 +602,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 ml[k] = make_float2(-INFINITY, 0.f);
                 v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i0 + k < parts) {
-                  const float* from = p.partials + (((size_t)bk * 2 + (bk == b_first ? 1 : 0)) * HP + j) * pstride;
+                  const float* from = p.partials + (((size_t)bk * 2 + (bk == b_first ? 1 : 0)) * HP + j) * stride_f;
                   ml[k] = __ldcg(reinterpret_cast<const float2*>(from + hd));
                   v[k] = __ldcg(reinterpret_cast<const float4*>(from + d));
                 }
@@ -568,15 +621,11 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
               }
               M = top;
             }
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-            *reinterpret_cast<uint2*>(out + (size_t)j * hd + d) =
-                make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            d8_store(out + (size_t)j * hd + d, acc, L);
           }
+          __syncwarp();
         }
       }
-      d8_consumer_sync();                                       // the merge area and last_one are used again by the next pair
-      it0 += n;
     }
     if (++pair == pairs) {
       pair = 0;
@@ -630,22 +679,13 @@ static int d8_map(CUtensorMap* map, const void* pool, long long rows, int hd, in
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? GLINT_OK : GLINT_ERR_BAD_ARG;
 }
 
-static long long d8_fixed(int G, int hd) {
-  const int HP = G < D8_HEADS ? G : D8_HEADS;
-  return (((long long)D8_WARPS * HP * (hd + 2) + 3) & ~3ll) * 4 + (long long)sizeof(Decode8Shared) + 1024;
-}
-
 }  // namespace glint
 
 using namespace glint;
 
-// Head sizes in steps of 16 up to 256, pages in steps of 16 of which one per consumer warp fits a block's shared memory.
+// Head sizes in steps of 16 up to 256, pages in steps of 16.
 GLINT_API int glint_attention_decode8_supported(int nh, int nkv, int hd, int page_size) {
-  if (!(nkv > 0 && nh > 0 && nh % nkv == 0 && hd % 16 == 0 && hd >= 16 && hd <= 256 && page_size % 16 == 0 && page_size >= 16 &&
-        page_size <= 256))
-    return 0;
-  const long long page_bytes = (long long)((hd + 127) / 128) * page_size * D8_ROW;
-  return D8_WARPS * 2 * page_bytes + d8_fixed(nh / nkv, hd) <= 227 * 1024 ? 1 : 0;
+  return nkv > 0 && nh > 0 && nh % nkv == 0 && hd % 16 == 0 && hd >= 16 && hd <= 256 && page_size % 16 == 0 && page_size >= 16 ? 1 : 0;
 }
 
 // Workspace of launches over `blocks` blocks: floats of partial results.
@@ -672,43 +712,56 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
   const int G = nh / nkv, groups = (G + D8_HEADS - 1) / D8_HEADS, pairs = nkv * groups;
   if (pairs > arrive_ints) return GLINT_ERR_UNSUPPORTED_SIZE;
   const int whole_page = hd % 128 == 0 ? 1 : 0;
+  const long long fixed = (long long)D8_WARPS * (G < D8_HEADS ? G : D8_HEADS) * (hd + 4) * 4 + sizeof(Decode8Shared) + 1024;
+  const long long row_bytes = (hd + 127) / 128 * D8_ROW;
+  // A large page is read in parts of 64, 32 or 16 rows, the largest of which two stages per warp let two blocks share an SM
+  int part = 64;
+  while (part > 16 && (page_size % part || 2 * D8_WARPS * 2 * part * row_bytes + fixed > D8_BLOCK_SMEM)) part >>= 1;
+  const int splits = page_size / part;
+  page_size = part;
   CUtensorMap map_k, map_v;
   int rc = d8_map(&map_k, k_pool, rows, hd, page_size, whole_page);
   if (rc == GLINT_OK) rc = d8_map(&map_v, v_pool, rows, hd, page_size, whole_page);
   if (rc != GLINT_OK) return rc;
-  const long long page_bytes = (long long)((hd + 127) / 128) * page_size * D8_ROW;
-  const long long fixed = d8_fixed(G, hd);
-  int stages = (int)((112 * 1024 - fixed) / (2 * page_bytes)) / D8_WARPS * D8_WARPS;     // two blocks share an SM
+  const long long page_bytes = page_size * row_bytes;
+  int stages = (int)((D8_BLOCK_SMEM - fixed) / (2 * page_bytes * D8_WARPS)) * D8_WARPS;
   if (stages > D8_MAX_STAGES) stages = D8_MAX_STAGES;
   if (stages < D8_WARPS) stages = D8_WARPS;
   const long long smem = stages * 2 * page_bytes + fixed;
-  if (smem > 227 * 1024) return GLINT_ERR_UNSUPPORTED_SIZE;
   // what a pair costs a block beside its pages, and the least a block is given, in pages of this size
   const long long unit = 2ll * page_size * hd;
-  const int pair_cost = (int)((48 * 1024 + unit / 2) / unit) + 1;
-  const int min_units = (int)((32 * 1024 + unit - 1) / unit) + 1;
+  const int pair_cost = (int)((96 * 1024 + unit / 2) / unit) + 1;
+  const int min_units = (int)((64 * 1024 + unit - 1) / unit) + 1;
   long long most_pages = ((long long)max_context + page_size - 1) / page_size;
   if (window > 0 && ((long long)window + page_size - 1) / page_size + 1 < most_pages)
     most_pages = ((long long)window + page_size - 1) / page_size + 1;
-  const int step = arrive_ints / pairs < D8_MAX_TOKENS ? arrive_ints / pairs : D8_MAX_TOKENS;
+  // units are counted in 32 bits
+  const long long fits = 0x3fffffffLL / ((long long)pairs * (most_pages + pair_cost));
+  if (fits < 1) return GLINT_ERR_UNSUPPORTED_SIZE;
+  int step = arrive_ints / pairs < D8_MAX_TOKENS ? arrive_ints / pairs : D8_MAX_TOKENS;
+  if (fits < step) step = (int)fits;
   for (int t0 = 0; t0 < T; t0 += step) {
     const int n = T - t0 < step ? T - t0 : step;
     Decode8Params p = {(const __nv_bfloat16*)q + (size_t)t0 * nh * hd, positions + t0, token_seq + t0, block_table, k_scale, v_scale,
                        (__nv_bfloat16*)out + (size_t)t0 * nh * hd, partials, arrive, status, multiplier, cap,
-                       n, nh, nkv, hd, groups, page_size, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units};
+                       n, nh, nkv, hd, groups, page_size, splits, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units};
     const long long most = (long long)n * pairs * (most_pages + pair_cost);
     const long long useful = (most + min_units - 1) / min_units;
     const int grid = useful < blocks ? (int)useful : blocks;
-#define LAUNCH(HD)                                                                                                       \
-  {                                                                                                                      \
-    cudaError_t e = cudaFuncSetAttribute(attention_decode8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
-    if (e != cudaSuccess) return (int)e;                                                                                 \
-    e = launch_kernel(attention_decode8_kernel<HD>, dim3(grid), dim3(D8_THREADS), (size_t)smem, stream, map_k, map_v, p); \
-    if (e != cudaSuccess) return (int)e;                                                                                 \
+#define LAUNCH(HD, FULL)                                                                                            \
+  {                                                                                                                 \
+    cudaError_t e = cudaFuncSetAttribute(attention_decode8_kernel<HD, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                                         (int)smem);                                                                \
+    if (e != cudaSuccess) return (int)e;                                                                            \
+    e = launch_kernel(attention_decode8_kernel<HD, FULL>, dim3(grid), dim3(D8_THREADS), (size_t)smem, stream, map_k, map_v, p); \
+    if (e != cudaSuccess) return (int)e;                                                                            \
   }
-    if (hd <= 64) LAUNCH(64)
-    else if (hd <= 128) LAUNCH(128)
-    else LAUNCH(256)
+    if (hd == 64) LAUNCH(64, true)
+    else if (hd == 128) LAUNCH(128, true)
+    else if (hd == 256) LAUNCH(256, true)
+    else if (hd < 64) LAUNCH(64, false)
+    else if (hd < 128) LAUNCH(128, false)
+    else LAUNCH(256, false)
 #undef LAUNCH
   }
   return (int)cudaGetLastError();
