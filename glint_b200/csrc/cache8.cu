@@ -52,6 +52,282 @@ __device__ __forceinline__ float2 rope_angle(int pos, double turns, float amplit
   return make_float2(c * amplitude, s * amplitude);
 }
 
+// ---- heads of up to 256: a lane holds NP pairs of a head ------------------------------------------------------------
+//
+// Memory-bound for portions (a float read and one to two bytes written per element), latency-bound for single tokens.
+// One launch of two kinds of blocks of eight warps.  Cache blocks: a window of 16 tokens x one kv head x keys or values.  A
+// block owns the runs (tokens of one request in one page) that begin in its window and takes them whole, so that the
+// largest magnitude of a run, and with it the page's new scale, is found in one block whatever the windows cut: a warp
+// per token, values kept in registers (four tokens a warp) between the maximum and the codes.  Query blocks: a warp
+// rotates four heads of a token with one set of sines and cosines.
+constexpr int AP_WARPS = 8;
+constexpr int AP_WINDOW = 16;                     // tokens
+constexpr int AP_HELD = 4;                        // tokens of a warp whose values stay in registers
+constexpr int AP_MOST_PAGE = AP_WARPS * 32 - AP_WINDOW;       // rows of a page: a thread per token of a block
+constexpr int AP_HEADS = 4;                       // query heads of a unit
+
+// Pair i of a head: its two dims.  The first rot / 2 are turned.
+__device__ __forceinline__ int2 rope_pair(int i, int rot, int interleaved) {
+  const int half = rot >> 1;
+  return interleaved || i >= half ? make_int2(2 * i, 2 * i + 1) : make_int2(i, i + half);
+}
+
+template <typename S, int NP>
+__global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const AppendParams p, int cache_blocks) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int width = (p.nh + 2 * p.nkv) * p.hd, half = p.rot >> 1, pairs = p.hd >> 1;
+  pdl_wait_release();
+  int2 at[NP];
+  double turns[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int i = lane + 32 * k;
+    at[k] = rope_pair(i, p.rot, p.interleaved);
+    turns[k] = i < half ? p.turns[i] : 0.0;
+  }
+
+  if ((int)blockIdx.x >= cache_blocks) {
+    // ---- queries ---------------------------------------------------------------------------------------------------
+    const int groups = (p.nh + AP_HEADS - 1) / AP_HEADS;
+    const long long unit = (long long)(blockIdx.x - cache_blocks) * AP_WARPS + warp;
+    const int t = (int)(unit / groups), h0 = (int)(unit - (long long)t * groups) * AP_HEADS;
+    if (t >= p.T) return;
+    const float* src = p.qkv + (size_t)t * width + (size_t)h0 * p.hd;
+    S* dst = (S*)p.q_out + ((size_t)t * p.nh + h0) * p.hd;
+    float a[AP_HEADS][NP], b[AP_HEADS][NP];
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; ++h)
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        if (h0 + h < p.nh && lane + 32 * k < pairs) {
+          a[h][k] = src[h * p.hd + at[k].x];
+          b[h][k] = src[h * p.hd + at[k].y];
+        }
+    const int pos = p.positions[t];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      if (lane + 32 * k >= pairs) continue;
+      const bool turned = lane + 32 * k < half;
+      const float2 cs = turned ? rope_angle(pos, turns[k], p.amplitude) : make_float2(1.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < AP_HEADS; ++h)
+        if (h0 + h < p.nh) {
+          const float x = a[h][k], y = b[h][k];
+          dst[h * p.hd + at[k].x] = from_float<S>(turned ? x * cs.x - y * cs.y : x);
+          dst[h * p.hd + at[k].y] = from_float<S>(turned ? x * cs.y + y * cs.x : y);
+        }
+    }
+    return;
+  }
+
+  // ---- keys and values -----------------------------------------------------------------------------------------------
+  __shared__ unsigned starts[AP_WARPS], bad[AP_WARPS];    // per token behind the window's first: does a run begin, in order
+  __shared__ int seqs[AP_WARPS * 32], poss[AP_WARPS * 32];
+  __shared__ unsigned tops[AP_WARPS * 32];                // largest magnitude of a token, as bits
+  const int kv = blockIdx.x % (2 * p.nkv), is_v = kv & 1, h = kv >> 1;
+  const int t0 = (int)(blockIdx.x / (2 * p.nkv)) * AP_WINDOW;
+  const int reach = min(AP_WINDOW + p.page_size, p.T - t0);
+  {
+    const int i = threadIdx.x, t = t0 + i;
+    bool start = true, wrong = false;                     // what lies behind the reach ends every run
+    if (i < reach) {
+      const int seq = p.token_seq[t], pos = p.positions[t];
+      seqs[i] = seq;
+      poss[i] = pos;
+      if (t > 0) {
+        const int before = p.token_seq[t - 1], pos_before = p.positions[t - 1];
+        wrong = before > seq || (before == seq && pos_before + 1 != pos);
+        start = wrong || before != seq || pos_before / p.page_size != pos / p.page_size;
+      }
+      if (wrong && i < AP_WINDOW) atomicExch(p.status, 5);
+    }
+    const unsigned s = __ballot_sync(0xffffffffu, start), w = __ballot_sync(0xffffffffu, wrong);
+    if (lane == 0) {
+      starts[warp] = s;
+      bad[warp] = w;
+    }
+  }
+  __syncthreads();
+  // the block's tokens: from the first run that begins in the window to the end of the last one that does
+  const unsigned in_window = starts[0] & 0xffffu;
+  if (!in_window || (__ffs(in_window) - 1) >= reach) return;
+  const int first = __ffs(in_window) - 1;
+  int last = reach;
+  {
+    const unsigned behind = starts[0] >> AP_WINDOW;
+    if (behind) {
+      last = AP_WINDOW + __ffs(behind) - 1;
+    } else {
+      for (int w = 1; w < AP_WARPS; ++w)
+        if (starts[w]) {
+          last = w * 32 + __ffs(starts[w]) - 1;
+          break;
+        }
+    }
+    last = min(last, reach);
+  }
+  const float* src = p.qkv + (size_t)t0 * width + (size_t)(p.nh + (is_v ? p.nkv : 0) + h) * p.hd;
+  // values of token i, rotated
+  auto load = [&](int i, float (&a)[NP], float (&b)[NP]) {
+    const float* row = src + (size_t)i * width;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const bool in = lane + 32 * k < pairs;
+      a[k] = in ? row[at[k].x] : 0.f;
+      b[k] = in ? row[at[k].y] : 0.f;
+    }
+  };
+  auto turn = [&](int i, float (&a)[NP], float (&b)[NP]) {
+    if (is_v) return;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      if (lane + 32 * k >= half) continue;
+      const float2 cs = rope_angle(poss[i], turns[k], p.amplitude);
+      const float x = a[k], y = b[k];
+      a[k] = x * cs.x - y * cs.y;
+      b[k] = x * cs.y + y * cs.x;
+    }
+  };
+  auto top_of = [&](const float (&a)[NP], const float (&b)[NP]) -> unsigned {
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) m = max(m, max(__float_as_uint(a[k]) & 0x7fffffffu, __float_as_uint(b[k]) & 0x7fffffffu));
+    return __reduce_max_sync(0xffffffffu, m);
+  };
+  const bool coded = p.k_scale != nullptr;
+  float a[AP_HELD][NP], b[AP_HELD][NP];
+#pragma unroll
+  for (int c = 0; c < AP_HELD; ++c)
+    if (first + warp + c * AP_WARPS < last) load(first + warp + c * AP_WARPS, a[c], b[c]);
+  unsigned old[AP_HELD];                                  // scales before this step, read before any is written
+  float* scale = is_v ? p.v_scale : p.k_scale;
+  // of token i: its run's first token, and the run's page (-1: none, or out of order)
+  auto run_of = [&](int i, int& page) -> int {
+    int w = i >> 5;
+    unsigned m = starts[w] & (0xffffffffu >> (31 - (i & 31)));
+    while (!m) m = starts[--w];                           // `first` begins a run
+    const int s = w * 32 + 31 - __clz(m);
+    const int pos = poss[s], place = pos / p.page_size;
+    page = -1;
+    if (!((bad[w] >> (s & 31)) & 1u)) {
+      if (pos >= 0 && place < p.max_pages) page = p.block_table[(size_t)seqs[s] * p.max_pages + place];
+      if (page < 0 || page >= p.num_pages) {
+        if (lane == 0) atomicExch(p.status, 2);
+        page = -1;
+      }
+    }
+    return s;
+  };
+  int pages[AP_HELD], begins[AP_HELD];
+#pragma unroll
+  for (int c = 0; c < AP_HELD; ++c) {
+    const int i = first + warp + c * AP_WARPS;
+    old[c] = 0;
+    pages[c] = -1;
+    if (i >= last) continue;
+    begins[c] = run_of(i, pages[c]);
+    if (coded && pages[c] >= 0 && poss[begins[c]] % p.page_size)
+      old[c] = __float_as_uint(scale[(size_t)pages[c] * p.nkv + h]) & 0x7fffffffu;
+  }
+#pragma unroll
+  for (int c = 0; c < AP_HELD; ++c) {
+    const int i = first + warp + c * AP_WARPS;
+    if (i >= last) continue;
+    turn(i, a[c], b[c]);
+    const unsigned m = top_of(a[c], b[c]);
+    if (lane == 0) tops[i] = m;
+  }
+  for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {    // pages of more than 16 rows
+    float x[NP], y[NP];
+    load(i, x, y);
+    turn(i, x, y);
+    const unsigned m = top_of(x, y);
+    if (lane == 0) tops[i] = m;
+  }
+  auto store = [&](int i, const float (&x)[NP], const float (&y)[NP], int s, int page, unsigned before) {
+    const size_t row = ((size_t)page * p.nkv + h) * p.page_size;
+    const int off = poss[i] % p.page_size;
+    if (!coded) {
+      S* dst = (S*)(is_v ? p.v_pool : p.k_pool) + (row + off) * p.hd;
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        if (lane + 32 * k < pairs) {
+          dst[at[k].x] = from_float<S>(x[k]);
+          dst[at[k].y] = from_float<S>(y[k]);
+        }
+      return;
+    }
+    // the run's largest magnitude: its tokens are s .. e - 1
+    const int off0 = poss[s] % p.page_size;
+    unsigned m = 0;
+    for (int j = s + lane; j < min(last, s + p.page_size - off0); j += 32) {
+      bool same = true;                                   // no run begins between s and j
+      for (int w = s >> 5; w <= j >> 5 && same; ++w) {
+        unsigned bits = starts[w];
+        if (w == s >> 5) bits &= ~(0xffffffffu >> (31 - (s & 31)));
+        if (w == j >> 5) bits &= 0xffffffffu >> (31 - (j & 31));
+        same = bits == 0;
+      }
+      if (same) m = max(m, tops[j]);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    const bool finite = m < C8_NOT_FINITE && before < C8_NOT_FINITE;
+    const int e_old = (int)(before >> 23) - 127;
+    const int e = off0 > 0 ? max(c8_exponent(m), e_old) : c8_exponent(m);
+    uint8_t* dst = (uint8_t*)(is_v ? p.v_pool : p.k_pool) + row * p.hd;
+    if (i == s) {
+      if (lane == 0) scale[(size_t)page * p.nkv + h] = finite ? c8_pow2(e) : __int_as_float(0x7fc00000);
+      if (finite && off0 > 0 && e > e_old) {              // the rows before move to the new scale
+        const int d = min(e - e_old, 31);
+        for (int j = lane; j < off0 * pairs; j += 32) {   // two codes at a time
+          uchar2* q = reinterpret_cast<uchar2*>(dst) + j;
+          uchar2 v = *q;
+          v.x = (unsigned char)((((int)v.x - 128) >> d) + 128);
+          v.y = (unsigned char)((((int)v.y - 128) >> d) + 128);
+          *q = v;
+        }
+      }
+    }
+    dst += (size_t)off * p.hd;
+    const float inv = c8_pow2(-e);
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      if (lane + 32 * k < pairs) {
+        const unsigned char cx = finite ? (unsigned char)c8_code(x[k], inv) : (unsigned char)128;
+        const unsigned char cy = finite ? (unsigned char)c8_code(y[k], inv) : (unsigned char)128;
+        if (at[k].y == at[k].x + 1 && !(at[k].x & 1)) {
+          *reinterpret_cast<uchar2*>(dst + at[k].x) = make_uchar2(cx, cy);
+        } else {
+          dst[at[k].x] = cx;
+          dst[at[k].y] = cy;
+        }
+      }
+  };
+  // Tokens that are not held need their run's scale from before this step as well: read now, kept in shared memory
+  __shared__ unsigned late[AP_WARPS * 32];
+  for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {
+    int page;
+    const int s = run_of(i, page);
+    if (lane == 0) late[i] = coded && page >= 0 && poss[s] % p.page_size ? __float_as_uint(scale[(size_t)page * p.nkv + h]) & 0x7fffffffu : 0u;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < AP_HELD; ++c) {
+    const int i = first + warp + c * AP_WARPS;
+    if (i < last && pages[c] >= 0) store(i, a[c], b[c], begins[c], pages[c], old[c]);
+  }
+  for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {
+    int page;
+    const int s = run_of(i, page);
+    if (page < 0) continue;
+    float x[NP], y[NP];
+    load(i, x, y);
+    turn(i, x, y);
+    store(i, x, y, s, page, late[i]);
+  }
+}
+
+// ---- any head size -------------------------------------------------------------------------------------------------
 // Element d of a head of token t (row of hd floats), rotated.
 __device__ __forceinline__ float rope_element(const AppendParams& p, const float* row, int pos, int d) {
   if (d >= p.rot) return row[d];
@@ -68,6 +344,7 @@ __device__ __forceinline__ float rope_element(const AppendParams& p, const float
 template <typename S>
 __global__ void __launch_bounds__(128) rope_append_simple_kernel(const AppendParams p) {
   __shared__ unsigned top[4];
+  pdl_wait_release();
   const int t0 = blockIdx.x;
   const int width = (p.nh + 2 * p.nkv) * p.hd;
   const int pos0 = p.positions[t0];
@@ -145,33 +422,99 @@ struct UnpackParams {
   int max_pages, window, nkv, page_elems, page_size, num_pages;
 };
 
-// Grid (pages of the longest request, kv heads, requests): the pages that the request's new tokens can reach, each to
-// its own place in the wide pools.  A page whose scale is not finite gives NaN keys and finite values: a query that
-// sees it gets NaN, and a tile that holds it behind a mask (probability 0) gets no 0 x NaN from its values.
-template <typename S>
-__global__ void __launch_bounds__(256) cache8_unpack_simple_kernel(const UnpackParams p) {
-  const int r = blockIdx.z, h = blockIdx.y;
+// A page that a request can reach: its place in the pools, -1 if there is none.
+__device__ __forceinline__ int unpack_page(const UnpackParams& p, int r, int ordinal) {
   const int start = p.seq_start[r], n = p.cu_seqlens[r + 1] - p.cu_seqlens[r];
-  if (n <= 0) return;
+  if (n <= 0) return -1;
   const int lo = p.window > 0 && start - p.window + 1 > 0 ? (start - p.window + 1) / p.page_size : 0;
-  const int place = lo + (int)blockIdx.x;
-  if (place > (start + n - 1) / p.page_size) return;
+  const int place = lo + ordinal;
+  if (place > (start + n - 1) / p.page_size) return -1;
   const int page = place >= p.max_pages ? -1 : p.block_table[(size_t)r * p.max_pages + place];
   if (page < 0 || page >= p.num_pages) {
     if (threadIdx.x == 0) atomicExch(p.status, 3);
-    return;
+    return -1;
   }
-  const size_t at = (size_t)page * p.nkv + h;
+  return page;
+}
+
+// The scales of a page as the readers take them.  One that is not finite becomes NaN keys and finite values: a query
+// that sees the page gets NaN, and a tile that holds it behind a mask (probability 0) gets no 0 x NaN from its values.
+__device__ __forceinline__ float2 unpack_scales(const UnpackParams& p, size_t at) {
   float ks = p.k_scale[at], vs = p.v_scale[at];
   if (!(fabsf(vs) <= 3.4e38f)) {
     ks = __int_as_float(0x7fc00000);
     vs = 0.f;
   }
   if (!(fabsf(ks) <= 3.4e38f)) ks = __int_as_float(0x7fc00000);
+  return make_float2(ks, vs);
+}
+
+// Four codes as values, exactly: a byte permutation puts a code c under the exponent of 2^15 as 32768 + c.
+__device__ __forceinline__ float widen(uint32_t raised, float s) { return (__uint_as_float(raised) - 32895.5f) * s; }
+__device__ __forceinline__ float4 widen4(uint32_t w, float s) {
+  const uint32_t under = 0x47000000u;
+  return make_float4(widen(__byte_perm(w, under, 0x7404), s), widen(__byte_perm(w, under, 0x7414), s),
+                     widen(__byte_perm(w, under, 0x7424), s), widen(__byte_perm(w, under, 0x7434), s));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void store16(__nv_bfloat16* to, const float4 (&v)[4]) {
+  uint4* t = reinterpret_cast<uint4*>(to);
+  t[0] = make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[0].z, v[0].w), pack_bf16(v[1].x, v[1].y), pack_bf16(v[1].z, v[1].w));
+  t[1] = make_uint4(pack_bf16(v[2].x, v[2].y), pack_bf16(v[2].z, v[2].w), pack_bf16(v[3].x, v[3].y), pack_bf16(v[3].z, v[3].w));
+}
+__device__ __forceinline__ void store16(float* to, const float4 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(to)[i] = v[i];
+}
+
+// Memory-bound: a byte read and two written per element.  Grid (pages of the longest range, requests, parts of 8192
+// elements of a page's keys, then of its values): a page's heads lie one behind the other, a thread takes 16 codes at a
+// time of one of them (a page of a head is a multiple of 16 elements).
+constexpr int UP_THREADS = 256;
+constexpr int UP_EACH = 2;                        // sixteens of a thread
+
+template <typename S>
+__global__ void __launch_bounds__(UP_THREADS) cache8_unpack_kernel(const UnpackParams p, int parts) {
+  pdl_wait_release();
+  const int page = unpack_page(p, blockIdx.y, blockIdx.x);
+  if (page < 0) return;
+  const int is_v = (int)blockIdx.z >= parts;
+  const int first = ((int)blockIdx.z - (is_v ? parts : 0)) * (UP_THREADS * UP_EACH) + (int)threadIdx.x;
+  const int sixteens = p.nkv * (p.page_elems >> 4), per_head = p.page_elems >> 4;
+  const size_t base = (size_t)page * sixteens;
+  const uint4* from = reinterpret_cast<const uint4*>(is_v ? p.v : p.k) + base;
+  S* to = (S*)(is_v ? p.v_out : p.k_out) + base * 16;
+  uint4 c[UP_EACH];
+#pragma unroll
+  for (int j = 0; j < UP_EACH; ++j)
+    if (first + j * UP_THREADS < sixteens) c[j] = from[first + j * UP_THREADS];
+#pragma unroll
+  for (int j = 0; j < UP_EACH; ++j) {
+    const int i = first + j * UP_THREADS;
+    if (i >= sixteens) break;
+    const float2 both = unpack_scales(p, (size_t)page * p.nkv + i / per_head);
+    const float s = is_v ? both.y : both.x;
+    const float4 v[4] = {widen4(c[j].x, s), widen4(c[j].y, s), widen4(c[j].z, s), widen4(c[j].w, s)};
+    store16(to + (size_t)i * 16, v);
+  }
+}
+
+// Any size, element by element.  Grid (pages of the longest request, kv heads, requests): the pages that the request's new tokens can reach, each to
+// its own place in the wide pools.
+template <typename S>
+__global__ void __launch_bounds__(256) cache8_unpack_simple_kernel(const UnpackParams p) {
+  pdl_wait_release();
+  const int page = unpack_page(p, blockIdx.z, blockIdx.x);
+  if (page < 0) return;
+  const size_t at = (size_t)page * p.nkv + blockIdx.y;
+  const float2 scale = unpack_scales(p, at);
   const size_t base = at * p.page_elems;
   for (int i = threadIdx.x; i < p.page_elems; i += blockDim.x) {
-    ((S*)p.k_out)[base + i] = from_float<S>(((float)p.k[base + i] - 127.5f) * ks);
-    ((S*)p.v_out)[base + i] = from_float<S>(((float)p.v[base + i] - 127.5f) * vs);
+    ((S*)p.k_out)[base + i] = from_float<S>(((float)p.k[base + i] - 127.5f) * scale.x);
+    ((S*)p.v_out)[base + i] = from_float<S>(((float)p.v[base + i] - 127.5f) * scale.y);
   }
 }
 
@@ -198,9 +541,22 @@ GLINT_API int glint_rope_append(const float* qkv, const int* positions, const in
   if (nkv > 32767) return GLINT_ERR_UNSUPPORTED_SIZE;
   AppendParams p = {qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_pool, k_scale, v_scale, status, amplitude,
                     T, nh, nkv, hd, rot, interleaved ? 1 : 0, page_size, num_pages, max_pages};
-  const dim3 grid(T, k_pool ? 1 + 2 * nkv : 1);
-  C8_DISPATCH(dtype, rope_append_simple_kernel<S><<<grid, 128, 0, stream>>>(p));
-  return (int)cudaGetLastError();
+  cudaError_t e = cudaSuccess;
+  if (hd <= 256 && page_size <= AP_MOST_PAGE) {
+    const long long cache_blocks = k_pool ? (long long)((T + AP_WINDOW - 1) / AP_WINDOW) * 2 * nkv : 0;
+    const long long units = (long long)T * ((nh + AP_HEADS - 1) / AP_HEADS);
+    const long long blocks = cache_blocks + (units + AP_WARPS - 1) / AP_WARPS;
+    if (blocks > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
+    const dim3 grid((unsigned)blocks), block(AP_WARPS * 32);
+    const int cb = (int)cache_blocks;
+    if (hd <= 64) { C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, 1>, grid, block, 0, stream, p, cb)) }
+    else if (hd <= 128) { C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, 2>, grid, block, 0, stream, p, cb)) }
+    else { C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, 4>, grid, block, 0, stream, p, cb)) }
+  } else {
+    const dim3 grid(T, k_pool ? 1 + 2 * nkv : 1);
+    C8_DISPATCH(dtype, e = launch_kernel(rope_append_simple_kernel<S>, grid, dim3(128), 0, stream, p))
+  }
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 // Codes of the pages that the new tokens of each request can reach (from the page of the first key that the first of
@@ -215,7 +571,15 @@ GLINT_API int glint_cache8_unpack(const uint8_t* k, const uint8_t* v, const floa
   if (nkv > 65535 || n_seqs > 65535) return GLINT_ERR_UNSUPPORTED_SIZE;
   UnpackParams p = {k, v, k_scale, v_scale, seq_start, cu_seqlens, block_table, k_out, v_out, status, max_pages, window, nkv,
                     page_size * hd, page_size, num_pages};
-  const dim3 grid(most_pages, nkv, n_seqs);
-  C8_DISPATCH(dtype, cache8_unpack_simple_kernel<S><<<grid, 256, 0, stream>>>(p));
-  return (int)cudaGetLastError();
+  cudaError_t e = cudaSuccess;
+  const long long parts = ((long long)nkv * page_size * hd / 16 + UP_THREADS * UP_EACH - 1) / (UP_THREADS * UP_EACH);
+  const bool aligned = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_out | (uintptr_t)v_out) & 15);
+  if ((long long)page_size * hd % 16 == 0 && aligned && 2 * parts <= 65535) {
+    const dim3 grid(most_pages, n_seqs, (unsigned)(2 * parts));
+    C8_DISPATCH(dtype, e = launch_kernel(cache8_unpack_kernel<S>, grid, dim3(UP_THREADS), 0, stream, p, (int)parts))
+  } else {
+    const dim3 grid(most_pages, nkv, n_seqs);
+    C8_DISPATCH(dtype, e = launch_kernel(cache8_unpack_simple_kernel<S>, grid, dim3(256), 0, stream, p))
+  }
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }

@@ -180,6 +180,14 @@ extern "C" int glint_op_rope_append(const GlintRuntime* rt, const GlintStep* ste
                                    step->num_tokens, nh, nkv, hd, view->page_size, view->num_pages, rt->status, stream));
 }
 
+// For callers with a rotary encoding at hand that is not kept in a GlintRope.
+extern "C" int glint_op_rope_append_with(const GlintRuntime* rt, const GlintStep* step, const float* qkv, void* q_out,
+                                         const GlintView* view, int nh, int nkv, int hd, const double* turns,
+                                         int rotary_dim, int interleaved, float amplitude, cudaStream_t stream) {
+  const GlintRope rope = {turns, rotary_dim, interleaved, amplitude, 1};
+  return glint_op_rope_append(rt, step, qkv, q_out, view, nh, nkv, hd, &rope, stream);
+}
+
 extern "C" int glint_op_cache8_unpack(const GlintRuntime* rt, const GlintStep* step, const GlintView* view, int nkv,
                                       int hd, int window, cudaStream_t stream) {
   if (!view->k_scale || !view->v_scale || !view->k_wide || !view->v_wide) return GLINT_ERR_BAD_ARG;

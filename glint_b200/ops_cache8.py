@@ -14,7 +14,7 @@ one ``Cache8`` belong on one stream, or on streams that wait for each other, gra
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, byref, c_float, c_int, c_void_p
+from ctypes import c_float, c_int, c_void_p
 from dataclasses import dataclass
 
 import torch
@@ -28,16 +28,15 @@ _routed = None
 
 
 def _lib():
-    """The core library with the routed operations of the coded cache typed."""
+    """The core library with the routed operations of the coded cache typed (structures go by address)."""
     global _routed
     if _routed is None:
         lib = native.lib()
-        step, view, rope = POINTER(native.StepStruct), POINTER(native.ViewStruct), POINTER(native.RopeStruct)
-        lib.glint_op_rope_append.argtypes = [c_void_p, step, c_void_p, c_void_p, view, c_int, c_int, c_int, rope, c_void_p]
-        lib.glint_op_cache8_unpack.argtypes = [c_void_p, step, view, c_int, c_int, c_int, c_void_p]
-        lib.glint_op_attention.argtypes = [c_void_p, step, c_void_p, view, c_void_p, c_int, c_int, c_int, c_float, c_float,
-                                           c_int, c_void_p]
-        for f in (lib.glint_op_rope_append, lib.glint_op_cache8_unpack, lib.glint_op_attention):
+        P, I, F = c_void_p, c_int, c_float
+        lib.glint_op_rope_append_with.argtypes = [P, P, P, P, P, I, I, I, P, I, I, F, P]
+        lib.glint_op_cache8_unpack.argtypes = [P, P, P, I, I, I, P]
+        lib.glint_op_attention.argtypes = [P, P, P, P, P, I, I, I, F, F, I, P]
+        for f in (lib.glint_op_rope_append_with, lib.glint_op_cache8_unpack, lib.glint_op_attention):
             f.restype = c_int
         _routed = lib
     return _routed
@@ -76,6 +75,7 @@ class Cache8:
                                         self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.k_wide.data_ptr(),
                                         self.v_wide.data_ptr(), partials.data_ptr(), partials.numel(), arrive.data_ptr(),
                                         arrive.numel())
+        self.addr, self.dtype, self.device_index = ctypes.addressof(self.struct), self.k_wide.dtype, self.k.get_device()
 
     @classmethod
     def empty(cls, num_pages, num_kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda:0"):
@@ -111,7 +111,7 @@ class StepArrays:
             raise KernelError(f"max_seq_len {max_seq_len} and max_context {max_context} do not fit {T} tokens")
         if len(contexts) > R:
             raise KernelError(f"{len(contexts)} contexts for {R} requests")
-        self.tensors, self.num_tokens, self.device = named, T, positions.device
+        self.tensors, self.num_tokens, self.device_index = named, T, positions.get_device()
         contexts = [int(c) for c in contexts]
         s = self.struct = native.StepStruct()
         s.num_tokens, s.num_seqs, s.max_seq_len, s.max_context = T, R, int(max_seq_len), int(max_context)
@@ -121,32 +121,46 @@ class StepArrays:
         s.positions, s.token_seq = positions.data_ptr(), token_seq.data_ptr()
         s.seq_start, s.cu_seqlens = seq_start.data_ptr(), cu_seqlens.data_ptr()
         s.block_table[0], s.max_pages[0] = block_table.data_ptr(), block_table.shape[1]
+        self.addr, self.max_context, self.table_pages = ctypes.addressof(s), int(max_context), block_table.shape[1]
         self.begin()
 
     def begin(self):
         self.struct.id = native.next_step_id()
 
 
+# A step of a few tokens is bound by the host: the checks below compare what is cheap to read (a fraction of a microsecond
+# each) and leave the wording of a refusal to the functions that raise it.
+
+
 def _check(rt, cache, step, window=0):
-    if cache.k_wide.dtype != rt.dtype:
-        raise KernelError(f"the wide pools are {cache.k_wide.dtype}, the runtime is {rt.dtype}")
-    if cache.k.device != rt.device or step.device != rt.device:
-        raise KernelError(f"the cache ({cache.k.device}), the step ({step.device}) and the runtime ({rt.device}) belong to "
-                          f"one device")
+    if cache.dtype is not rt.dtype:
+        raise KernelError(f"the wide pools are {cache.dtype}, the runtime is {rt.dtype}")
+    if not cache.device_index == step.device_index == rt.device_index:
+        raise KernelError(f"the cache (device {cache.device_index}), the step ({step.device_index}) and the runtime "
+                          f"({rt.device_index}) belong to one device")
     if window < 0:
         raise KernelError(f"a window of {window} tokens")
-    if step.struct.max_context > step.struct.max_pages[0] * cache.page_size:
-        raise KernelError(f"a context of {step.struct.max_context} exceeds the block table of {step.struct.max_pages[0]} "
-                          f"pages of {cache.page_size}")
+    if step.max_context > step.table_pages * cache.page_size:
+        raise KernelError(f"a context of {step.max_context} exceeds the block table of {step.table_pages} pages of "
+                          f"{cache.page_size}")
 
 
-def _rows(t, rows, width, dtype, name):
+def _rows(t, rows, width, dtype, name, index):
+    if t.dtype is dtype and t.get_device() == index and t.shape == (rows, width) and t.is_contiguous():
+        return
     ops.require(t, dtype, name)
     if t.dim() != 2 or tuple(t.shape) != (rows, width):
         raise KernelError(f"{name} {tuple(t.shape)} is not [{rows}, {width}]")
+    raise KernelError(f"{name} belongs to device {t.get_device()}, the runtime to {index}")
 
 
-def _run(rc, what):
+def _call(rt, what, fn, *args):
+    """One routed operation on the current stream of the runtime's device."""
+    if torch._C._cuda_getDevice() == rt.device_index:
+        rc = fn(*args, ops.stream())
+    else:
+        with torch.cuda.device(rt.device_index):
+            rc = fn(*args, ops.stream())
     if rc != 0:
         raise KernelError(f"{what}: {ops.error_string(rc)} (code {rc})")
 
@@ -164,33 +178,31 @@ def append(rt, cache, step, qkv, turns, num_heads, q_out=None, layout="half", am
     in 64 bits.  ``amplitude`` scales the turned dims.  A key or value that is not finite makes its page's scale NaN."""
     _check(rt, cache, step)
     _heads(num_heads, cache)
-    if layout not in LAYOUTS:
+    interleaved = LAYOUTS.get(layout)
+    if interleaved is None:
         raise KernelError(f"rotary layout {layout!r} is none of {sorted(LAYOUTS)}")
-    T, hd = step.num_tokens, cache.hd
-    _rows(qkv, T, (num_heads + 2 * cache.nkv) * hd, torch.float32, "qkv")
-    ops.require(turns, torch.float64, "turns")
-    if turns.dim() != 1 or 2 * turns.numel() > hd:
-        raise KernelError(f"turns {tuple(turns.shape)} do not fit heads of {hd}")
+    T, hd, index = step.num_tokens, cache.hd, rt.device_index
+    _rows(qkv, T, (num_heads + 2 * cache.nkv) * hd, torch.float32, "qkv", index)
+    pairs = turns.numel()
+    if turns.dtype is not torch.float64 or turns.get_device() != index or turns.dim() != 1 or 2 * pairs > hd:
+        ops.require(turns, torch.float64, "turns")
+        raise KernelError(f"turns {tuple(turns.shape)} on device {turns.get_device()} do not fit heads of {hd} on device {index}")
     if q_out is None:
-        q_out = torch.empty((T, num_heads * hd), dtype=rt.dtype, device=rt.device)
-    _rows(q_out, T, num_heads * hd, rt.dtype, "q_out")
-    if qkv.device != rt.device or q_out.device != rt.device or turns.device != rt.device:
-        raise KernelError(f"qkv, turns and q_out belong to the runtime's device {rt.device}")
-    rope = native.rope_struct(turns, LAYOUTS[layout], amplitude)
-    with torch.cuda.device(rt.device):
-        _run(_lib().glint_op_rope_append(ctypes.addressof(rt.native), byref(step.struct), ops.ptr(qkv), ops.ptr(q_out),
-                                         byref(cache.struct), num_heads, cache.nkv, hd, byref(rope), ops.stream()),
-             "cache8 append")
+        q_out = qkv.new_empty((T, num_heads * hd), dtype=rt.dtype)
+    else:
+        _rows(q_out, T, num_heads * hd, rt.dtype, "q_out", index)
+    _call(rt, "cache8 append", _lib().glint_op_rope_append_with, ctypes.addressof(rt.native), step.addr, qkv.data_ptr(),
+          q_out.data_ptr(), cache.addr, num_heads, cache.nkv, hd, turns.data_ptr(), 2 * pairs, interleaved, amplitude)
     return q_out
 
 
 def unpack(rt, cache, step, window=0):
     """The values of every page that the step's tokens can reach (through ``window``, or all before them), at the same
     places of the wide pools (returned); other places are left as they were."""
-    _check(rt, cache, step, window or 0)
-    with torch.cuda.device(rt.device):
-        _run(_lib().glint_op_cache8_unpack(ctypes.addressof(rt.native), byref(step.struct), byref(cache.struct), cache.nkv,
-                                           cache.hd, int(window or 0), ops.stream()), "cache8 unpack")
+    window = window or 0
+    _check(rt, cache, step, window)
+    _call(rt, "cache8 unpack", _lib().glint_op_cache8_unpack, ctypes.addressof(rt.native), step.addr, cache.addr, cache.nkv,
+          cache.hd, window)
     return cache.k_wide, cache.v_wide
 
 
@@ -198,17 +210,15 @@ def attention(rt, cache, step, q, num_heads, multiplier, softcap=0.0, window=0, 
     """Attention of the step's queries ``q`` [tokens, heads * head size] (the runtime's dtype) over the coded pages, keys
     and values of the step among them: scores times ``multiplier``, soft cap, keys of the last ``window`` positions (0:
     all).  Returns ``out`` [tokens, heads * head size]."""
-    _check(rt, cache, step, window or 0)
+    window = window or 0
+    _check(rt, cache, step, window)
     _heads(num_heads, cache)
-    T, hd = step.num_tokens, cache.hd
-    _rows(q, T, num_heads * hd, rt.dtype, "q")
+    T, hd, index = step.num_tokens, cache.hd, rt.device_index
+    _rows(q, T, num_heads * hd, rt.dtype, "q", index)
     if out is None:
         out = torch.empty_like(q)
-    _rows(out, T, num_heads * hd, rt.dtype, "out")
-    if q.device != rt.device or out.device != rt.device:
-        raise KernelError(f"q and out belong to the runtime's device {rt.device}")
-    with torch.cuda.device(rt.device):
-        _run(_lib().glint_op_attention(ctypes.addressof(rt.native), byref(step.struct), ops.ptr(q), byref(cache.struct),
-                                       ops.ptr(out), num_heads, cache.nkv, hd, multiplier, softcap or 0.0, int(window or 0),
-                                       ops.stream()), "cache8 attention")
+    else:
+        _rows(out, T, num_heads * hd, rt.dtype, "out", index)
+    _call(rt, "cache8 attention", _lib().glint_op_attention, ctypes.addressof(rt.native), step.addr, q.data_ptr(), cache.addr,
+          out.data_ptr(), num_heads, cache.nkv, hd, multiplier, softcap or 0.0, window)
     return out

@@ -53,6 +53,7 @@ class Runtime:
             raise KernelError("no CUDA device is available: the engine has no CPU path")
         ops.core()  # build or load the kernels now, loudly
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.device_index = self.status.get_device()
         self.shared = {}          # what several parts of a model share (a table of rotation angles), by key
         from . import native
         self.native = native.make_runtime_struct(self)     # the C++ side's view of this runtime

@@ -133,7 +133,7 @@ def test_call_refusals(monkeypatch):
     """Every refusal comes before the launch."""
     _pretend(monkeypatch)
     cache, step = ops_cache8.Cache8(*_tensors()), _step()
-    rt = SimpleNamespace(dtype=torch.bfloat16, device=torch.device("cpu"), native=None)
+    rt = SimpleNamespace(dtype=torch.bfloat16, device_index=-1, native=None)
     qkv, turns = torch.zeros(3, (4 + 4) * 32), torch.zeros(16, dtype=torch.float64)
     q = torch.zeros(3, 4 * 32, dtype=torch.bfloat16)
     for args, kw, what in [((qkv, turns, 3), {}, "evenly"), ((qkv, turns, 0), {}, "evenly"),
@@ -154,9 +154,9 @@ def test_call_refusals(monkeypatch):
     with pytest.raises(KernelError, match="block table"):
         ops_cache8.unpack(rt, cache, far)
     with pytest.raises(KernelError, match="wide"):
-        ops_cache8.unpack(SimpleNamespace(dtype=torch.float32, device=torch.device("cpu")), cache, step)
+        ops_cache8.unpack(SimpleNamespace(dtype=torch.float32, device_index=-1), cache, step)
     with pytest.raises(KernelError, match="one device"):
-        ops_cache8.unpack(SimpleNamespace(dtype=torch.bfloat16, device=torch.device("cuda:0")), cache, step)
+        ops_cache8.unpack(SimpleNamespace(dtype=torch.bfloat16, device_index=0), cache, step)
 
 
 # ---- scaled rotary frequencies -----------------------------------------------------------------------------------
