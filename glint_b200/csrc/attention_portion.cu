@@ -1,0 +1,596 @@
+// Attention of prompt portions over wide pages on the 5th-generation tensor cores, for the coded cache: its pages are
+// widened in front (cache8.cu), this kernel reads them.
+//
+// A block owns 128 query rows, rows being (token, query head of the group) pairs, and walks their keys in tiles of 64.
+// What bounds such a walk here is not the products (a tile of head size 256 takes the tensor pipe 0.55 us) but the soft cap
+// and the exponential of 8,192 scores, two operations of the special-function unit each: 0.55 us of its time if it
+// never pauses.  So nothing waits that need not:
+//   warp 0     TMA: the query tile once, then key and value tiles page by page into two-deep rings
+//   warp 1     tcgen05.mma: S = Q K^T into one of two score buffers of tensor memory, as soon as that has been read
+//   warp 2     tcgen05.mma: O += P V, P (bfloat16 pairs) from one of two buffers of tensor memory
+//   warps 4-7  softmax of the even tiles, warps 8-11 of the odd ones, one thread per row: no maximum or sum is exchanged
+//              within a tile, and one group computes while the other loads, stores and waits
+// With a soft cap of up to 55 the exponentials need no running maximum at all: scores lie within +-cap, so that probabilities
+// relative to cap / 2 lie between 2^-120 (2^-108 for a cap of 50) and 2^40, which float32 sums and bfloat16 probabilities hold
+// with the precision they always have.  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that has
+// grown by more than 8 log2 units, and O is rescaled then).
+// When there are fewer blocks than SMs (a few rows over a long context) the key tiles of a row are split over several
+// blocks, whose partial results a second kernel adds up in order.
+// Blocks are found from the portions' lengths, so that short portions beside long ones cost no empty blocks.
+// Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx; keys of a token at position p from
+// max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit.
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace glint {
+
+constexpr int AT_M = 128;             // query rows of a block
+constexpr int AT_N = 64;              // keys of a tile
+constexpr int AT_THREADS = 384;
+constexpr int AT_Q_SUB = AT_M * 128;  // bytes of a 64-column slice of the query tile
+constexpr int AT_KV_SUB = AT_N * 128;
+constexpr float AT_GROW = 8.f;        // log2 units
+constexpr float AT_FIXED_CAP = 55.f;  // largest soft cap whose exponentials need no maximum
+
+struct PortionParams {
+  const int* cu_seqlens;
+  const int* seq_start;
+  const int* block_table;
+  __nv_bfloat16* out;
+  float* part_o;                // [splits][T * nh][hd], null: one split
+  float2* part_ml;              // [splits][T * nh] (reference in log2 units, sum)
+  int* status;
+  float multiplier, cap;
+  int max_pages, T, nh, nkv, hd, page_size, num_pages, window, n_seqs, whole, per_split;
+};
+
+struct PortionShared {
+  uint64_t q_full, o_full;
+  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], turn[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  float row_ref[AT_M];
+  float row_sum[2][AT_M];
+  float row_own[2][AT_M];
+};
+
+// The (request, query tile) of a block, counted from the last: late tiles have the most keys and start first.  False: none.
+__device__ __forceinline__ bool portion_tile(const int* cu, int n_seqs, int tok_per_tile, int index, int& seq, int& tile) {
+  const int lane = threadIdx.x & 31;
+  int total = 0;
+  for (int b = 0; b < n_seqs; b += 32) {
+    int n = b + lane < n_seqs ? (cu[b + lane + 1] - cu[b + lane] + tok_per_tile - 1) / tok_per_tile : 0;
+    total += __reduce_add_sync(0xffffffffu, max(n, 0));
+  }
+  int at = total - 1 - index;
+  if (at < 0) return false;
+  for (int b = 0; b < n_seqs; b += 32) {
+    const int n = b + lane < n_seqs ? max(0, (cu[b + lane + 1] - cu[b + lane] + tok_per_tile - 1) / tok_per_tile) : 0;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, at < incl);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      seq = b + who;
+      tile = at - __shfl_sync(0xffffffffu, incl - n, who);
+      return true;
+    }
+    at -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+template <bool FIXED>
+__global__ void __launch_bounds__(AT_THREADS, 1)
+attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const PortionParams p) {
+  extern __shared__ uint8_t at_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(at_raw) + 1023) & ~(uintptr_t)1023);
+  const int hd = p.hd, hd16 = hd >> 4, nsub = (hd + 63) >> 6;
+  const int G = p.nh / p.nkv;
+  const int tok_per_tile = AT_M / G;
+  constexpr int TMEM_COLS = 512;
+  uint8_t* sq = smem;
+  uint8_t* sk = sq + (size_t)nsub * AT_Q_SUB;            // [2][nsub][64 keys x 128 B]
+  uint8_t* sv = sk + (size_t)2 * nsub * AT_KV_SUB;
+  PortionShared* sh = reinterpret_cast<PortionShared*>(sv + (size_t)2 * nsub * AT_KV_SUB);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&sh->q_full, 1);
+    tc::mbar_init(&sh->o_full, 1);
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(&sh->s_full[b], 1);
+      tc::mbar_init(&sh->s_free[b], AT_M);
+      tc::mbar_init(&sh->p_ready[b], AT_M);
+      tc::mbar_init(&sh->pv_done[b], 1);
+      tc::mbar_init(&sh->turn[b], AT_M);
+      tc::mbar_init(&sh->k_full[b], 1);
+      tc::mbar_init(&sh->k_empty[b], 1);
+      tc::mbar_init(&sh->v_full[b], 1);
+      tc::mbar_init(&sh->v_empty[b], 1);
+    }
+    sh->abort_flag = 0;
+    tc::fence_barrier_init();
+    tc::tma_prefetch_desc(&map_q);
+    tc::tma_prefetch_desc(&map_k);
+    tc::tma_prefetch_desc(&map_v);
+  }
+  pdl_wait_release();
+  // blockIdx.x counts (query tile from the last, kv head), blockIdx.y the splits
+  int seq = 0, tile = 0;
+  const int kvh = (int)blockIdx.x % p.nkv, split = blockIdx.y;
+  if (!portion_tile(p.cu_seqlens, p.n_seqs, tok_per_tile, (int)blockIdx.x / p.nkv, seq, tile)) return;
+  const int t_begin = p.cu_seqlens[seq];
+  const int q_len = p.cu_seqlens[seq + 1] - t_begin;
+  const int tok0 = tile * tok_per_tile;
+  const int n_tok = min(tok_per_tile, q_len - tok0);
+  const int n_rows = n_tok * G;
+  const int pos0 = p.seq_start[seq] + tok0;
+  const int pos_last = pos0 + n_tok - 1;
+  const int kv_first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+  const int kv_begin = (kv_first & ~(AT_N - 1)) + split * p.per_split * AT_N;     // this split's first tile
+  const int n_tiles = min(p.per_split, (pos_last - kv_begin + AT_N) / AT_N);
+  if (kv_begin > pos_last) return;                       // the rows' keys end before this split (the same for all threads)
+  if (warp == 1) tc::tmem_alloc(&sh->tmem_base, TMEM_COLS);
+  tc::fence_before_thread_sync();
+  __syncthreads();
+  tc::fence_after_thread_sync();
+  const uint32_t tmem_s = sh->tmem_base;                 // two score buffers of 64 columns
+  const uint32_t tmem_p = tmem_s + 2 * AT_N;             // two of P as bfloat16 pairs, 32 columns each
+  const uint32_t tmem_o = tmem_p + AT_N;                 // up to 256 columns
+  volatile int* abort_flag = &sh->abort_flag;
+
+  if (warp == 0) {
+    // ---- producer: the whole warp walks the tiles; lane pi looks up page pi of the next tile, one elected thread issues ----
+    if (tc::elect_one()) {
+      tc::mbar_expect_tx(&sh->q_full, (uint32_t)nsub * tok_per_tile * G * 128);
+      for (int sub = 0; sub < nsub; ++sub)
+        tc::tma_load_4d(sq + (size_t)sub * AT_Q_SUB, &map_q, &sh->q_full, sub * 64, 0, kvh, t_begin + tok0);
+    }
+    __syncwarp();
+    const int ppt = AT_N / p.page_size;                  // pages per tile: 4, 2 or 1
+    const int* table = p.block_table + (size_t)seq * p.max_pages;
+    const int page_lo = kv_first / p.page_size, page_hi = min(pos_last / p.page_size, p.max_pages - 1);
+    const int first_page = kv_begin / p.page_size;
+    // pages outside [page_lo, page_hi] are masked; they are filled from page 0, which is finite as all wide values are
+    auto fetch = [&](int j) -> int {
+      const int page_idx = first_page + j * ppt + lane;
+      return lane < ppt ? table[min(max(page_idx, page_lo), page_hi)] : 0;
+    };
+    int next = fetch(0);
+    bool ok = true;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int b = j & 1;
+      int mine = next;
+      const int page_idx = first_page + j * ppt + lane;
+      if (lane >= ppt || page_idx < page_lo || page_idx > page_hi) {
+        mine = 0;
+      } else if (mine < 0 || mine >= p.num_pages) {
+        atomicExch(p.status, 3);
+        mine = 0;
+      }
+      if (j + 1 < n_tiles) next = fetch(j + 1);
+      int pages[4];
+#pragma unroll
+      for (int pi = 0; pi < 4; ++pi) pages[pi] = __shfl_sync(0xffffffffu, mine, pi);
+      for (int which = 0; which < 2 && ok; ++which) {    // keys first: they are needed first
+        uint64_t* full = which ? &sh->v_full[b] : &sh->k_full[b];
+        if (j >= 2) ok = tc::mbar_wait(which ? &sh->v_empty[b] : &sh->k_empty[b], ((j >> 1) - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (tc::elect_one()) {
+          tc::mbar_expect_tx(full, (uint32_t)nsub * AT_KV_SUB);
+          const CUtensorMap* map = which ? &map_v : &map_k;
+          uint8_t* ring = (which ? sv : sk) + (size_t)b * nsub * AT_KV_SUB;
+          if (p.whole && which) {                        // values: a box per page, [slice][row of the page][64 columns]
+#pragma unroll
+            for (int pi = 0; pi < 4; ++pi)
+              if (pi < ppt)
+                tc::tma_load_3d(ring + (size_t)pi * nsub * p.page_size * 128, map, full, 0, (pages[pi] * p.nkv + kvh) * p.page_size, 0);
+          } else if (p.whole) {                          // keys: a box per 8 rows, [slice][8 rows][64 columns]
+#pragma unroll
+            for (int a = 0; a < AT_N / 8; ++a) {
+              const int key = a * 8;
+              const int pg = p.page_size == 16 ? pages[a >> 1] : p.page_size == 32 ? pages[a >> 2] : pages[0];
+              tc::tma_load_3d(ring + (size_t)a * nsub * 1024, map, full, 0, (pg * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1)), 0);
+            }
+          } else {
+#pragma unroll
+            for (int pi = 0; pi < 4; ++pi) {
+              if (pi < ppt) {
+                const int row = (pages[pi] * p.nkv + kvh) * p.page_size;
+                uint8_t* dst = ring + (size_t)pi * p.page_size * 128;
+                for (int sub = 0; sub < nsub; ++sub) tc::tma_load_2d(dst + (size_t)sub * AT_KV_SUB, map, full, sub * 64, row);
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    // ---- S = Q K^T, a tile ahead of the softmax as soon as a score buffer has been read -----------------------------------
+    if (tc::elect_one()) {
+      const uint32_t idesc = tc::idesc_bf16_f32(AT_M, AT_N);
+      const uint64_t qd = tc::smem_desc_k_sw128(tc::smem_u32(sq));
+      const uint32_t k_slice = p.whole ? 1024u : (uint32_t)AT_KV_SUB;          // bytes between slices of keys
+      const uint32_t k_sbo = p.whole ? (uint32_t)nsub * 1024u : 1024u;         // bytes between groups of 8 keys
+      const uint64_t kd0 = tc::smem_desc_k_sw128_sbo(tc::smem_u32(sk), k_sbo);
+      const uint32_t k_tile = ((uint32_t)nsub * AT_KV_SUB) >> 4;
+      bool ok = tc::mbar_wait(&sh->q_full, 0, abort_flag);
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int b = j & 1;
+        if (j >= 2) ok = tc::mbar_wait(&sh->s_free[b], ((j >> 1) - 1) & 1, abort_flag);
+        if (ok) ok = tc::mbar_wait(&sh->k_full[b], (j >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc::fence_after_thread_sync();
+        const uint32_t d = tmem_s + b * AT_N;
+        const uint64_t kd = kd0 + b * k_tile;
+#pragma unroll
+        for (int ks = 0; ks < 16; ++ks) {
+          if (ks < hd16) {
+            const uint32_t oq = ((ks >> 2) * AT_Q_SUB + (ks & 3) * 32) >> 4;
+            const uint32_t ok_ = ((ks >> 2) * k_slice + (ks & 3) * 32) >> 4;
+            tc::mma_bf16_ss(d, qd + oq, kd + ok_, idesc, ks > 0 ? 1u : 0u);
+          }
+        }
+        tc::mma_commit(&sh->s_full[b]);
+        tc::mma_commit(&sh->k_empty[b]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---- O += P V --------------------------------------------------------------------------------------------------------
+    if (tc::elect_one()) {
+      const uint32_t idesc = tc::idesc_bf16_f32_b_mn(AT_M, hd);
+      const uint32_t v_lbo = p.whole ? (uint32_t)p.page_size * 128u : (uint32_t)AT_KV_SUB;
+      const uint32_t v_page = (uint32_t)nsub * p.page_size * 128u;             // whole boxes: bytes of a page
+      const uint64_t vd0 = tc::smem_desc_mn_sw128(tc::smem_u32(sv), v_lbo, 1024);
+      const uint32_t v_tile = ((uint32_t)nsub * AT_KV_SUB) >> 4;
+      uint32_t v_step[AT_N / 16];                                              // start of keys 16 kk, in 16 bytes
+#pragma unroll
+      for (int kk = 0; kk < AT_N / 16; ++kk)
+        v_step[kk] = p.whole ? (((kk * 16) / p.page_size) * v_page + ((kk * 16) % p.page_size) * 128u) >> 4
+                             : (uint32_t)(kk * 2048) >> 4;
+      bool ok = true;
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int b = j & 1;
+        ok = tc::mbar_wait(&sh->v_full[b], (j >> 1) & 1, abort_flag);
+        if (ok) ok = tc::mbar_wait(&sh->p_ready[b], (j >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc::fence_after_thread_sync();
+#pragma unroll
+        for (int kk = 0; kk < AT_N / 16; ++kk)
+          tc::mma_bf16_ts(tmem_o, tmem_p + b * (AT_N / 2) + 8 * kk, vd0 + b * v_tile + v_step[kk], idesc, (j > 0 || kk > 0) ? 1u : 0u);
+        tc::mma_commit(&sh->v_empty[b]);
+        tc::mma_commit(&sh->pv_done[b]);
+      }
+      tc::mma_commit(&sh->o_full);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---- softmax: group 0 takes the even tiles, group 1 the odd ones; a thread has a row -------------------------------
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    const int r = quarter * 32 + lane;
+    const bool rv = r < n_rows;
+    const int qpos = pos0 + (rv ? r / G : 0);
+    const int lo = p.window > 0 ? qpos - p.window + 1 : 0;
+    const uint32_t lane_base = ((uint32_t)(quarter * 32) << 16);
+    const uint32_t my_s = tmem_s + group * AT_N + lane_base, my_p = tmem_p + group * (AT_N / 2) + lane_base;
+    const float LOG2E = 1.4426950408889634f;
+    const float in_scale = p.cap > 0.f ? p.multiplier / p.cap : p.multiplier;
+    const float out_scale = p.cap > 0.f ? p.cap * LOG2E : LOG2E;   // scores are kept in log2 units
+    const float fixed_ref = 0.5f * out_scale;
+    float ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = group; j < n_tiles; j += 2) {
+      ok = tc::mbar_wait(&sh->s_full[group], (j >> 1) & 1, abort_flag);
+      if (!ok) break;
+      tc::fence_after_thread_sync();
+      uint32_t raw[AT_N];
+#pragma unroll
+      for (int c0 = 0; c0 < AT_N; c0 += 16) tc::tmem_ld_16(my_s + c0, raw + c0);
+      tc::tmem_ld_wait();
+      tc::fence_before_thread_sync();
+      tc::mbar_arrive(&sh->s_free[group]);
+      const int key0 = kv_begin + j * AT_N;
+      // scores in log2 units; FIXED: less the fixed reference
+      if (FIXED || p.cap > 0.f) {
+#pragma unroll
+        for (int c = 0; c < AT_N; ++c) {
+          const float v = tc::tanh_approx(__uint_as_float(raw[c]) * in_scale);
+          raw[c] = __float_as_uint(FIXED ? fmaf(v, out_scale, -fixed_ref) : v * out_scale);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < AT_N; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) * (in_scale * out_scale));
+      }
+      // most tiles lie wholly inside every row's range
+      if (!__all_sync(0xffffffffu, rv && key0 >= lo && key0 + AT_N - 1 <= qpos)) {
+#pragma unroll
+        for (int c = 0; c < AT_N; ++c)
+          if (!(rv && key0 + c <= qpos && key0 + c >= lo)) raw[c] = 0xff800000u;      // -inf
+      }
+      if (!FIXED) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < AT_N; ++c) top = fmaxf(top, __uint_as_float(raw[c]));
+        // the row's reference comes from the tile before, goes to the tile behind
+        if (j > 0) ok = tc::mbar_wait(&sh->turn[group], ((j + group) / 2 - 1) & 1, abort_flag);
+        if (!ok) break;
+        const float before = j > 0 ? sh->row_ref[r] : -INFINITY;
+        const bool grow = top > before + AT_GROW || (before == -INFINITY && top > -INFINITY);
+        const float now = grow ? top : before;
+        if (grow || j == 0) sh->row_ref[r] = now;
+        tc::mbar_arrive(&sh->turn[group ^ 1]);
+        if (now != ref) {                                // what this group has summed so far follows
+          l *= ref == -INFINITY ? 0.f : tc::exp2_approx(ref - now);
+          ref = now;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {    // O follows when the product of the tile before is in
+          ok = tc::mbar_wait(&sh->pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag);
+          if (!ok) break;
+          tc::fence_after_thread_sync();
+          const float corr = grow ? (before == -INFINITY ? 0.f : tc::exp2_approx(before - now)) : 1.f;
+          for (int c0 = 0; c0 < hd; c0 += 16) {
+            uint32_t o[16];
+            tc::tmem_ld_16(tmem_o + lane_base + c0, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tc::tmem_st_16(tmem_o + lane_base + c0, o);
+          }
+          tc::tmem_st_wait();
+        }
+      }
+      const float base = FIXED || ref == -INFINITY ? 0.f : ref;
+      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < AT_N; c += 2) {
+        const float p0 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c]) : __uint_as_float(raw[c]) - base);
+        const float p1 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c + 1]) : __uint_as_float(raw[c + 1]) - base);
+        l4[c & 3] += p0;
+        l4[(c + 1) & 3] += p1;
+        const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+        raw[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      if (j >= 2) ok = tc::mbar_wait(&sh->pv_done[group], ((j >> 1) - 1) & 1, abort_flag);     // P of two tiles ago was read
+      if (!ok) break;
+      tc::fence_after_thread_sync();
+      tc::tmem_st_16(my_p, raw);
+      tc::tmem_st_16(my_p + 16, raw + 16);
+      tc::tmem_st_wait();
+      tc::fence_before_thread_sync();
+      tc::mbar_arrive(&sh->p_ready[group]);
+    }
+    // ---- epilogue: O over the row's sum, a half of the columns each --------------------------------------------------
+    sh->row_sum[group][r] = l;
+    sh->row_own[group][r] = ref;
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    if (ok) ok = tc::mbar_wait(&sh->o_full, 0, abort_flag);
+    if (ok) {
+      tc::fence_after_thread_sync();
+      float total = sh->row_sum[0][r] + sh->row_sum[1][r], last = 0.f;
+      if (!FIXED) {
+        last = sh->row_ref[r];
+        total = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          if (sh->row_own[b][r] != -INFINITY) total += sh->row_sum[b][r] * tc::exp2_approx(sh->row_own[b][r] - last);
+          else total += sh->row_sum[b][r];               // 0, or NaN where every score was
+      }
+      const int o_lo = group ? ((hd16 + 1) >> 1) * 16 : 0, o_hi = group ? hd : ((hd16 + 1) >> 1) * 16;
+      const size_t row = (size_t)(t_begin + tok0 + (rv ? r / G : 0)) * p.nh + kvh * G + (rv ? r % G : 0);
+      const float inv = p.part_o ? 1.f : total == 0.f ? 0.f : 1.0f / total;
+      if (p.part_o && rv && group == 0) p.part_ml[(size_t)split * p.T * p.nh + row] = make_float2(last, total);
+      for (int c0 = o_lo; c0 < o_hi; c0 += 16) {
+        uint32_t o[16];
+        tc::tmem_ld_16(tmem_o + lane_base + c0, o);
+        tc::tmem_ld_wait();
+        if (!rv) continue;
+        if (p.part_o) {
+          float4* to = reinterpret_cast<float4*>(p.part_o + ((size_t)split * p.T * p.nh + row) * hd + c0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            to[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+        } else {
+          uint32_t h[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            h[i] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          uint4* to = reinterpret_cast<uint4*>(p.out + row * hd + c0);
+          to[0] = make_uint4(h[0], h[1], h[2], h[3]);
+          to[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+      }
+    }
+  }
+  tc::fence_before_thread_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_thread_sync();
+    tc::tmem_dealloc(sh->tmem_base, TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && sh->abort_flag) atomicExch(p.status, 4);
+}
+
+// Adds up the splits of every row, in order: a warp per row.
+__global__ void __launch_bounds__(256) attention_portion_merge_kernel(const PortionParams p) {
+  pdl_wait_release();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int t = row / p.nh;
+  // the request of the token: portions are few, and their offsets ascend
+  int seq = -1;
+  for (int b = 0; b < p.n_seqs && seq < 0; b += 32) {
+    const bool here = b + lane < p.n_seqs && p.cu_seqlens[b + lane] <= t && t < p.cu_seqlens[b + lane + 1];
+    const unsigned hit = __ballot_sync(0xffffffffu, here);
+    if (hit) seq = b + __ffs(hit) - 1;
+  }
+  if (t >= p.T || seq < 0) return;                       // a token in front of the portions
+  const int G = p.nh / p.nkv, tok_per_tile = AT_M / G;
+  const int tok0 = (t - p.cu_seqlens[seq]) / tok_per_tile * tok_per_tile;
+  const int q_len = p.cu_seqlens[seq + 1] - p.cu_seqlens[seq];
+  const int pos0 = p.seq_start[seq] + tok0, pos_last = pos0 + min(tok_per_tile, q_len - tok0) - 1;
+  const int kv_begin = (p.window > 0 ? max(0, pos0 - p.window + 1) : 0) & ~(AT_N - 1);
+  const int parts = ((pos_last - kv_begin) / AT_N + p.per_split) / p.per_split;
+  const size_t stride = (size_t)p.T * p.nh;
+  float M = -INFINITY;
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.part_ml[s * stride + row].x);
+  float L = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = p.part_ml[s * stride + row];
+    // a split whose keys are all masked for this row has no reference and L = 0; one whose scores were NaN has L = NaN
+    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : tc::exp2_approx(ml.x - M);
+    L += ml.y * w;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int d = lane * 4 + k * 128;
+      if (d < p.hd) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * stride + row) * p.hd + d);
+        acc[k].x += v.x * w; acc[k].y += v.y * w; acc[k].z += v.z * w; acc[k].w += v.w * w;
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = lane * 4 + k * 128;
+    if (d < p.hd) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv), b = __floats2bfloat162_rn(acc[k].z * inv, acc[k].w * inv);
+      *reinterpret_cast<uint2*>(p.out + (size_t)row * p.hd + d) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------
+
+typedef CUresult (*AtEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static AtEncodeFn at_encode_fn() {
+  static AtEncodeFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<AtEncodeFn>(ptr);
+  }
+  return fn;
+}
+
+static int at_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                  const cuuint32_t* box) {
+  AtEncodeFn fn = at_encode_fn();
+  if (!fn) return GLINT_ERR_BAD_ARG;
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? GLINT_OK : GLINT_ERR_BAD_ARG;
+}
+
+}  // namespace glint
+
+using namespace glint;
+
+// head_dim a multiple of 16 up to 256; at most 128 query heads per kv head; pages of 16, 32 or 64.
+GLINT_API int glint_attention_portion_supported(int nh, int nkv, int hd, int page_size) {
+  return (nkv > 0 && nh % nkv == 0 && nh / nkv <= AT_M && hd % 16 == 0 && hd >= 16 && hd <= 256 &&
+          (page_size == 16 || page_size == 32 || page_size == 64)) ? 1 : 0;
+}
+
+// q, out: [T, nh * hd] bf16; pools [pages][nkv][page_size][hd] bf16, finite everywhere; cu_seqlens (absolute token offsets),
+// seq_start and block_table of the n_seqs portions, of which none is longer than max_q_len or attends more than
+// max_context keys.  `scratch`: floats for partial results, 16-byte aligned (none, or too few: the keys are not split).
+GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const void* v_pool, const int* cu_seqlens,
+                                      const int* seq_start, const int* block_table, int max_pages, void* out, int T,
+                                      int n_seqs, int max_q_len, int max_context, int nh, int nkv, int hd, int page_size,
+                                      int num_pages, float multiplier, float cap, int window, int sms, float* scratch,
+                                      long long scratch_floats, int* status, cudaStream_t stream) {
+  if (n_seqs <= 0 || max_q_len <= 0 || T <= 0) return GLINT_OK;
+  if (!glint_attention_portion_supported(nh, nkv, hd, page_size)) return GLINT_ERR_UNSUPPORTED_SIZE;
+  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) return GLINT_ERR_UNSUPPORTED_SIZE;
+  if ((long long)num_pages * nkv * page_size > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
+  const int G = nh / nkv;
+  const int tok_per_tile = AT_M / G;
+  CUtensorMap map_q, map_k, map_v;
+  {
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)G, (cuuint64_t)nkv, (cuuint64_t)T};
+    const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)G * hd * 2, (cuuint64_t)nh * hd * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)G, 1, (cuuint32_t)tok_per_tile};
+    const int rc = at_map(&map_q, q, 4, dims, strides, box);
+    if (rc != GLINT_OK) return rc;
+  }
+  // With head_dim a multiple of 64 the 64-column slices are a third dimension of the pools, and one box brings all
+  // slices of its rows (the copy unit spends about 65 cycles on a box whatever its size).
+  const int whole = hd % 64 == 0 ? 1 : 0;
+  const cuuint64_t rows = (cuuint64_t)num_pages * nkv * page_size;
+  int rc;
+  if (whole) {
+    const cuuint64_t dims[3] = {64, rows, (cuuint64_t)(hd / 64)};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, 128};
+    const cuuint32_t box_k[3] = {64, 8, (cuuint32_t)(hd / 64)};
+    const cuuint32_t box_v[3] = {64, (cuuint32_t)page_size, (cuuint32_t)(hd / 64)};
+    rc = at_map(&map_k, k_pool, 3, dims, strides, box_k);
+    if (rc == GLINT_OK) rc = at_map(&map_v, v_pool, 3, dims, strides, box_v);
+  } else {
+    const cuuint64_t dims[2] = {(cuuint64_t)hd, rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)page_size};
+    rc = at_map(&map_k, k_pool, 2, dims, strides, box);
+    if (rc == GLINT_OK) rc = at_map(&map_v, v_pool, 2, dims, strides, box);
+  }
+  if (rc != GLINT_OK) return rc;
+  PortionParams p = {};
+  p.cu_seqlens = cu_seqlens; p.seq_start = seq_start; p.block_table = block_table; p.max_pages = max_pages; p.T = T;
+  p.out = (__nv_bfloat16*)out; p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.num_pages = num_pages;
+  p.multiplier = multiplier; p.cap = cap; p.window = window; p.whole = whole; p.status = status; p.n_seqs = n_seqs;
+  const int nsub = (hd + 63) / 64;
+  const int smem = nsub * AT_Q_SUB + 4 * nsub * AT_KV_SUB + (int)sizeof(PortionShared) + 1024;
+  // at most a tile more than whole ones for every portion
+  const long long blocks = ((long long)T / tok_per_tile + n_seqs) * nkv;
+  if (blocks > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
+  // Fewer blocks than SMs: their keys are split, as far as that makes work for all SMs and leaves a split four tiles.
+  const long long reach = window > 0 && (long long)window + max_q_len < max_context ? (long long)window + max_q_len + AT_N : max_context;
+  const int most_tiles = (int)((reach + AT_N - 1) / AT_N);
+  int splits = (int)(sms / blocks);
+  if (splits > most_tiles / 4) splits = most_tiles / 4;
+  const long long part = (long long)T * nh * (hd + 2);
+  if (splits > 1 && (!scratch || ((uintptr_t)scratch & 15) || part * splits > scratch_floats))
+    splits = scratch && !((uintptr_t)scratch & 15) ? (int)(scratch_floats / part) : 1;
+  if (splits < 1) splits = 1;
+  p.per_split = (most_tiles + splits - 1) / splits;
+  splits = (most_tiles + p.per_split - 1) / p.per_split;
+  if (splits > 1) {
+    p.part_o = scratch;
+    p.part_ml = reinterpret_cast<float2*>(scratch + (long long)splits * T * nh * hd);
+  } else {
+    p.per_split = 0x7fffff;                              // all of them, whatever max_context said
+  }
+  const dim3 grid((unsigned)blocks, splits);
+  const bool fixed = cap > 0.f && cap <= AT_FIXED_CAP;
+  cudaError_t e = cudaSuccess;
+#define LAUNCH(FIXED)                                                                                             \
+  {                                                                                                               \
+    e = cudaFuncSetAttribute(attention_portion_kernel<FIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
+    if (e == cudaSuccess)                                                                                         \
+      e = launch_kernel(attention_portion_kernel<FIXED>, grid, dim3(AT_THREADS), (size_t)smem, stream, map_q, map_k, map_v, p); \
+  }
+  if (fixed) LAUNCH(true) else LAUNCH(false)
+#undef LAUNCH
+  if (e == cudaSuccess && splits > 1)
+    e = launch_kernel(attention_portion_merge_kernel, dim3((unsigned)(((long long)T * nh + 7) / 8)), dim3(256), 0, stream, p);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}

@@ -32,7 +32,8 @@ NVCC_FLAGS += os.environ.get("GLINT_NVCC_EXTRA", "").split()
 
 LIBRARIES = {
     "core": ["elementwise.cu", "cache8.cu", "gemm_plain.cu", "attention_plain.cu", "sampling.cu", "sample_noalloc.cu", "runtime.cu"],
-    "tensor": ["gemm_tcgen05.cu", "gemm_skinny.cu", "attention_decode.cu", "attention_decode8.cu", "attention_prefill.cu", "attention_tcgen05.cu"],
+    "tensor": ["gemm_tcgen05.cu", "gemm_skinny.cu", "attention_decode.cu", "attention_decode8.cu", "attention_portion.cu",
+               "attention_prefill.cu", "attention_tcgen05.cu"],
     "host": ["host/cache_core.cpp"],
 }
 HEADERS = ["common.cuh", "tcgen05.cuh", "noalloc.h", "runtime.h"]

@@ -80,6 +80,7 @@ bool tiled_attention_supported(int nh, int nkv, int hd, int page) {
   return nkv > 0 && nh % nkv == 0 && nh / nkv <= 128 && hd % 16 == 0 && hd >= 16 && hd <= 256 &&
          (page == 16 || page == 32 || page == 64);
 }
+constexpr long long FEW_TOKEN_BYTES = 32ll << 20;   // codes read in all, up to which any tokens take the single-token kernel
 constexpr int SPLIT_SINGLES_FROM = 4096;   // context from which single tokens in front of portions leave the tiled kernel
 constexpr int SPLIT_SINGLES_UP_TO = 8;     // so few of them leave it at any context
 
@@ -310,7 +311,11 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
   const bool single = rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_decode8 && view->partials && view->arrive &&
                       t.attention_decode8_supported(nh, nkv, hd, page) &&
                       t.attention_decode8_workspace(blocks, nh, nkv, hd) <= view->partial_floats;
-  const int lead = !single ? 0 : step->max_seq_len == 1 ? step->num_tokens : step->leading_single;
+  // Few tokens over little cache take the single-token kernel whatever the portions: it reads the codes once for every
+  // token, but in one launch of many warps
+  const int reach = window > 0 && window < step->max_context ? window : step->max_context;
+  const bool few = (long long)step->num_tokens * reach * nkv * hd * 2 <= FEW_TOKEN_BYTES;
+  const int lead = !single ? 0 : step->max_seq_len == 1 || few ? step->num_tokens : step->leading_single;
   if (lead > 0) {
     const int rc = counted(t.attention_decode8(
         q, (const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale, step->positions, step->token_seq,
@@ -330,6 +335,12 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
   wide.k = view->k_wide;
   wide.v = view->v_wide;
   wide.k_scale = wide.v_scale = nullptr;
+  if (rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_portion && rest.max_seq_len > 1 &&
+      t.attention_portion_supported(nh, nkv, hd, page))
+    return counted(t.attention_portion(q, wide.k, wide.v, rest.cu_seqlens, rest.seq_start, rest.block_table[g], rest.max_pages[g],
+                                       out, step->num_tokens, rest.num_seqs, rest.max_seq_len, rest.max_context, nh, nkv, hd, page,
+                                       view->num_pages, multiplier, cap, window, rt->sms, view->partials, view->partial_floats,
+                                       rt->status, stream));
   return glint_op_attention(rt, lead ? &rest : step, q, &wide, out, nh, nkv, hd, multiplier, cap, window, stream);
 }
 

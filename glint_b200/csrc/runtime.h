@@ -56,6 +56,9 @@ struct GlintTensorEntries {
                            int, int*, cudaStream_t);
   int (*attention_decode8_supported)(int, int, int, int);
   long long (*attention_decode8_workspace)(int, int, int, int);
+  int (*attention_portion)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int, int, int,
+                           int, int, int, int, int, int, float, float, int, int, float*, long long, int*, cudaStream_t);
+  int (*attention_portion_supported)(int, int, int, int);
   int (*attention_prefill)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int,
                            int, int, int, int, int, int, float, float, int, int*, cudaStream_t);
   int (*attention_tcgen05)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int,
@@ -105,8 +108,8 @@ struct GlintView {
   float* v_scale;
   void* k_wide;
   void* v_wide;
-  float* partials;              // scratch of the single-token attention over codes: partial results, and counters that are
-  long long partial_floats;     // zero between launches
+  float* partials;              // scratch of the attention over codes: partial results, and counters that are zero between
+  long long partial_floats;     // launches
   int* arrive;
   int arrive_ints;
 };

@@ -38,7 +38,7 @@ class TensorEntries(Structure):
                                               "attention_decode", "attention_decode_stream_plan",
                                               "attention_decode_stream", "attention_decode8",
                                               "attention_decode8_supported", "attention_decode8_workspace",
-                                              "attention_prefill", "attention_tcgen05")]
+                                              "attention_portion", "attention_portion_supported", "attention_prefill", "attention_tcgen05")]
 
 
 ATTN_PLANS = 8
@@ -70,11 +70,12 @@ CACHE8_ARRIVE = 65536        # pairs of a token and a kv head that one launch of
 
 
 def cache8_scratch(num_kv_heads, head_dim, device):
-    """Scratch of the single-token attention over coded pages, for up to 8 query heads a pair and two blocks per SM:
-    (partial results float32, arrival counters int32, zero between launches).  It belongs to one cache, like the wide pages:
-    launches on one stream share it."""
-    blocks = 2 * torch.cuda.get_device_properties(device).multi_processor_count if torch.device(device).type == "cuda" else 1
-    return (torch.empty(blocks * 2 * 8 * (head_dim + 4), dtype=torch.float32, device=device),
+    """Scratch of the attention over coded pages: (partial results float32, arrival counters int32, zero between launches),
+    enough for single tokens with 8 query heads a pair on two blocks per SM and for portions whose keys are split over as many
+    blocks of 128 rows as the SMs hold.  It belongs to one cache, like the wide pages: launches on one stream share it."""
+    sms = torch.cuda.get_device_properties(device).multi_processor_count if torch.device(device).type == "cuda" else 1
+    rows = 128 * sms
+    return (torch.empty(max(2 * sms * 2 * 8 * (head_dim + 4), rows * (head_dim + 2)), dtype=torch.float32, device=device),
             torch.zeros(CACHE8_ARRIVE, dtype=torch.int32, device=device))
 
 
