@@ -500,7 +500,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             vs = 1.f;
           }
           if (vs == 0.f) vs = 7.5231638e-37f;                   // 2^-120: a page that nothing was written to
-          if (tc::mbar_wait(&sh->full[stage], phase, abort_flag)) {
+          if (__all_sync(0xffffffffu, tc::mbar_wait(&sh->full[stage], phase, abort_flag))) {   // together: what follows is .aligned
             const uint32_t kaddr = lane_addr + (uint32_t)stage * 2 * page_bytes;
             d8_page<HD, FULL>(st, qy, kaddr, kaddr + page_bytes, ks, vs, (sg.page_lo + off + it - it0) * p.page_size, pos, sg.first,
                               p.page_size, hd, sub_bytes, cap2, lane);

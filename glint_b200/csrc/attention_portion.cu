@@ -5,7 +5,8 @@
 // What bounds such a walk here is not the products (a tile of head size 256 takes the tensor pipe 0.55 us) but the soft cap
 // and the exponential of 8,192 scores, two operations of the special-function unit each: 0.55 us of its time if it
 // never pauses.  So nothing waits that need not:
-//   warp 0     TMA: the query tile once, then key and value tiles page by page into two-deep rings
+//   warps 0, 3 TMA: the query tile once and key tiles; value tiles: page by page into rings as deep as shared memory allows
+//              (head size 256: three tiles of keys, two of values)
 //   warp 1     tcgen05.mma: S = Q K^T into one of two score buffers of tensor memory, as soon as that has been read
 //   warp 2     tcgen05.mma: O += P V, P (bfloat16 pairs) from one of two buffers of tensor memory
 //   warps 4-7  softmax of the even tiles, warps 8-11 of the odd ones, one thread per row: no maximum or sum is exchanged
@@ -29,6 +30,7 @@ constexpr int AT_N = 64;              // keys of a tile
 constexpr int AT_THREADS = 384;
 constexpr int AT_Q_SUB = AT_M * 128;  // bytes of a 64-column slice of the query tile
 constexpr int AT_KV_SUB = AT_N * 128;
+constexpr int AT_STAGES = 4;          // most tiles of keys, or of values, in shared memory
 constexpr float AT_GROW = 8.f;        // log2 units
 constexpr float AT_FIXED_CAP = 55.f;  // largest soft cap whose exponentials need no maximum
 
@@ -41,19 +43,24 @@ struct PortionParams {
   float2* part_ml;              // [splits][T * nh] (reference in log2 units, sum)
   int* status;
   float multiplier, cap;
-  int max_pages, T, nh, nkv, hd, page_size, num_pages, window, n_seqs, whole, per_split;
+  int max_pages, T, nh, nkv, hd, page_size, num_pages, window, n_seqs, whole, per_split, k_stages, v_stages;
 };
 
 struct PortionShared {
   uint64_t q_full, o_full;
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], turn[2];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t k_full[AT_STAGES], k_empty[AT_STAGES], v_full[AT_STAGES], v_empty[AT_STAGES];
   uint32_t tmem_base;
   int abort_flag;
   float row_ref[AT_M];
   float row_sum[2][AT_M];
   float row_own[2][AT_M];
 };
+
+// A wait of a whole warp: its lanes go on together (what follows is .aligned), or not at all.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
+}
 
 // The (request, query tile) of a block, counted from the last: late tiles have the most keys and start first.  False: none.
 __device__ __forceinline__ bool portion_tile(const int* cu, int n_seqs, int tok_per_tile, int index, int& seq, int& tile) {
@@ -89,16 +96,16 @@ template <bool FIXED>
 __global__ void __launch_bounds__(AT_THREADS, 1)
 attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const PortionParams p) {
-  extern __shared__ uint8_t at_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(at_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t at_raw[];    // begins at a multiple of 1024: there is no room for less (checked)
+  uint8_t* smem = at_raw;
   const int hd = p.hd, hd16 = hd >> 4, nsub = (hd + 63) >> 6;
   const int G = p.nh / p.nkv;
   const int tok_per_tile = AT_M / G;
   constexpr int TMEM_COLS = 512;
   uint8_t* sq = smem;
-  uint8_t* sk = sq + (size_t)nsub * AT_Q_SUB;            // [2][nsub][64 keys x 128 B]
-  uint8_t* sv = sk + (size_t)2 * nsub * AT_KV_SUB;
-  PortionShared* sh = reinterpret_cast<PortionShared*>(sv + (size_t)2 * nsub * AT_KV_SUB);
+  uint8_t* sk = sq + (size_t)nsub * AT_Q_SUB;            // [stages][nsub][64 keys x 128 B]
+  uint8_t* sv = sk + (size_t)p.k_stages * nsub * AT_KV_SUB;
+  PortionShared* sh = reinterpret_cast<PortionShared*>(sv + (size_t)p.v_stages * nsub * AT_KV_SUB);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -110,6 +117,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       tc::mbar_init(&sh->p_ready[b], AT_M);
       tc::mbar_init(&sh->pv_done[b], 1);
       tc::mbar_init(&sh->turn[b], AT_M);
+    }
+    for (int b = 0; b < AT_STAGES; ++b) {
       tc::mbar_init(&sh->k_full[b], 1);
       tc::mbar_init(&sh->k_empty[b], 1);
       tc::mbar_init(&sh->v_full[b], 1);
@@ -122,6 +131,10 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     tc::tma_prefetch_desc(&map_v);
   }
   pdl_wait_release();
+  if (tc::smem_u32(at_raw) & 1023) {                     // the operands' swizzle wants it
+    if (threadIdx.x == 0) atomicExch(p.status, 4);
+    return;
+  }
   // blockIdx.x counts (query tile from the last, kv head), blockIdx.y the splits
   int seq = 0, tile = 0;
   const int kvh = (int)blockIdx.x % p.nkv, split = blockIdx.y;
@@ -146,9 +159,11 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const uint32_t tmem_o = tmem_p + AT_N;                 // up to 256 columns
   volatile int* abort_flag = &sh->abort_flag;
 
-  if (warp == 0) {
-    // ---- producer: the whole warp walks the tiles; lane pi looks up page pi of the next tile, one elected thread issues ----
-    if (tc::elect_one()) {
+  if (warp == 0 || warp == 3) {
+    // ---- producers, of keys and of values: each at the pace of its own ring.  The whole warp walks the tiles; lane pi looks
+    // up page pi of the next tile, one elected thread issues. ----------------------------------------------------------
+    const bool values = warp == 3;
+    if (!values && tc::elect_one()) {
       tc::mbar_expect_tx(&sh->q_full, (uint32_t)nsub * tok_per_tile * G * 128);
       for (int sub = 0; sub < nsub; ++sub)
         tc::tma_load_4d(sq + (size_t)sub * AT_Q_SUB, &map_q, &sh->q_full, sub * 64, 0, kvh, t_begin + tok0);
@@ -158,15 +173,19 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const int* table = p.block_table + (size_t)seq * p.max_pages;
     const int page_lo = kv_first / p.page_size, page_hi = min(pos_last / p.page_size, p.max_pages - 1);
     const int first_page = kv_begin / p.page_size;
+    const CUtensorMap* map = values ? &map_v : &map_k;
+    uint64_t* full = values ? sh->v_full : sh->k_full;
+    uint64_t* empty = values ? sh->v_empty : sh->k_empty;
+    uint8_t* ring = values ? sv : sk;
+    const int stages = values ? p.v_stages : p.k_stages;
     // pages outside [page_lo, page_hi] are masked; they are filled from page 0, which is finite as all wide values are
     auto fetch = [&](int j) -> int {
       const int page_idx = first_page + j * ppt + lane;
       return lane < ppt ? table[min(max(page_idx, page_lo), page_hi)] : 0;
     };
-    int next = fetch(0);
+    int next = fetch(0), stage = 0, lap = 0;
     bool ok = true;
     for (int j = 0; j < n_tiles && ok; ++j) {
-      const int b = j & 1;
       int mine = next;
       const int page_idx = first_page + j * ppt + lane;
       if (lane >= ppt || page_idx < page_lo || page_idx > page_hi) {
@@ -179,39 +198,38 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       int pages[4];
 #pragma unroll
       for (int pi = 0; pi < 4; ++pi) pages[pi] = __shfl_sync(0xffffffffu, mine, pi);
-      for (int which = 0; which < 2 && ok; ++which) {    // keys first: they are needed first
-        uint64_t* full = which ? &sh->v_full[b] : &sh->k_full[b];
-        if (j >= 2) ok = tc::mbar_wait(which ? &sh->v_empty[b] : &sh->k_empty[b], ((j >> 1) - 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (tc::elect_one()) {
-          tc::mbar_expect_tx(full, (uint32_t)nsub * AT_KV_SUB);
-          const CUtensorMap* map = which ? &map_v : &map_k;
-          uint8_t* ring = (which ? sv : sk) + (size_t)b * nsub * AT_KV_SUB;
-          if (p.whole && which) {                        // values: a box per page, [slice][row of the page][64 columns]
+      if (lap > 0) ok = warp_wait(&empty[stage], (lap - 1) & 1, abort_flag);
+      if (!ok) break;
+      if (tc::elect_one()) {
+        tc::mbar_expect_tx(&full[stage], (uint32_t)nsub * AT_KV_SUB);
+        uint8_t* to = ring + (size_t)stage * nsub * AT_KV_SUB;
+        if (p.whole && values) {                         // values: a box per page, [slice][row of the page][64 columns]
 #pragma unroll
-            for (int pi = 0; pi < 4; ++pi)
-              if (pi < ppt)
-                tc::tma_load_3d(ring + (size_t)pi * nsub * p.page_size * 128, map, full, 0, (pages[pi] * p.nkv + kvh) * p.page_size, 0);
-          } else if (p.whole) {                          // keys: a box per 8 rows, [slice][8 rows][64 columns]
+          for (int pi = 0; pi < 4; ++pi)
+            if (pi < ppt)
+              tc::tma_load_3d(to + (size_t)pi * nsub * p.page_size * 128, map, &full[stage], 0, (pages[pi] * p.nkv + kvh) * p.page_size, 0);
+        } else if (p.whole) {                            // keys: a box per 8 rows, [slice][8 rows][64 columns]
 #pragma unroll
-            for (int a = 0; a < AT_N / 8; ++a) {
-              const int key = a * 8;
-              const int pg = p.page_size == 16 ? pages[a >> 1] : p.page_size == 32 ? pages[a >> 2] : pages[0];
-              tc::tma_load_3d(ring + (size_t)a * nsub * 1024, map, full, 0, (pg * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1)), 0);
-            }
-          } else {
+          for (int a = 0; a < AT_N / 8; ++a) {
+            const int key = a * 8;
+            const int pg = p.page_size == 16 ? pages[a >> 1] : p.page_size == 32 ? pages[a >> 2] : pages[0];
+            tc::tma_load_3d(to + (size_t)a * nsub * 1024, map, &full[stage], 0, (pg * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1)), 0);
+          }
+        } else {
 #pragma unroll
-            for (int pi = 0; pi < 4; ++pi) {
-              if (pi < ppt) {
-                const int row = (pages[pi] * p.nkv + kvh) * p.page_size;
-                uint8_t* dst = ring + (size_t)pi * p.page_size * 128;
-                for (int sub = 0; sub < nsub; ++sub) tc::tma_load_2d(dst + (size_t)sub * AT_KV_SUB, map, full, sub * 64, row);
-              }
+          for (int pi = 0; pi < 4; ++pi) {
+            if (pi < ppt) {
+              const int row = (pages[pi] * p.nkv + kvh) * p.page_size;
+              uint8_t* dst = to + (size_t)pi * p.page_size * 128;
+              for (int sub = 0; sub < nsub; ++sub) tc::tma_load_2d(dst + (size_t)sub * AT_KV_SUB, map, &full[stage], sub * 64, row);
             }
           }
         }
-        __syncwarp();
+      }
+      __syncwarp();
+      if (++stage == stages) {
+        stage = 0;
+        ++lap;
       }
     }
   } else if (warp == 1) {
@@ -224,14 +242,14 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const uint64_t kd0 = tc::smem_desc_k_sw128_sbo(tc::smem_u32(sk), k_sbo);
       const uint32_t k_tile = ((uint32_t)nsub * AT_KV_SUB) >> 4;
       bool ok = tc::mbar_wait(&sh->q_full, 0, abort_flag);
-      for (int j = 0; j < n_tiles && ok; ++j) {
+      for (int j = 0, stage = 0, phase = 0; j < n_tiles && ok; ++j) {
         const int b = j & 1;
-        if (j >= 2) ok = tc::mbar_wait(&sh->s_free[b], ((j >> 1) - 1) & 1, abort_flag);
-        if (ok) ok = tc::mbar_wait(&sh->k_full[b], (j >> 1) & 1, abort_flag);
+        ok = tc::mbar_wait(&sh->k_full[stage], phase, abort_flag);
+        if (ok && j >= 2) ok = tc::mbar_wait(&sh->s_free[b], ((j >> 1) - 1) & 1, abort_flag);
         if (!ok) break;
         tc::fence_after_thread_sync();
         const uint32_t d = tmem_s + b * AT_N;
-        const uint64_t kd = kd0 + b * k_tile;
+        const uint64_t kd = kd0 + stage * k_tile;
 #pragma unroll
         for (int ks = 0; ks < 16; ++ks) {
           if (ks < hd16) {
@@ -241,7 +259,11 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
         tc::mma_commit(&sh->s_full[b]);
-        tc::mma_commit(&sh->k_empty[b]);
+        tc::mma_commit(&sh->k_empty[stage]);
+        if (++stage == p.k_stages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
     }
     __syncwarp();
@@ -259,17 +281,21 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         v_step[kk] = p.whole ? (((kk * 16) / p.page_size) * v_page + ((kk * 16) % p.page_size) * 128u) >> 4
                              : (uint32_t)(kk * 2048) >> 4;
       bool ok = true;
-      for (int j = 0; j < n_tiles && ok; ++j) {
+      for (int j = 0, stage = 0, phase = 0; j < n_tiles && ok; ++j) {
         const int b = j & 1;
-        ok = tc::mbar_wait(&sh->v_full[b], (j >> 1) & 1, abort_flag);
+        ok = tc::mbar_wait(&sh->v_full[stage], phase, abort_flag);
         if (ok) ok = tc::mbar_wait(&sh->p_ready[b], (j >> 1) & 1, abort_flag);
         if (!ok) break;
         tc::fence_after_thread_sync();
 #pragma unroll
         for (int kk = 0; kk < AT_N / 16; ++kk)
-          tc::mma_bf16_ts(tmem_o, tmem_p + b * (AT_N / 2) + 8 * kk, vd0 + b * v_tile + v_step[kk], idesc, (j > 0 || kk > 0) ? 1u : 0u);
-        tc::mma_commit(&sh->v_empty[b]);
+          tc::mma_bf16_ts(tmem_o, tmem_p + b * (AT_N / 2) + 8 * kk, vd0 + stage * v_tile + v_step[kk], idesc, (j > 0 || kk > 0) ? 1u : 0u);
+        tc::mma_commit(&sh->v_empty[stage]);
         tc::mma_commit(&sh->pv_done[b]);
+        if (++stage == p.v_stages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
       tc::mma_commit(&sh->o_full);
     }
@@ -288,9 +314,9 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const float out_scale = p.cap > 0.f ? p.cap * LOG2E : LOG2E;   // scores are kept in log2 units
     const float fixed_ref = 0.5f * out_scale;
     float ref = -INFINITY, l = 0.f;
-    bool ok = true;
+    bool ok = true;                                      // the same in all lanes of a warp
     for (int j = group; j < n_tiles; j += 2) {
-      ok = tc::mbar_wait(&sh->s_full[group], (j >> 1) & 1, abort_flag);
+      ok = warp_wait(&sh->s_full[group], (j >> 1) & 1, abort_flag);
       if (!ok) break;
       tc::fence_after_thread_sync();
       uint32_t raw[AT_N];
@@ -322,7 +348,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
         for (int c = 0; c < AT_N; ++c) top = fmaxf(top, __uint_as_float(raw[c]));
         // the row's reference comes from the tile before, goes to the tile behind
-        if (j > 0) ok = tc::mbar_wait(&sh->turn[group], ((j + group) / 2 - 1) & 1, abort_flag);
+        if (j > 0) ok = warp_wait(&sh->turn[group], ((j + group) / 2 - 1) & 1, abort_flag);
         if (!ok) break;
         const float before = j > 0 ? sh->row_ref[r] : -INFINITY;
         const bool grow = top > before + AT_GROW || (before == -INFINITY && top > -INFINITY);
@@ -334,7 +360,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           ref = now;
         }
         if (j > 0 && __any_sync(0xffffffffu, grow)) {    // O follows when the product of the tile before is in
-          ok = tc::mbar_wait(&sh->pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag);
+          ok = warp_wait(&sh->pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag);
           if (!ok) break;
           tc::fence_after_thread_sync();
           const float corr = grow ? (before == -INFINITY ? 0.f : tc::exp2_approx(before - now)) : 1.f;
@@ -361,7 +387,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         raw[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
       }
       l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-      if (j >= 2) ok = tc::mbar_wait(&sh->pv_done[group], ((j >> 1) - 1) & 1, abort_flag);     // P of two tiles ago was read
+      if (j >= 2) ok = warp_wait(&sh->pv_done[group], ((j >> 1) - 1) & 1, abort_flag);     // P of two tiles ago was read
       if (!ok) break;
       tc::fence_after_thread_sync();
       tc::tmem_st_16(my_p, raw);
@@ -374,7 +400,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     sh->row_sum[group][r] = l;
     sh->row_own[group][r] = ref;
     asm volatile("bar.sync 2, 256;" ::: "memory");
-    if (ok) ok = tc::mbar_wait(&sh->o_full, 0, abort_flag);
+    if (ok) ok = warp_wait(&sh->o_full, 0, abort_flag);
     if (ok) {
       tc::fence_after_thread_sync();
       float total = sh->row_sum[0][r] + sh->row_sum[1][r], last = 0.f;
@@ -558,7 +584,14 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   p.out = (__nv_bfloat16*)out; p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.num_pages = num_pages;
   p.multiplier = multiplier; p.cap = cap; p.window = window; p.whole = whole; p.status = status; p.n_seqs = n_seqs;
   const int nsub = (hd + 63) / 64;
-  const int smem = nsub * AT_Q_SUB + 4 * nsub * AT_KV_SUB + (int)sizeof(PortionShared) + 1024;
+  // As many tiles ahead as fit: a tile's copies take 1.5 us from L2, four tiles' work at head size 128
+  auto bytes = [&](int k, int v) { return nsub * AT_Q_SUB + (k + v) * nsub * AT_KV_SUB + (int)sizeof(PortionShared); };
+  p.k_stages = p.v_stages = AT_STAGES;
+  while (bytes(p.k_stages, p.v_stages) > 227 * 1024) {
+    if (p.v_stages >= p.k_stages) --p.v_stages;
+    else --p.k_stages;
+  }
+  const int smem = bytes(p.k_stages, p.v_stages);
   // at most a tile more than whole ones for every portion
   const long long blocks = ((long long)T / tok_per_tile + n_seqs) * nkv;
   if (blocks > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
