@@ -43,13 +43,27 @@ struct AppendParams {
   int T, nh, nkv, hd, rot, interleaved, page_size, num_pages, max_pages;
 };
 
-// (cos, sin) of 2 pi pos turns, times the amplitude.  The product is taken in 64 bits and reduced to half a turn either
-// way before anything is rounded to 32: at position 100,000 the 32-bit product alone is off by 4e-3 radians.
+// (cos, sin) of 2 pi pos turns, times the amplitude.  The product is taken in 64 bits and reduced to an eighth of a turn
+// either way before anything is rounded to 32: at position 100,000 the 32-bit product alone is off by 4e-3 radians.  Then
+// the Taylor polynomials of sine and cosine to x^9 and x^10, |x| <= pi / 4: what they leave out is below 2e-9.
 __device__ __forceinline__ float2 rope_angle(int pos, double turns, float amplitude) {
-  const double t = (double)pos * turns;
-  float s, c;
-  sincospif((float)(2.0 * (t - rint(t))), &s, &c);
-  return make_float2(c * amplitude, s * amplitude);
+  const double quarters = 4.0 * turns * (double)pos;
+  const double magic = 6755399441055744.0;                 // 1.5 * 2^52: the nearest whole number sits in the low bits
+  const double shifted = quarters + magic;
+  const int n = __double2loint(shifted);
+  const float x = (float)(quarters - (shifted - magic)) * 1.57079632679f;
+  const float y = x * x;
+  float s = fmaf(y, 2.7557319e-6f, -1.9841270e-4f);        // 1/9!, 1/7!, 1/5!, 1/3!
+  s = fmaf(s, y, 8.3333333e-3f);
+  s = fmaf(s, y, -1.6666667e-1f);
+  s = fmaf(s * y, x, x);
+  float c = fmaf(y, -2.7557319e-7f, 2.4801587e-5f);        // 1/10!, 1/8!, 1/6!, 1/4!, 1/2!
+  c = fmaf(c, y, -1.3888889e-3f);
+  c = fmaf(c, y, 4.1666667e-2f);
+  c = fmaf(c, y, -0.5f);
+  c = fmaf(c, y, 1.f);
+  const float cs = (n & 1) ? s : c, sn = (n & 1) ? c : s;
+  return make_float2((((n + 1) & 2) ? -cs : cs) * amplitude, ((n & 2) ? -sn : sn) * amplitude);
 }
 
 // ---- heads of up to 256: a lane holds NP pairs of a head ------------------------------------------------------------
@@ -58,11 +72,11 @@ __device__ __forceinline__ float2 rope_angle(int pos, double turns, float amplit
 // One launch of two kinds of blocks of eight warps.  Cache blocks: a window of 16 tokens x one kv head x keys or values.  A
 // block owns the runs (tokens of one request in one page) that begin in its window and takes them whole, so that the
 // largest magnitude of a run, and with it the page's new scale, is found in one block whatever the windows cut: a warp
-// per token, values kept in registers (four tokens a warp) between the maximum and the codes.  Query blocks: a warp
+// per token, values kept in registers (two tokens a warp) between the maximum and the codes.  Query blocks: a warp
 // rotates four heads of a token with one set of sines and cosines.
 constexpr int AP_WARPS = 8;
 constexpr int AP_WINDOW = 16;                     // tokens
-constexpr int AP_HELD = 4;                        // tokens of a warp whose values stay in registers
+constexpr int AP_HELD = 2;                        // tokens of a warp whose values stay in registers
 constexpr int AP_MOST_PAGE = AP_WARPS * 32 - AP_WINDOW;       // rows of a page: a thread per token of a block
 constexpr int AP_HEADS = 4;                       // query heads of a unit
 
@@ -72,8 +86,9 @@ __device__ __forceinline__ int2 rope_pair(int i, int rot, int interleaved) {
   return interleaved || i >= half ? make_int2(2 * i, 2 * i + 1) : make_int2(i, i + half);
 }
 
-template <typename S, int NP>
-__global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const AppendParams p, int cache_blocks) {
+// FULL: heads of 64 NP dims, all of them turned.
+template <typename S, int NP, bool FULL>
+__global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const AppendParams p, int cache_blocks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int width = (p.nh + 2 * p.nkv) * p.hd, half = p.rot >> 1, pairs = p.hd >> 1;
   pdl_wait_release();
@@ -83,7 +98,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const Append
   for (int k = 0; k < NP; ++k) {
     const int i = lane + 32 * k;
     at[k] = rope_pair(i, p.rot, p.interleaved);
-    turns[k] = i < half ? p.turns[i] : 0.0;
+    turns[k] = FULL || i < half ? p.turns[i] : 0.0;
   }
 
   if ((int)blockIdx.x >= cache_blocks) {
@@ -99,15 +114,15 @@ __global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const Append
     for (int h = 0; h < AP_HEADS; ++h)
 #pragma unroll
       for (int k = 0; k < NP; ++k)
-        if (h0 + h < p.nh && lane + 32 * k < pairs) {
+        if (h0 + h < p.nh && (FULL || lane + 32 * k < pairs)) {
           a[h][k] = src[h * p.hd + at[k].x];
           b[h][k] = src[h * p.hd + at[k].y];
         }
     const int pos = p.positions[t];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      if (lane + 32 * k >= pairs) continue;
-      const bool turned = lane + 32 * k < half;
+      if (!FULL && lane + 32 * k >= pairs) continue;
+      const bool turned = FULL || lane + 32 * k < half;
       const float2 cs = turned ? rope_angle(pos, turns[k], p.amplitude) : make_float2(1.f, 0.f);
 #pragma unroll
       for (int h = 0; h < AP_HEADS; ++h)
@@ -121,25 +136,32 @@ __global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const Append
   }
 
   // ---- keys and values -----------------------------------------------------------------------------------------------
-  __shared__ unsigned starts[AP_WARPS], bad[AP_WARPS];    // per token behind the window's first: does a run begin, in order
-  __shared__ int seqs[AP_WARPS * 32], poss[AP_WARPS * 32];
-  __shared__ unsigned tops[AP_WARPS * 32];                // largest magnitude of a token, as bits
+  // Of the window's tokens and those behind it that may belong to its runs: what a thread finds out for all.
+  __shared__ unsigned starts[AP_WARPS], bad[AP_WARPS];    // does a run begin there; does it break the order
+  __shared__ int poss[AP_WARPS * 32], offs[AP_WARPS * 32];
+  __shared__ int runs[AP_WARPS * 32];                     // the run's first token
+  __shared__ int pages[AP_WARPS * 32];                    // of a run, at its first token: page (-1: none), ...
+  __shared__ unsigned olds[AP_WARPS * 32];                // ... bits of the scale it had (0 when the run begins the page), ...
+  __shared__ unsigned tops[AP_WARPS * 32];                // ... bits of its largest magnitude
   const int kv = blockIdx.x % (2 * p.nkv), is_v = kv & 1, h = kv >> 1;
   const int t0 = (int)(blockIdx.x / (2 * p.nkv)) * AP_WINDOW;
   const int reach = min(AP_WINDOW + p.page_size, p.T - t0);
+  const int me = threadIdx.x;
+  int seq = 0, pos = 0, place = 0;
   {
-    const int i = threadIdx.x, t = t0 + i;
     bool start = true, wrong = false;                     // what lies behind the reach ends every run
-    if (i < reach) {
-      const int seq = p.token_seq[t], pos = p.positions[t];
-      seqs[i] = seq;
-      poss[i] = pos;
-      if (t > 0) {
-        const int before = p.token_seq[t - 1], pos_before = p.positions[t - 1];
+    if (me < reach) {
+      seq = p.token_seq[t0 + me];
+      pos = p.positions[t0 + me];
+      place = pos / p.page_size;
+      poss[me] = pos;
+      offs[me] = pos - place * p.page_size;
+      if (t0 + me > 0) {
+        const int before = p.token_seq[t0 + me - 1], pos_before = p.positions[t0 + me - 1];
         wrong = before > seq || (before == seq && pos_before + 1 != pos);
-        start = wrong || before != seq || pos_before / p.page_size != pos / p.page_size;
+        start = wrong || before != seq || offs[me] == 0;
       }
-      if (wrong && i < AP_WINDOW) atomicExch(p.status, 5);
+      if (wrong && me < AP_WINDOW) atomicExch(p.status, 5);
     }
     const unsigned s = __ballot_sync(0xffffffffu, start), w = __ballot_sync(0xffffffffu, wrong);
     if (lane == 0) {
@@ -150,127 +172,100 @@ __global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const Append
   __syncthreads();
   // the block's tokens: from the first run that begins in the window to the end of the last one that does
   const unsigned in_window = starts[0] & 0xffffu;
-  if (!in_window || (__ffs(in_window) - 1) >= reach) return;
   const int first = __ffs(in_window) - 1;
+  if (first < 0 || first >= reach) return;
   int last = reach;
-  {
-    const unsigned behind = starts[0] >> AP_WINDOW;
-    if (behind) {
-      last = AP_WINDOW + __ffs(behind) - 1;
-    } else {
-      for (int w = 1; w < AP_WARPS; ++w)
-        if (starts[w]) {
-          last = w * 32 + __ffs(starts[w]) - 1;
-          break;
-        }
-    }
-    last = min(last, reach);
+  if (starts[0] >> AP_WINDOW) {
+    last = min(reach, AP_WINDOW + __ffs(starts[0] >> AP_WINDOW) - 1);
+  } else {
+    for (int w = 1; w < AP_WARPS; ++w)
+      if (starts[w]) {
+        last = min(reach, w * 32 + __ffs(starts[w]) - 1);
+        break;
+      }
   }
   const float* src = p.qkv + (size_t)t0 * width + (size_t)(p.nh + (is_v ? p.nkv : 0) + h) * p.hd;
-  // values of token i, rotated
   auto load = [&](int i, float (&a)[NP], float (&b)[NP]) {
     const float* row = src + (size_t)i * width;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const bool in = lane + 32 * k < pairs;
+      const bool in = FULL || lane + 32 * k < pairs;
       a[k] = in ? row[at[k].x] : 0.f;
       b[k] = in ? row[at[k].y] : 0.f;
     }
   };
-  auto turn = [&](int i, float (&a)[NP], float (&b)[NP]) {
-    if (is_v) return;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      if (lane + 32 * k >= half) continue;
-      const float2 cs = rope_angle(poss[i], turns[k], p.amplitude);
-      const float x = a[k], y = b[k];
-      a[k] = x * cs.x - y * cs.y;
-      b[k] = x * cs.y + y * cs.x;
-    }
-  };
-  auto top_of = [&](const float (&a)[NP], const float (&b)[NP]) -> unsigned {
-    unsigned m = 0;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) m = max(m, max(__float_as_uint(a[k]) & 0x7fffffffu, __float_as_uint(b[k]) & 0x7fffffffu));
-    return __reduce_max_sync(0xffffffffu, m);
-  };
-  const bool coded = p.k_scale != nullptr;
   float a[AP_HELD][NP], b[AP_HELD][NP];
 #pragma unroll
   for (int c = 0; c < AP_HELD; ++c)
     if (first + warp + c * AP_WARPS < last) load(first + warp + c * AP_WARPS, a[c], b[c]);
-  unsigned old[AP_HELD];                                  // scales before this step, read before any is written
+  const bool coded = p.k_scale != nullptr;
   float* scale = is_v ? p.v_scale : p.k_scale;
-  // of token i: its run's first token, and the run's page (-1: none, or out of order)
-  auto run_of = [&](int i, int& page) -> int {
-    int w = i >> 5;
-    unsigned m = starts[w] & (0xffffffffu >> (31 - (i & 31)));
+  if (me >= first && me < last) {
+    int w = me >> 5;
+    unsigned m = starts[w] & (0xffffffffu >> (31 - (me & 31)));
     while (!m) m = starts[--w];                           // `first` begins a run
     const int s = w * 32 + 31 - __clz(m);
-    const int pos = poss[s], place = pos / p.page_size;
-    page = -1;
-    if (!((bad[w] >> (s & 31)) & 1u)) {
-      if (pos >= 0 && place < p.max_pages) page = p.block_table[(size_t)seqs[s] * p.max_pages + place];
-      if (page < 0 || page >= p.num_pages) {
-        if (lane == 0) atomicExch(p.status, 2);
-        page = -1;
+    runs[me] = s;
+    if (s == me) {
+      int page = -1;
+      if (!((bad[me >> 5] >> (me & 31)) & 1u)) {
+        if (pos >= 0 && place < p.max_pages) page = p.block_table[(size_t)seq * p.max_pages + place];
+        if (page < 0 || page >= p.num_pages) {
+          atomicExch(p.status, 2);
+          page = -1;
+        }
       }
+      pages[me] = page;
+      olds[me] = coded && page >= 0 && offs[me] ? __float_as_uint(scale[(size_t)page * p.nkv + h]) & 0x7fffffffu : 0u;
+      tops[me] = 0u;
     }
-    return s;
+  }
+  __syncthreads();
+  // rotates token i's values and brings their largest magnitude to its run
+  auto prepare = [&](int i, float (&x)[NP], float (&y)[NP]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      if (!is_v && (FULL || lane + 32 * k < half)) {
+        const float2 cs = rope_angle(poss[i], turns[k], p.amplitude);
+        const float u = x[k], v = y[k];
+        x[k] = u * cs.x - v * cs.y;
+        y[k] = u * cs.y + v * cs.x;
+      }
+      m = max(m, max(__float_as_uint(x[k]) & 0x7fffffffu, __float_as_uint(y[k]) & 0x7fffffffu));
+    }
+    return m;
   };
-  int pages[AP_HELD], begins[AP_HELD];
-#pragma unroll
-  for (int c = 0; c < AP_HELD; ++c) {
-    const int i = first + warp + c * AP_WARPS;
-    old[c] = 0;
-    pages[c] = -1;
-    if (i >= last) continue;
-    begins[c] = run_of(i, pages[c]);
-    if (coded && pages[c] >= 0 && poss[begins[c]] % p.page_size)
-      old[c] = __float_as_uint(scale[(size_t)pages[c] * p.nkv + h]) & 0x7fffffffu;
-  }
 #pragma unroll
   for (int c = 0; c < AP_HELD; ++c) {
     const int i = first + warp + c * AP_WARPS;
     if (i >= last) continue;
-    turn(i, a[c], b[c]);
-    const unsigned m = top_of(a[c], b[c]);
-    if (lane == 0) tops[i] = m;
+    const unsigned m = __reduce_max_sync(0xffffffffu, prepare(i, a[c], b[c]));
+    if (lane == 0) atomicMax(&tops[runs[i]], m);
   }
-  for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {    // pages of more than 16 rows
+  for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {    // a run cut by the window, pages of many rows
     float x[NP], y[NP];
     load(i, x, y);
-    turn(i, x, y);
-    const unsigned m = top_of(x, y);
-    if (lane == 0) tops[i] = m;
+    const unsigned m = __reduce_max_sync(0xffffffffu, prepare(i, x, y));
+    if (lane == 0) atomicMax(&tops[runs[i]], m);
   }
-  auto store = [&](int i, const float (&x)[NP], const float (&y)[NP], int s, int page, unsigned before) {
+  __syncthreads();
+  auto store = [&](int i, const float (&x)[NP], const float (&y)[NP]) {
+    const int s = runs[i], page = pages[s];
+    if (page < 0) return;
     const size_t row = ((size_t)page * p.nkv + h) * p.page_size;
-    const int off = poss[i] % p.page_size;
     if (!coded) {
-      S* dst = (S*)(is_v ? p.v_pool : p.k_pool) + (row + off) * p.hd;
+      S* dst = (S*)(is_v ? p.v_pool : p.k_pool) + (row + offs[i]) * p.hd;
 #pragma unroll
       for (int k = 0; k < NP; ++k)
-        if (lane + 32 * k < pairs) {
+        if (FULL || lane + 32 * k < pairs) {
           dst[at[k].x] = from_float<S>(x[k]);
           dst[at[k].y] = from_float<S>(y[k]);
         }
       return;
     }
-    // the run's largest magnitude: its tokens are s .. e - 1
-    const int off0 = poss[s] % p.page_size;
-    unsigned m = 0;
-    for (int j = s + lane; j < min(last, s + p.page_size - off0); j += 32) {
-      bool same = true;                                   // no run begins between s and j
-      for (int w = s >> 5; w <= j >> 5 && same; ++w) {
-        unsigned bits = starts[w];
-        if (w == s >> 5) bits &= ~(0xffffffffu >> (31 - (s & 31)));
-        if (w == j >> 5) bits &= 0xffffffffu >> (31 - (j & 31));
-        same = bits == 0;
-      }
-      if (same) m = max(m, tops[j]);
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
+    const unsigned m = tops[s], before = olds[s];
+    const int off0 = offs[s];
     const bool finite = m < C8_NOT_FINITE && before < C8_NOT_FINITE;
     const int e_old = (int)(before >> 23) - 127;
     const int e = off0 > 0 ? max(c8_exponent(m), e_old) : c8_exponent(m);
@@ -288,14 +283,14 @@ __global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const Append
         }
       }
     }
-    dst += (size_t)off * p.hd;
+    dst += (size_t)offs[i] * p.hd;
     const float inv = c8_pow2(-e);
 #pragma unroll
     for (int k = 0; k < NP; ++k)
-      if (lane + 32 * k < pairs) {
+      if (FULL || lane + 32 * k < pairs) {
         const unsigned char cx = finite ? (unsigned char)c8_code(x[k], inv) : (unsigned char)128;
         const unsigned char cy = finite ? (unsigned char)c8_code(y[k], inv) : (unsigned char)128;
-        if (at[k].y == at[k].x + 1 && !(at[k].x & 1)) {
+        if (p.interleaved) {
           *reinterpret_cast<uchar2*>(dst + at[k].x) = make_uchar2(cx, cy);
         } else {
           dst[at[k].x] = cx;
@@ -303,27 +298,14 @@ __global__ void __launch_bounds__(AP_WARPS * 32) rope_append_kernel(const Append
         }
       }
   };
-  // Tokens that are not held need their run's scale from before this step as well: read now, kept in shared memory
-  __shared__ unsigned late[AP_WARPS * 32];
-  for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {
-    int page;
-    const int s = run_of(i, page);
-    if (lane == 0) late[i] = coded && page >= 0 && poss[s] % p.page_size ? __float_as_uint(scale[(size_t)page * p.nkv + h]) & 0x7fffffffu : 0u;
-  }
-  __syncthreads();
 #pragma unroll
-  for (int c = 0; c < AP_HELD; ++c) {
-    const int i = first + warp + c * AP_WARPS;
-    if (i < last && pages[c] >= 0) store(i, a[c], b[c], begins[c], pages[c], old[c]);
-  }
+  for (int c = 0; c < AP_HELD; ++c)
+    if (first + warp + c * AP_WARPS < last) store(first + warp + c * AP_WARPS, a[c], b[c]);
   for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {
-    int page;
-    const int s = run_of(i, page);
-    if (page < 0) continue;
     float x[NP], y[NP];
     load(i, x, y);
-    turn(i, x, y);
-    store(i, x, y, s, page, late[i]);
+    prepare(i, x, y);
+    store(i, x, y);
   }
 }
 
@@ -549,9 +531,14 @@ GLINT_API int glint_rope_append(const float* qkv, const int* positions, const in
     if (blocks > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
     const dim3 grid((unsigned)blocks), block(AP_WARPS * 32);
     const int cb = (int)cache_blocks;
-    if (hd <= 64) { C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, 1>, grid, block, 0, stream, p, cb)) }
-    else if (hd <= 128) { C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, 2>, grid, block, 0, stream, p, cb)) }
-    else { C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, 4>, grid, block, 0, stream, p, cb)) }
+#define APPEND(NP, FULL) C8_DISPATCH(dtype, e = launch_kernel(rope_append_kernel<S, NP, FULL>, grid, block, 0, stream, p, cb))
+    if (hd == 64 && rot == hd) { APPEND(1, true) }
+    else if (hd == 128 && rot == hd) { APPEND(2, true) }
+    else if (hd == 256 && rot == hd) { APPEND(4, true) }
+    else if (hd <= 64) { APPEND(1, false) }
+    else if (hd <= 128) { APPEND(2, false) }
+    else { APPEND(4, false) }
+#undef APPEND
   } else {
     const dim3 grid(T, k_pool ? 1 + 2 * nkv : 1);
     C8_DISPATCH(dtype, e = launch_kernel(rope_append_simple_kernel<S>, grid, dim3(128), 0, stream, p))
