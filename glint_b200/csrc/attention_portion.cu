@@ -92,8 +92,11 @@ __device__ __forceinline__ bool portion_tile(const int* cu, int n_seqs, int tok_
   return false;
 }
 
-template <bool FIXED>
-__global__ void __launch_bounds__(AT_THREADS, 1)
+// FIXED: the soft cap spares the running maximum.  PAIR: two blocks on an SM (head sizes up to 128): each has half of the
+// tensor memory, so that P is written over the scores it came from and the scores two tiles on wait for the product that
+// reads it; one block's beginning and end pass under the other's tiles.
+template <bool FIXED, bool PAIR>
+__global__ void __launch_bounds__(AT_THREADS, PAIR ? 2 : 1)
 attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const PortionParams p) {
   extern __shared__ __align__(1024) uint8_t at_raw[];    // begins at a multiple of 1024: there is no room for less (checked)
@@ -101,7 +104,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int hd = p.hd, hd16 = hd >> 4, nsub = (hd + 63) >> 6;
   const int G = p.nh / p.nkv;
   const int tok_per_tile = AT_M / G;
-  constexpr int TMEM_COLS = 512;
+  constexpr int TMEM_COLS = PAIR ? 256 : 512;
   uint8_t* sq = smem;
   uint8_t* sk = sq + (size_t)nsub * AT_Q_SUB;            // [stages][nsub][64 keys x 128 B]
   uint8_t* sv = sk + (size_t)p.k_stages * nsub * AT_KV_SUB;
@@ -155,8 +158,9 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   __syncthreads();
   tc::fence_after_thread_sync();
   const uint32_t tmem_s = sh->tmem_base;                 // two score buffers of 64 columns
-  const uint32_t tmem_p = tmem_s + 2 * AT_N;             // two of P as bfloat16 pairs, 32 columns each
-  const uint32_t tmem_o = tmem_p + AT_N;                 // up to 256 columns
+  // two of P as bfloat16 pairs, 32 columns each; O, up to 256 columns (PAIR: 128)
+  const uint32_t tmem_p = PAIR ? tmem_s : tmem_s + 2 * AT_N, p_step = PAIR ? AT_N : AT_N / 2;
+  const uint32_t tmem_o = tmem_s + (PAIR ? 2 * AT_N : 3 * AT_N);
   volatile int* abort_flag = &sh->abort_flag;
 
   if (warp == 0 || warp == 3) {
@@ -245,7 +249,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       for (int j = 0, stage = 0, phase = 0; j < n_tiles && ok; ++j) {
         const int b = j & 1;
         ok = tc::mbar_wait(&sh->k_full[stage], phase, abort_flag);
-        if (ok && j >= 2) ok = tc::mbar_wait(&sh->s_free[b], ((j >> 1) - 1) & 1, abort_flag);
+        if (ok && j >= 2) ok = tc::mbar_wait(PAIR ? &sh->pv_done[b] : &sh->s_free[b], ((j >> 1) - 1) & 1, abort_flag);
         if (!ok) break;
         tc::fence_after_thread_sync();
         const uint32_t d = tmem_s + b * AT_N;
@@ -289,7 +293,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         tc::fence_after_thread_sync();
 #pragma unroll
         for (int kk = 0; kk < AT_N / 16; ++kk)
-          tc::mma_bf16_ts(tmem_o, tmem_p + b * (AT_N / 2) + 8 * kk, vd0 + stage * v_tile + v_step[kk], idesc, (j > 0 || kk > 0) ? 1u : 0u);
+          tc::mma_bf16_ts(tmem_o, tmem_p + b * p_step + 8 * kk, vd0 + stage * v_tile + v_step[kk], idesc, (j > 0 || kk > 0) ? 1u : 0u);
         tc::mma_commit(&sh->v_empty[stage]);
         tc::mma_commit(&sh->pv_done[b]);
         if (++stage == p.v_stages) {
@@ -308,45 +312,55 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const int qpos = pos0 + (rv ? r / G : 0);
     const int lo = p.window > 0 ? qpos - p.window + 1 : 0;
     const uint32_t lane_base = ((uint32_t)(quarter * 32) << 16);
-    const uint32_t my_s = tmem_s + group * AT_N + lane_base, my_p = tmem_p + group * (AT_N / 2) + lane_base;
+    const uint32_t my_s = tmem_s + group * AT_N + lane_base, my_p = tmem_p + group * p_step + lane_base;
     const float LOG2E = 1.4426950408889634f;
     const float in_scale = p.cap > 0.f ? p.multiplier / p.cap : p.multiplier;
     const float out_scale = p.cap > 0.f ? p.cap * LOG2E : LOG2E;   // scores are kept in log2 units
     const float fixed_ref = 0.5f * out_scale;
     float ref = -INFINITY, l = 0.f;
     bool ok = true;                                      // the same in all lanes of a warp
+    constexpr int CH = PAIR ? 32 : AT_N;                 // columns in registers at a time
     for (int j = group; j < n_tiles; j += 2) {
       ok = warp_wait(&sh->s_full[group], (j >> 1) & 1, abort_flag);
       if (!ok) break;
       tc::fence_after_thread_sync();
-      uint32_t raw[AT_N];
-#pragma unroll
-      for (int c0 = 0; c0 < AT_N; c0 += 16) tc::tmem_ld_16(my_s + c0, raw + c0);
-      tc::tmem_ld_wait();
-      tc::fence_before_thread_sync();
-      tc::mbar_arrive(&sh->s_free[group]);
       const int key0 = kv_begin + j * AT_N;
-      // scores in log2 units; FIXED: less the fixed reference
-      if (FIXED || p.cap > 0.f) {
-#pragma unroll
-        for (int c = 0; c < AT_N; ++c) {
-          const float v = tc::tanh_approx(__uint_as_float(raw[c]) * in_scale);
-          raw[c] = __float_as_uint(FIXED ? fmaf(v, out_scale, -fixed_ref) : v * out_scale);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < AT_N; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) * (in_scale * out_scale));
-      }
       // most tiles lie wholly inside every row's range
-      if (!__all_sync(0xffffffffu, rv && key0 >= lo && key0 + AT_N - 1 <= qpos)) {
+      const bool inside = __all_sync(0xffffffffu, rv && key0 >= lo && key0 + AT_N - 1 <= qpos);
+      uint32_t raw[CH];
+      // scores of columns c0 .. c0 + CH - 1 in log2 units, masked; FIXED: less the fixed reference
+      auto scores = [&](int c0) {
 #pragma unroll
-        for (int c = 0; c < AT_N; ++c)
-          if (!(rv && key0 + c <= qpos && key0 + c >= lo)) raw[c] = 0xff800000u;      // -inf
-      }
+        for (int c = 0; c < CH; c += 16) tc::tmem_ld_16(my_s + c0 + c, raw + c);
+        tc::tmem_ld_wait();
+        if (!PAIR) {
+          tc::fence_before_thread_sync();
+          tc::mbar_arrive(&sh->s_free[group]);
+        }
+        if (FIXED || p.cap > 0.f) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const float v = tc::tanh_approx(__uint_as_float(raw[c]) * in_scale);
+            raw[c] = __float_as_uint(FIXED ? fmaf(v, out_scale, -fixed_ref) : v * out_scale);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < CH; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) * (in_scale * out_scale));
+        }
+        if (!inside) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            if (!(rv && key0 + c0 + c <= qpos && key0 + c0 + c >= lo)) raw[c] = 0xff800000u;      // -inf
+        }
+      };
       if (!FIXED) {
         float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < AT_N; ++c) top = fmaxf(top, __uint_as_float(raw[c]));
+        for (int c0 = 0; c0 < AT_N; c0 += CH) {
+          scores(c0);
+#pragma unroll
+          for (int c = 0; c < CH; ++c) top = fmaxf(top, __uint_as_float(raw[c]));
+        }
         // the row's reference comes from the tile before, goes to the tile behind
         if (j > 0) ok = warp_wait(&sh->turn[group], ((j + group) / 2 - 1) & 1, abort_flag);
         if (!ok) break;
@@ -378,20 +392,27 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const float base = FIXED || ref == -INFINITY ? 0.f : ref;
       float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < AT_N; c += 2) {
-        const float p0 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c]) : __uint_as_float(raw[c]) - base);
-        const float p1 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c + 1]) : __uint_as_float(raw[c + 1]) - base);
-        l4[c & 3] += p0;
-        l4[(c + 1) & 3] += p1;
-        const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-        raw[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int c0 = 0; c0 < AT_N; c0 += CH) {
+        if (FIXED || PAIR) scores(c0);                   // else they are in registers still
+#pragma unroll
+        for (int c = 0; c < CH; c += 2) {
+          const float p0 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c]) : __uint_as_float(raw[c]) - base);
+          const float p1 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c + 1]) : __uint_as_float(raw[c + 1]) - base);
+          l4[c & 3] += p0;
+          l4[(c + 1) & 3] += p1;
+          const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+          raw[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (!PAIR && j >= 2) {                           // P of two tiles ago was read
+          ok = warp_wait(&sh->pv_done[group], ((j >> 1) - 1) & 1, abort_flag);
+          if (!ok) break;
+          tc::fence_after_thread_sync();
+        }
+#pragma unroll
+        for (int c = 0; c < CH / 2; c += 16) tc::tmem_st_16(my_p + c0 / 2 + c, raw + c);
       }
-      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-      if (j >= 2) ok = warp_wait(&sh->pv_done[group], ((j >> 1) - 1) & 1, abort_flag);     // P of two tiles ago was read
       if (!ok) break;
-      tc::fence_after_thread_sync();
-      tc::tmem_st_16(my_p, raw);
-      tc::tmem_st_16(my_p + 16, raw + 16);
+      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
       tc::tmem_st_wait();
       tc::fence_before_thread_sync();
       tc::mbar_arrive(&sh->p_ready[group]);
@@ -586,8 +607,9 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   const int nsub = (hd + 63) / 64;
   // As many tiles ahead as fit: a tile's copies take 1.5 us from L2, four tiles' work at head size 128
   auto bytes = [&](int k, int v) { return nsub * AT_Q_SUB + (k + v) * nsub * AT_KV_SUB + (int)sizeof(PortionShared); };
+  const bool pair = hd <= 128;                           // two blocks on an SM
   p.k_stages = p.v_stages = AT_STAGES;
-  while (bytes(p.k_stages, p.v_stages) > 227 * 1024) {
+  while (bytes(p.k_stages, p.v_stages) > (pair ? 113 * 1024 : 227 * 1024)) {
     if (p.v_stages >= p.k_stages) --p.v_stages;
     else --p.k_stages;
   }
@@ -598,7 +620,7 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   // Fewer blocks than SMs: their keys are split, as far as that makes work for all SMs and leaves a split four tiles.
   const long long reach = window > 0 && (long long)window + max_q_len < max_context ? (long long)window + max_q_len + AT_N : max_context;
   const int most_tiles = (int)((reach + AT_N - 1) / AT_N);
-  int splits = (int)(sms / blocks);
+  int splits = (int)(sms * (pair ? 2 : 1) / blocks);
   if (splits > most_tiles / 4) splits = most_tiles / 4;
   const long long part = (long long)T * nh * (hd + 2);
   if (splits > 1 && (!scratch || ((uintptr_t)scratch & 15) || part * splits > scratch_floats))
@@ -615,13 +637,17 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   const dim3 grid((unsigned)blocks, splits);
   const bool fixed = cap > 0.f && cap <= AT_FIXED_CAP;
   cudaError_t e = cudaSuccess;
-#define LAUNCH(FIXED)                                                                                             \
-  {                                                                                                               \
-    e = cudaFuncSetAttribute(attention_portion_kernel<FIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
-    if (e == cudaSuccess)                                                                                         \
-      e = launch_kernel(attention_portion_kernel<FIXED>, grid, dim3(AT_THREADS), (size_t)smem, stream, map_q, map_k, map_v, p); \
+#define LAUNCH(FIXED, PAIR)                                                                                             \
+  {                                                                                                                     \
+    e = cudaFuncSetAttribute(attention_portion_kernel<FIXED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
+    if (e == cudaSuccess)                                                                                               \
+      e = launch_kernel(attention_portion_kernel<FIXED, PAIR>, grid, dim3(AT_THREADS), (size_t)smem, stream, map_q, map_k, map_v, p); \
   }
-  if (fixed) LAUNCH(true) else LAUNCH(false)
+  if (pair) {
+    if (fixed) LAUNCH(true, true) else LAUNCH(false, true)
+  } else {
+    if (fixed) LAUNCH(true, false) else LAUNCH(false, false)
+  }
 #undef LAUNCH
   if (e == cudaSuccess && splits > 1)
     e = launch_kernel(attention_portion_merge_kernel, dim3((unsigned)(((long long)T * nh + 7) / 8)), dim3(256), 0, stream, p);
