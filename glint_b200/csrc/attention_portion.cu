@@ -62,18 +62,32 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
 }
 
-// The (request, query tile) of a block, counted from the last: late tiles have the most keys and start first.  False: none.
-__device__ __forceinline__ bool portion_tile(const int* cu, int n_seqs, int tok_per_tile, int index, int& seq, int& tile) {
+// The query tile of a block, counted from the last: late tiles have the most keys and start first.
+struct PortionTile {
+  int seq, tile, begin, len, start;      // request, tile of its portion, first token, tokens, position of the first
+};
+// False: there are fewer.  A warp looks at 32 requests at a time; up to 32 cost one trip to memory.
+__device__ __forceinline__ bool portion_tile(const PortionParams& p, int tok_per_tile, int index, PortionTile& found) {
   const int lane = threadIdx.x & 31;
-  int total = 0;
-  for (int b = 0; b < n_seqs; b += 32) {
-    int n = b + lane < n_seqs ? (cu[b + lane + 1] - cu[b + lane] + tok_per_tile - 1) / tok_per_tile : 0;
-    total += __reduce_add_sync(0xffffffffu, max(n, 0));
+  int total = 0, lo = 0, hi = 0, start = 0;
+  auto look = [&](int b) -> int {        // tiles of request b + lane
+    lo = hi = start = 0;
+    if (b + lane < p.n_seqs) {
+      lo = p.cu_seqlens[b + lane];
+      hi = p.cu_seqlens[b + lane + 1];
+      start = p.seq_start[b + lane];
+    }
+    return max(0, (hi - lo + tok_per_tile - 1) / tok_per_tile);
+  };
+  int n = 0;
+  for (int b = 0; b < p.n_seqs; b += 32) {
+    n = look(b);
+    total += __reduce_add_sync(0xffffffffu, n);
   }
   int at = total - 1 - index;
   if (at < 0) return false;
-  for (int b = 0; b < n_seqs; b += 32) {
-    const int n = b + lane < n_seqs ? max(0, (cu[b + lane + 1] - cu[b + lane] + tok_per_tile - 1) / tok_per_tile) : 0;
+  for (int b = 0; b < p.n_seqs; b += 32) {
+    if (p.n_seqs > 32) n = look(b);
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -83,8 +97,11 @@ __device__ __forceinline__ bool portion_tile(const int* cu, int n_seqs, int tok_
     const unsigned hit = __ballot_sync(0xffffffffu, at < incl);
     if (hit) {
       const int who = __ffs(hit) - 1;
-      seq = b + who;
-      tile = at - __shfl_sync(0xffffffffu, incl - n, who);
+      found.seq = b + who;
+      found.tile = at - __shfl_sync(0xffffffffu, incl - n, who);
+      found.begin = __shfl_sync(0xffffffffu, lo, who);
+      found.len = __shfl_sync(0xffffffffu, hi, who) - found.begin;
+      found.start = __shfl_sync(0xffffffffu, start, who);
       return true;
     }
     at -= __shfl_sync(0xffffffffu, incl, 31);
@@ -111,53 +128,55 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   PortionShared* sh = reinterpret_cast<PortionShared*>(sv + (size_t)p.v_stages * nsub * AT_KV_SUB);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    tc::mbar_init(&sh->q_full, 1);
-    tc::mbar_init(&sh->o_full, 1);
-    for (int b = 0; b < 2; ++b) {
-      tc::mbar_init(&sh->s_full[b], 1);
-      tc::mbar_init(&sh->s_free[b], AT_M);
-      tc::mbar_init(&sh->p_ready[b], AT_M);
-      tc::mbar_init(&sh->pv_done[b], 1);
-      tc::mbar_init(&sh->turn[b], AT_M);
+  {
+    // a barrier per thread; arrivals of a group's rows where threads arrive, of one thread or copy elsewhere
+    uint64_t* const single[] = {&sh->q_full, &sh->o_full, sh->s_full, sh->pv_done, sh->k_full, sh->k_empty, sh->v_full, sh->v_empty};
+    const int many[] = {1, 1, 2, 2, AT_STAGES, AT_STAGES, AT_STAGES, AT_STAGES};
+    uint64_t* const rows[] = {sh->s_free, sh->p_ready, sh->turn};
+    int i = threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i >= 0 && i < many[k]) tc::mbar_init(single[k] + i, 1);
+      i -= many[k];
     }
-    for (int b = 0; b < AT_STAGES; ++b) {
-      tc::mbar_init(&sh->k_full[b], 1);
-      tc::mbar_init(&sh->k_empty[b], 1);
-      tc::mbar_init(&sh->v_full[b], 1);
-      tc::mbar_init(&sh->v_empty[b], 1);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (i >= 0 && i < 2) tc::mbar_init(rows[k] + i, AT_M);
+      i -= 2;
     }
-    sh->abort_flag = 0;
-    tc::fence_barrier_init();
-    tc::tma_prefetch_desc(&map_q);
-    tc::tma_prefetch_desc(&map_k);
-    tc::tma_prefetch_desc(&map_v);
+    if (i == 0) sh->abort_flag = 0;
+    if (threadIdx.x < 32) tc::fence_barrier_init();
+    if (threadIdx.x == 64) tc::tma_prefetch_desc(&map_q);
+    if (threadIdx.x == 65) tc::tma_prefetch_desc(&map_k);
+    if (threadIdx.x == 66) tc::tma_prefetch_desc(&map_v);
   }
+  __syncthreads();
   pdl_wait_release();
   if (tc::smem_u32(at_raw) & 1023) {                     // the operands' swizzle wants it
     if (threadIdx.x == 0) atomicExch(p.status, 4);
     return;
   }
   // blockIdx.x counts (query tile from the last, kv head), blockIdx.y the splits
-  int seq = 0, tile = 0;
   const int kvh = (int)blockIdx.x % p.nkv, split = blockIdx.y;
-  if (!portion_tile(p.cu_seqlens, p.n_seqs, tok_per_tile, (int)blockIdx.x / p.nkv, seq, tile)) return;
-  const int t_begin = p.cu_seqlens[seq];
-  const int q_len = p.cu_seqlens[seq + 1] - t_begin;
+  PortionTile work;
+  if (!portion_tile(p, tok_per_tile, (int)blockIdx.x / p.nkv, work)) return;
+  const int seq = work.seq, tile = work.tile, t_begin = work.begin, q_len = work.len;
   const int tok0 = tile * tok_per_tile;
   const int n_tok = min(tok_per_tile, q_len - tok0);
   const int n_rows = n_tok * G;
-  const int pos0 = p.seq_start[seq] + tok0;
+  const int pos0 = work.start + tok0;
   const int pos_last = pos0 + n_tok - 1;
   const int kv_first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
   const int kv_begin = (kv_first & ~(AT_N - 1)) + split * p.per_split * AT_N;     // this split's first tile
   const int n_tiles = min(p.per_split, (pos_last - kv_begin + AT_N) / AT_N);
   if (kv_begin > pos_last) return;                       // the rows' keys end before this split (the same for all threads)
-  if (warp == 1) tc::tmem_alloc(&sh->tmem_base, TMEM_COLS);
-  tc::fence_before_thread_sync();
-  __syncthreads();
-  tc::fence_after_thread_sync();
-  const uint32_t tmem_s = sh->tmem_base;                 // two score buffers of 64 columns
+  if (warp != 0 && warp != 3) {                          // the producers begin at once
+    if (warp == 1) tc::tmem_alloc(&sh->tmem_base, TMEM_COLS);
+    tc::fence_before_thread_sync();
+    asm volatile("bar.sync 3, %0;" ::"n"(AT_THREADS - 64) : "memory");
+    tc::fence_after_thread_sync();
+  }
+  const uint32_t tmem_s = warp != 0 && warp != 3 ? sh->tmem_base : 0u;      // two score buffers of 64 columns
   // two of P as bfloat16 pairs, 32 columns each; O, up to 256 columns (PAIR: 128)
   const uint32_t tmem_p = PAIR ? tmem_s : tmem_s + 2 * AT_N, p_step = PAIR ? AT_N : AT_N / 2;
   const uint32_t tmem_o = tmem_s + (PAIR ? 2 * AT_N : 3 * AT_N);
@@ -434,29 +453,62 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           else total += sh->row_sum[b][r];               // 0, or NaN where every score was
       }
       const int o_lo = group ? ((hd16 + 1) >> 1) * 16 : 0, o_hi = group ? hd : ((hd16 + 1) >> 1) * 16;
-      const size_t row = (size_t)(t_begin + tok0 + (rv ? r / G : 0)) * p.nh + kvh * G + (rv ? r % G : 0);
       const float inv = p.part_o ? 1.f : total == 0.f ? 0.f : 1.0f / total;
-      if (p.part_o && rv && group == 0) p.part_ml[(size_t)split * p.T * p.nh + row] = make_float2(last, total);
-      for (int c0 = o_lo; c0 < o_hi; c0 += 16) {
-        uint32_t o[16];
+      if (p.part_o && rv && group == 0) {
+        const size_t row = (size_t)(t_begin + tok0 + r / G) * p.nh + kvh * G + r % G;
+        p.part_ml[(size_t)split * p.T * p.nh + row] = make_float2(last, total);
+      }
+      // Rows go out by way of shared memory, which all copies and products have left: a thread has a row of O, but a
+      // warp should write rows as a whole (a thread writing its own row's 32 bytes at a time took 5 us).  16-byte chunk c of
+      // row r sits at c ^ (r mod 8), as far as the chunks of a row are a multiple of a power of two.
+      const int chunk_shift = p.part_o ? 2 : 3;          // elements of a chunk: 4 floats, 8 bfloat16
+      const int chunks = hd >> chunk_shift, swizzle = r & 7 & ((chunks & -chunks) - 1);
+      uint4* row_at = reinterpret_cast<uint4*>(smem) + (size_t)r * chunks;
+      for (int c0 = o_lo; c0 < o_hi; c0 += 32) {
+        uint32_t o[32];
         tc::tmem_ld_16(tmem_o + lane_base + c0, o);
+        if (c0 + 16 < o_hi) tc::tmem_ld_16(tmem_o + lane_base + c0 + 16, o + 16);
         tc::tmem_ld_wait();
-        if (!rv) continue;
-        if (p.part_o) {
-          float4* to = reinterpret_cast<float4*>(p.part_o + ((size_t)split * p.T * p.nh + row) * hd + c0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            to[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-        } else {
-          uint32_t h[8];
+        for (int half = 0; half < 2; ++half) {
+          if (c0 + 16 * half >= o_hi) break;
+          const uint32_t* v = o + 16 * half;
+          const int c = (c0 + 16 * half) >> chunk_shift;
+          if (p.part_o) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-            h[i] = *reinterpret_cast<const uint32_t*>(&v);
+            for (int i = 0; i < 4; ++i) row_at[(c + i) ^ swizzle] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+              h[i] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+            row_at[c ^ swizzle] = make_uint4(h[0], h[1], h[2], h[3]);
+            row_at[(c + 1) ^ swizzle] = make_uint4(h[4], h[5], h[6], h[7]);
           }
-          uint4* to = reinterpret_cast<uint4*>(p.out + row * hd + c0);
-          to[0] = make_uint4(h[0], h[1], h[2], h[3]);
-          to[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+      }
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    if (ok) {
+      // 8, 16 or 32 lanes to a row; a warp's rows are 8 x (rows at once) apart, their (token, head) counted without division
+      const int chunks = hd >> (p.part_o ? 2 : 3);
+      const int lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32, at_once = 32 / lanes, step = 8 * at_once;
+      const int step_tok = step / G, step_head = step - step_tok * G, wrap = (chunks & -chunks) - 1;
+      uint4* to = p.part_o ? reinterpret_cast<uint4*>(p.part_o + (size_t)split * p.T * p.nh * hd) : reinterpret_cast<uint4*>(p.out);
+      int row = (warp - 4) * at_once + lane / lanes;
+      int tok = row / G, head = row - tok * G;
+      const int c0 = lane & (lanes - 1);
+      for (; row < n_rows; row += step) {
+        const uint4* from = reinterpret_cast<const uint4*>(smem) + (size_t)row * chunks;
+        uint4* dst = to + ((size_t)(t_begin + tok0 + tok) * p.nh + kvh * G + head) * chunks;
+        for (int c = c0; c < chunks; c += lanes) dst[c] = from[c ^ (row & 7 & wrap)];
+        tok += step_tok;
+        head += step_head;
+        if (head >= G) {
+          head -= G;
+          ++tok;
         }
       }
     }
