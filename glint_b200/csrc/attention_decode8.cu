@@ -64,6 +64,7 @@ struct Decode8Entry {
 struct Decode8Shared {
   uint64_t full[D8_MAX_STAGES];
   Decode8Entry entry[2][D8_CHUNK];
+  int walk[6];                  // where the last lookup ended
   int abort_flag;
   int last_one;
 };
@@ -329,10 +330,9 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   int voff = inside - pair * (p.pair_cost + sg.pages);
 
   // ---- the block's pages are looked up 128 at a time, one by a thread, into one of two halves of `entry`: chunk c + 1
-  // when the block comes to chunk c.  The walk over the pairs goes on where the last lookup ended. ----------------------
-  int wt = t, wpos = pos, wrow = row, wpair = pair, woff = voff, wleft = remaining;
-  auto look_up = [&](int half) -> int {                        // place of this thread's page in the scales, -1: none
-    int at = -1, first_row = -1;
+  // when the block is in the middle of chunk c.  The walk over the pairs goes on where the last lookup ended. ------------
+  auto look_up = [&](int half, int wt, int wpos, int wrow, int wpair, int woff, int wleft) -> int {
+    int at = -1, first_row = -1;                               // place of this thread's page in the scales, -1: none
     const int i = threadIdx.x;
     for (int i0 = 0; i0 < D8_CHUNK && wleft > 0 && wt < p.T;) {           // the same walk in all threads, pair by pair
       const Decode8Segment ws = d8_segment(wpos, p.window, p.page_size);
@@ -364,12 +364,11 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       }
     }
     if (i < D8_CHUNK) sh->entry[half][i].row = first_row;
+    if (i == 0) {
+      sh->walk[0] = wt; sh->walk[1] = wpos; sh->walk[2] = wrow;
+      sh->walk[3] = wpair; sh->walk[4] = woff; sh->walk[5] = wleft;
+    }
     return at;
-  };
-  auto scales = [&](int half, int at) {
-    if (at < 0) return;
-    sh->entry[half][threadIdx.x].ks = p.k_scale[at];
-    sh->entry[half][threadIdx.x].vs = p.v_scale[at];
   };
   // Copies page i of the block into stage s: called by the warp whose page it is, which has read what was there before.
   auto fetch = [&](int i, int s) {
@@ -388,12 +387,18 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       }
     }
   };
-  // The first pages are on their way before anything else is waited for.
-  const int at0 = look_up(0);
-  __syncthreads();
-  for (int s = warp; s < p.stages; s += D8_WARPS) fetch(s, s);            // a stage is always the same warp's
-  scales(0, at0);
-  scales(1, look_up(1));
+  // The first pages' scales are requested before their copies: behind the burst of all blocks' first copies they would
+  // arrive 5 us later.
+  {
+    const int at = look_up(0, t, pos, row, pair, voff, remaining);
+    const float ks = at >= 0 ? p.k_scale[at] : 0.f, vs = at >= 0 ? p.v_scale[at] : 1.f;
+    __syncthreads();
+    for (int s = warp; s < p.stages; s += D8_WARPS) fetch(s, s);          // a stage is always the same warp's
+    if (at >= 0) {
+      sh->entry[0][threadIdx.x].ks = ks;
+      sh->entry[0][threadIdx.x].vs = vs;
+    }
+  }
   bool looked_up = false;                                      // by all threads: a barrier away
 
   const int g = lane >> 2, tq = lane & 3;
@@ -422,15 +427,18 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       {
         const __nv_bfloat16* qrow = p.q + ((size_t)t * p.nh + kvh * G + h0 + (g < H ? g : 0)) * hd;
         uint2 raw[HD / 32][2];
-        unsigned top = 0;
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             raw[s][j] = make_uint2(0, 0);
-            if (s * 32 + j * 16 < hd && g < H) raw[s][j] = *reinterpret_cast<const uint2*>(qrow + s * 32 + j * 16 + tq * 4);
-            top = __vmaxu2(top, __vmaxu2(raw[s][j].x & 0x7fff7fffu, raw[s][j].y & 0x7fff7fffu));
+            if ((FULL || s * 32 + j * 16 < hd) && g < H) raw[s][j] = *reinterpret_cast<const uint2*>(qrow + s * 32 + j * 16 + tq * 4);
           }
+        unsigned top = 0;
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top = __vmaxu2(top, __vmaxu2(raw[s][j].x & 0x7fff7fffu, raw[s][j].y & 0x7fff7fffu));
         top = max(top & 0xffffu, top >> 16);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -485,13 +493,20 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       // Page `it` of the block belongs to warp it % warps and stage it % stages (a multiple of them: a stage is always
       // filled and read by the same warp, which therefore sees every phase of the stage's barrier).
       for (int done = it0; done < it0 + n;) {
-        if (done > 0 && (done & (D8_CHUNK - 1)) == 0) {        // all warps have left the chunk before
+        if ((done & (D8_CHUNK - 1)) == D8_CHUNK / 2) {         // all warps have left the chunk before
           __syncthreads();
           const int half = (done / D8_CHUNK + 1) & 1;
-          scales(half, look_up(half));
+          const int* w = sh->walk;
+          const int w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = w[4], w5 = w[5];
+          __syncthreads();                                     // all have read where to go on
+          const int at = look_up(half, w0, w1, w2, w3, w4, w5);
+          if (at >= 0) {
+            sh->entry[half][threadIdx.x].ks = p.k_scale[at];
+            sh->entry[half][threadIdx.x].vs = p.v_scale[at];
+          }
           __syncthreads();
         }
-        done = min(it0 + n, (done & ~(D8_CHUNK - 1)) + D8_CHUNK);
+        done = min(it0 + n, ((done + D8_CHUNK / 2) & ~(D8_CHUNK - 1)) + D8_CHUNK / 2);
         for (; it < done; it += D8_WARPS) {
           const Decode8Entry& en = sh->entry[(it / D8_CHUNK) & 1][it & (D8_CHUNK - 1)];
           float ks = en.ks, vs = en.vs;
