@@ -80,7 +80,16 @@ bool tiled_attention_supported(int nh, int nkv, int hd, int page) {
   return nkv > 0 && nh % nkv == 0 && nh / nkv <= 128 && hd % 16 == 0 && hd >= 16 && hd <= 256 &&
          (page == 16 || page == 32 || page == 64);
 }
-constexpr long long FEW_TOKEN_BYTES = 32ll << 20;   // codes read in all, up to which any tokens take the single-token kernel
+// Tokens of portions over coded pages that take the single-token kernel all the same.  It reads the codes again for every
+// token, a (token, kv head) pair costs it about 96 KB beside them, but it needs no wide pages and spreads over all SMs: bytes
+// that count as much as 32 MB and seven readings of the longest context.  Measured on both sides of that (us, this kernel
+// against wide pages and the tiled one), 8 heads in 4 groups of 256: 8 tokens at 2,000 keys 15.4 / 17.9, 32 at 2,000 26 / 19,
+// 8 at 8,000 25.7 / 31, 16 at 8,000 40 / 32; 32 heads in 16 groups of 128: 8 at 500 12.8 / 16.1, 32 at 500 22.7 / 18.8.
+// Below 256 keys the tiled kernel's one or two tiles are as fast (64 tokens at 100 keys 17 / 12).
+bool few_tokens(long long tokens, int reach, int nkv, int hd) {
+  const long long context = (long long)reach * nkv * hd * 2;
+  return reach > 256 && tokens * (context + nkv * (96ll << 10)) <= (32ll << 20) + 7 * context;
+}
 constexpr int SPLIT_SINGLES_FROM = 4096;   // context from which single tokens in front of portions leave the tiled kernel
 constexpr int SPLIT_SINGLES_UP_TO = 8;     // so few of them leave it at any context
 
@@ -311,11 +320,9 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
   const bool single = rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_decode8 && view->partials && view->arrive &&
                       t.attention_decode8_supported(nh, nkv, hd, page) &&
                       t.attention_decode8_workspace(blocks, nh, nkv, hd) <= view->partial_floats;
-  // Few tokens over little cache take the single-token kernel whatever the portions: it reads the codes once for every
-  // token, but in one launch of many warps
   const int reach = window > 0 && window < step->max_context ? window : step->max_context;
-  const bool few = (long long)step->num_tokens * reach * nkv * hd * 2 <= FEW_TOKEN_BYTES;
-  const int lead = !single ? 0 : step->max_seq_len == 1 || few ? step->num_tokens : step->leading_single;
+  const bool each_alone = step->max_seq_len == 1 || few_tokens(step->num_tokens, reach, nkv, hd);
+  const int lead = !single ? 0 : each_alone ? step->num_tokens : step->leading_single;
   if (lead > 0) {
     const int rc = counted(t.attention_decode8(
         q, (const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale, step->positions, step->token_seq,
