@@ -19,7 +19,8 @@
 // blocks, whose partial results a second kernel adds up in order.
 // Blocks are found from the portions' lengths, so that short portions beside long ones cost no empty blocks.
 // Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx; keys of a token at position p from
-// max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit.
+// max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the second product, and their sum
+// is that of the rounded ones.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -417,10 +418,11 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int c = 0; c < CH; c += 2) {
           const float p0 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c]) : __uint_as_float(raw[c]) - base);
           const float p1 = tc::exp2_approx(FIXED ? __uint_as_float(raw[c + 1]) : __uint_as_float(raw[c + 1]) - base);
-          l4[c & 3] += p0;
-          l4[(c + 1) & 3] += p1;
           const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-          raw[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+          const uint32_t both = *reinterpret_cast<const uint32_t*>(&h);
+          l4[c & 3] += __uint_as_float(both << 16);      // the sum of what the product will see
+          l4[(c + 1) & 3] += __uint_as_float(both & 0xffff0000u);
+          raw[c >> 1] = both;
         }
         if (!PAIR && j >= 2) {                           // P of two tiles ago was read
           ok = warp_wait(&sh->pv_done[group], ((j >> 1) - 1) & 1, abort_flag);
