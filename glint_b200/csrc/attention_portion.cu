@@ -502,16 +502,32 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       int row = (warp - 4) * at_once + lane / lanes;
       int tok = row / G, head = row - tok * G;
       const int c0 = lane & (lanes - 1);
-      for (; row < n_rows; row += step) {
-        const uint4* from = reinterpret_cast<const uint4*>(smem) + (size_t)row * chunks;
-        uint4* dst = to + ((size_t)(t_begin + tok0 + tok) * p.nh + kvh * G + head) * chunks;
-        for (int c = c0; c < chunks; c += lanes) dst[c] = from[c ^ (row & 7 & wrap)];
-        tok += step_tok;
-        head += step_head;
-        if (head >= G) {
-          head -= G;
-          ++tok;
+      constexpr int AHEAD = 4;                           // rows on their way through registers
+      auto advance = [&](int& t, int& h) {
+        t += step_tok;
+        h += step_head;
+        if (h >= G) {
+          h -= G;
+          ++t;
         }
+      };
+      for (; row < n_rows; row += AHEAD * step) {
+        for (int c = c0; c < chunks; c += lanes) {
+          uint4 v[AHEAD];
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const int r_ = row + k * step;
+            if (r_ < n_rows) v[k] = reinterpret_cast<const uint4*>(smem)[(size_t)r_ * chunks + (c ^ (r_ & 7 & wrap))];
+          }
+          int t_ = tok, h_ = head;
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            if (row + k * step < n_rows) to[((size_t)(t_begin + tok0 + t_) * p.nh + kvh * G + h_) * chunks + c] = v[k];
+            advance(t_, h_);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) advance(tok, head);
       }
     }
   }
