@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from ..errors import GlintError, RequestError
+from ..runtime import parse_cache_dtype
 from ..sampling import DeviceSampler, SamplingParams
 from .loading import build_engine, load_model, random_model
 from .scheduler import Request, Scheduler
@@ -46,6 +47,8 @@ class LLM:
     def __init__(self, model_path=None, dtype="bfloat16", device="cuda:0", cache_tokens=None, max_active=64,
                  max_step_tokens=2048, page_size=16, kernels="auto", model=None, lookahead=True, cache_dtype=None):
         try:
+            if model is not None and cache_dtype is not None and parse_cache_dtype(cache_dtype) != model.rt.cache_dtype:
+                raise RequestError(f"the model given keeps its cache as {model.rt.cache_dtype or 'auto'}, not {cache_dtype}")
             self.model = model if model is not None else load_model(model_path, dtype, device, kernels, cache_dtype)
         except GlintError as e:
             raise ValueError(str(e)) from e

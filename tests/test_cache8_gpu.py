@@ -394,6 +394,53 @@ def test_attention_over_pages_of_very_different_scales(rts):
                 assert err <= 0.012 * np.abs(want).max(), (big_page, gap, head, err)
 
 
+def test_more_single_tokens_than_a_launch_takes(rts):
+    """1,100 single tokens (a launch takes 1,024): every one as if it were alone, up to the order of its sums, which depends on
+    the launch (a few ulp of 32 bits before the result's rounding: at most the two nearest bfloat16 values apart)."""
+    from glint_b200 import ops_cache8
+    rt, n, nh, nkv, hd = rts["bfloat16"], 1100, 2, 1, 16
+    starts = [(7 * i) % 50 for i in range(n)]
+    s = Setup(rt, [1] * n, starts, nkv, hd, 16, seed=4)
+    q = (0.1 * torch.randn(n, nh * hd, generator=torch.Generator().manual_seed(2))).to(DEV, torch.bfloat16)
+    out = ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.25)
+    t = s.step.tensors
+    for i in (0, 500, 1023, 1024, 1099):
+        one = ops_cache8.StepArrays(t["positions"][i:i + 1].contiguous(), torch.zeros(1, dtype=torch.int32, device=DEV),
+                                    t["seq_start"][i:i + 1].contiguous(), torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+                                    t["block_table"][i:i + 1].contiguous(), 1, starts[i] + 1, contexts=[starts[i] + 1])
+        alone = ops_cache8.attention(rt, s.cache, one, q[i:i + 1].contiguous(), nh, 0.25)
+        far = (alone[0].float() - out[i].float()).abs()
+        assert (far <= 2.0 ** -7 * alone[0].float().abs()).all()
+    rt.check_status()
+
+
+def test_pages_beyond_32_bit_offsets(rts):
+    """A pool of 4.9e9 codes: requests in its last pages give, bit for bit, what they give in a small pool."""
+    from glint_b200 import ops_cache8
+    rt, nh, nkv, hd, P, pages = rts["bfloat16"], 4, 2, 256, 16, 600_000
+    turns = _turns(hd // 2).to(DEV)
+    outs = []
+    for base, total in ((0, 16), (pages - 16, pages)):
+        cache = ops_cache8.Cache8.empty(total, nkv, P, hd)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+        table = i32([[base + p for p in range(16)]])
+        qkv = _qkv(201, nh, nkv, hd, 5, 0.3).to(DEV)
+        got = []
+        for a, b in ((0, 200), (200, 201)):
+            step = ops_cache8.StepArrays(i32(list(range(a, b))), i32([0] * (b - a)), i32([a]), i32([0, b - a]), table, b - a, b,
+                                         contexts=[b] if b - a == 1 else [])
+            q = ops_cache8.append(rt, cache, step, qkv[a:b].contiguous(), turns, nh)
+            got += [q, ops_cache8.attention(rt, cache, step, q, nh, 0.0625, softcap=50.0)]
+        k, v = ops_cache8.unpack(rt, cache, step)
+        outs.append([t.clone() for t in got] + [cache.k[base:base + 13].clone(), cache.v[base:base + 13].clone(),
+                                               cache.k_scale[base:base + 13].clone(), k[base:base + 12].clone(), v[base:base + 12].clone()])
+        del cache, k, v
+        torch.cuda.empty_cache()
+    rt.check_status()
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
 def test_a_step_as_it_is_made(rts):
     """Append, then attention of the appended tokens, for a portion, single tokens behind it and the mixture: against the
     definition over what the pages hold (read back), and on a stream of its own."""
@@ -617,6 +664,8 @@ def test_entry_point_and_commands(folder, capsys):
     check_generate(llm, prompts, new_tokens=12)
     with pytest.raises(ValueError, match="cache dtype"):
         LLM(folder, cache_dtype="int4")
+    with pytest.raises(ValueError, match="keeps its cache"):
+        LLM(model=llm.model, cache_dtype="auto", cache_tokens=256)
     assert main(["generate", "-f", folder, "-t", "5,17,3", "-m", "4", "--cache-dtype", "int8"]) == 0
     assert "Generated token ids: [5, 17, 3" in capsys.readouterr().out
 
