@@ -520,6 +520,7 @@ GLINT_API int glint_rope_append(const float* qkv, const int* positions, const in
   if (T <= 0) return GLINT_OK;
   if (hd <= 0 || hd % 2 || rot % 2 || rot < 0 || rot > hd || nh <= 0 || nkv <= 0 || page_size <= 0) return GLINT_ERR_BAD_ARG;
   if (!k_pool != !v_pool || !k_scale != !v_scale || (k_scale && !k_pool)) return GLINT_ERR_BAD_ARG;
+  if (k_scale && (((uintptr_t)k_pool | (uintptr_t)v_pool) & 1)) return GLINT_ERR_BAD_ARG;      // codes are moved in pairs
   if (nkv > 32767) return GLINT_ERR_UNSUPPORTED_SIZE;
   AppendParams p = {qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_pool, k_scale, v_scale, status, amplitude,
                     T, nh, nkv, hd, rot, interleaved ? 1 : 0, page_size, num_pages, max_pages};

@@ -70,6 +70,8 @@ class Cache8:
             raise KernelError(f"a coded cache takes even head sizes, not {self.hd}")
         if any(t.device != self.k.device for t in (self.v, self.k_scale, self.v_scale, self.k_wide, self.v_wide)):
             raise KernelError("the tensors of a coded cache belong to one device")
+        if any(t.data_ptr() % 16 for t in (self.k, self.v, self.k_wide, self.v_wide)):
+            raise KernelError("the pools of a coded cache begin at multiples of 16 bytes")
         self.scratch = partials, arrive = native.cache8_scratch(self.nkv, self.hd, self.k.device)
         self.struct = native.ViewStruct(self.k.data_ptr(), self.v.data_ptr(), self.page_size, self.num_pages, 0, 1,
                                         self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.k_wide.data_ptr(),

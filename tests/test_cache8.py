@@ -115,6 +115,11 @@ def test_cache_refusals(monkeypatch):
             ops_cache8.Cache8(*t)
     with pytest.raises(KernelError, match="even"):
         ops_cache8.Cache8(*_tensors(hd=33))
+    for k in (0, 1, 4, 5):                        # kernels move these 2 to 16 bytes at a time
+        t = _tensors()
+        t[k] = torch.zeros(t[k].numel() + 1, dtype=t[k].dtype)[1:].view(t[k].shape)
+        with pytest.raises(KernelError, match="16 bytes"):
+            ops_cache8.Cache8(*t)
 
 
 def test_step_refusals(monkeypatch):
