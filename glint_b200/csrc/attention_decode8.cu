@@ -132,13 +132,17 @@ __device__ __forceinline__ float d8_inverse(float power_of_two) { return __int_a
 struct Decode8Segment {
   int first, page_lo, pages;    // of a token: first key, first page, pages
 };
-__device__ __forceinline__ Decode8Segment d8_segment(int pos, int window, int page_size) {
+// `last`: the last page that the block table has room for.  A position outside it is held to it here (units stay
+// positive and bounded) and reported once, by d8_outside.
+__device__ __forceinline__ Decode8Segment d8_segment(int pos, int window, int page_size, int last) {
   Decode8Segment s;
+  pos = max(pos, 0);
   s.first = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
-  s.page_lo = s.first / page_size;
-  s.pages = pos / page_size - s.page_lo + 1;
+  s.page_lo = min(s.first / page_size, last);
+  s.pages = min(pos / page_size, last) - s.page_lo + 1;
   return s;
 }
+__device__ __forceinline__ bool d8_outside(int pos, int page_size, int last) { return pos < 0 || pos / page_size > last; }
 
 // What a warp has of a pair so far.
 template <int HD>
@@ -295,7 +299,12 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int r0 = min(lane * per, p.T), r1 = min(r0 + per, p.T);
   int mine = 0, row_first = 0;
   if (r0 < r1) row_first = p.token_seq[r0];
-  for (int r = r0; r < r1; ++r) mine += (p.pair_cost + d8_segment(p.positions[r], p.window, p.page_size).pages) * pairs;
+  const int last_page = p.max_pages * p.splits - 1;
+  for (int r = r0; r < r1; ++r) {
+    const int at = p.positions[r];
+    if (d8_outside(at, p.page_size, last_page)) atomicExch(p.status, 3);
+    mine += (p.pair_cost + d8_segment(at, p.window, p.page_size, last_page).pages) * pairs;
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -313,7 +322,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     row = row_first;
     for (;; ++t) {
       pos = p.positions[t];
-      const int u = (p.pair_cost + d8_segment(pos, p.window, p.page_size).pages) * pairs;
+      const int u = (p.pair_cost + d8_segment(pos, p.window, p.page_size, last_page).pages) * pairs;
       if (inside < u) break;
       inside -= u;
     }
@@ -325,7 +334,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   row = __shfl_sync(0xffffffffu, row, who);
   inside = __shfl_sync(0xffffffffu, inside, who);
   int remaining = min(W, total - (int)begin);                  // units
-  Decode8Segment sg = d8_segment(pos, p.window, p.page_size);
+  Decode8Segment sg = d8_segment(pos, p.window, p.page_size, last_page);
   int pair = inside / (p.pair_cost + sg.pages);
   int voff = inside - pair * (p.pair_cost + sg.pages);
 
@@ -335,7 +344,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     int at = -1, first_row = -1;                               // place of this thread's page in the scales, -1: none
     const int i = threadIdx.x;
     for (int i0 = 0; i0 < D8_CHUNK && wleft > 0 && wt < p.T;) {           // the same walk in all threads, pair by pair
-      const Decode8Segment ws = d8_segment(wpos, p.window, p.page_size);
+      const Decode8Segment ws = d8_segment(wpos, p.window, p.page_size, last_page);
       const int skipped = max(woff, p.pair_cost) - woff;       // empty units
       const int off = woff + skipped - p.pair_cost;            // first page of this pair here
       const int n = max(0, min(D8_CHUNK - i0, min(wleft - skipped, ws.pages - off)));
@@ -646,7 +655,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       pair = 0;
       if (++t < p.T && remaining > 0) {
         pos = p.positions[t];
-        sg = d8_segment(pos, p.window, p.page_size);
+        sg = d8_segment(pos, p.window, p.page_size, last_page);
       }
     }
   }
@@ -719,7 +728,7 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
                                       float multiplier, float cap, int window, int max_context, int blocks, float* partials,
                                       int* arrive, int arrive_ints, int* status, cudaStream_t stream) {
   if (T <= 0) return GLINT_OK;
-  if (!partials || !arrive || blocks < 1 || ((uintptr_t)partials & 15)) return GLINT_ERR_BAD_ARG;
+  if (!partials || !arrive || blocks < 1 || max_pages < 1 || ((uintptr_t)partials & 15)) return GLINT_ERR_BAD_ARG;
   if (!glint_attention_decode8_supported(nh, nkv, hd, page_size)) return GLINT_ERR_UNSUPPORTED_SIZE;
   if (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)q | (uintptr_t)out) & 15) return GLINT_ERR_UNSUPPORTED_SIZE;
   const long long rows = (long long)num_pages * nkv * page_size;
@@ -750,8 +759,12 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
   long long most_pages = ((long long)max_context + page_size - 1) / page_size;
   if (window > 0 && ((long long)window + page_size - 1) / page_size + 1 < most_pages)
     most_pages = ((long long)window + page_size - 1) / page_size + 1;
-  // units are counted in 32 bits
-  const long long fits = 0x3fffffffLL / ((long long)pairs * (most_pages + pair_cost));
+  // units are counted in 32 bits, whatever the positions turn out to be
+  long long table_pages = (long long)max_pages * splits;
+  if (table_pages > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
+  if (window > 0 && ((long long)window + page_size - 1) / page_size + 1 < table_pages)
+    table_pages = ((long long)window + page_size - 1) / page_size + 1;
+  const long long fits = 0x3fffffffLL / ((long long)pairs * (table_pages + pair_cost));
   if (fits < 1) return GLINT_ERR_UNSUPPORTED_SIZE;
   int step = arrive_ints / pairs < D8_MAX_TOKENS ? arrive_ints / pairs : D8_MAX_TOKENS;
   if (fits < step) step = (int)fits;

@@ -269,6 +269,31 @@ def test_bad_pages_and_orders_are_reported_and_nothing_is_written(rts):
         rt.check_status()
 
 
+def test_positions_outside_the_block_table_are_reported():
+    """Single tokens at positions that the block table has no room for, or below zero: reported, and the others' results are
+    what they are without them, up to the order of their sums (a few ulp of 32 bits of values up to 8, before the result's
+    rounding)."""
+    from glint_b200 import ops_cache8
+    from glint_b200.errors import KernelError
+    from glint_b200.runtime import Runtime
+    rt, nh, nkv, hd = Runtime(DEV, "bfloat16"), 2, 1, 32
+    q = (0.1 * torch.randn(3, nh * hd, generator=torch.Generator().manual_seed(1))).to(DEV, torch.bfloat16)
+    for P in (16, 128):
+        for window in (0, 20):
+            s = Setup(rt, [1, 1, 1], [3, 40, 20], nkv, hd, P, seed=3)
+            good = ops_cache8.attention(rt, s.cache, s.step, q, nh, 1.0, window=window)
+            rt.check_status()
+            for bad in (-1, -1000, -2 ** 31, 16 * 128, 2 ** 31 - 1):
+                s.step.tensors["positions"][1] = bad
+                out = ops_cache8.attention(rt, s.cache, s.step, q, nh, 1.0, window=window)
+                with pytest.raises(KernelError, match="attention read"):
+                    rt.check_status()
+                far = (out[[0, 2]].float() - good[[0, 2]].float()).abs()
+                assert (far <= 2.0 ** -7 * good[[0, 2]].float().abs() + 2.0 ** -17).all()
+                if bad < 0:
+                    assert not out[1].any()
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("lens,starts,nkv,hd,P,window", [([1], [0], 1, 16, 16, 0), ([3, 1, 40], [0, 50, 30], 2, 48, 16, 0),
                                                          ([5, 20], [100, 63], 3, 10, 7, 20), ([9], [200], 2, 128, 64, 64)])
