@@ -11,10 +11,11 @@
 //   warp 2     tcgen05.mma: O += P V, P (bfloat16 pairs) from one of two buffers of tensor memory
 //   warps 4-7  softmax of the even tiles, warps 8-11 of the odd ones, one thread per row: no maximum or sum is exchanged
 //              within a tile, and one group computes while the other loads, stores and waits
-// With a soft cap of up to 55 the exponentials need no running maximum at all: scores lie within +-cap, so that probabilities
-// relative to cap / 2 lie between 2^-120 (2^-108 for a cap of 50) and 2^40, which float32 sums and bfloat16 probabilities hold
-// with the precision they always have.  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that has
-// grown by more than 8 log2 units, and O is rescaled then).
+// With a soft cap of up to 55 the exponentials need no running maximum at all: scores lie within +-cap (80 log2 units), and
+// probabilities relative to 2^10, between 2^-90 and 2^70, keep the precision they always have in float32 sums and as bfloat16.
+// So do their products with values of up to 2^36 (a row of 2^20 keys that all reach +cap) and down to 2^-36 (one whose
+// keys all stay at -cap).  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that
+// has grown by more than 8 log2 units, and O is rescaled then).
 // When there are fewer blocks than SMs (a few rows over a long context) the key tiles of a row are split over several
 // blocks, whose partial results a second kernel adds up in order.
 // Blocks are found from the portions' lengths, so that short portions beside long ones cost no empty blocks.
@@ -34,6 +35,7 @@ constexpr int AT_KV_SUB = AT_N * 128;
 constexpr int AT_STAGES = 4;          // most tiles of keys, or of values, in shared memory
 constexpr float AT_GROW = 8.f;        // log2 units
 constexpr float AT_FIXED_CAP = 55.f;  // largest soft cap whose exponentials need no maximum
+constexpr float AT_FIXED_REF = 10.f;  // log2 units: their reference
 
 struct PortionParams {
   const int* cu_seqlens;
@@ -202,7 +204,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint64_t* empty = values ? sh->v_empty : sh->k_empty;
     uint8_t* ring = values ? sv : sk;
     const int stages = values ? p.v_stages : p.k_stages;
-    // pages outside [page_lo, page_hi] are masked; they are filled from page 0, which is finite as all wide values are
+    // pages outside [page_lo, page_hi] are masked; they are filled from page 0, whose values are finite as all wide ones are
     auto fetch = [&](int j) -> int {
       const int page_idx = first_page + j * ppt + lane;
       return lane < ppt ? table[min(max(page_idx, page_lo), page_hi)] : 0;
@@ -336,7 +338,6 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const float LOG2E = 1.4426950408889634f;
     const float in_scale = p.cap > 0.f ? p.multiplier / p.cap : p.multiplier;
     const float out_scale = p.cap > 0.f ? p.cap * LOG2E : LOG2E;   // scores are kept in log2 units
-    const float fixed_ref = 0.5f * out_scale;
     float ref = -INFINITY, l = 0.f;
     bool ok = true;                                      // the same in all lanes of a warp
     constexpr int CH = PAIR ? 32 : AT_N;                 // columns in registers at a time
@@ -361,7 +362,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             const float v = tc::tanh_approx(__uint_as_float(raw[c]) * in_scale);
-            raw[c] = __float_as_uint(FIXED ? fmaf(v, out_scale, -fixed_ref) : v * out_scale);
+            raw[c] = __float_as_uint(FIXED ? fmaf(v, out_scale, -AT_FIXED_REF) : v * out_scale);
           }
         } else {
 #pragma unroll

@@ -409,8 +409,9 @@ __device__ __forceinline__ int unpack_page(const UnpackParams& p, int r, int ord
   const int start = p.seq_start[r], n = p.cu_seqlens[r + 1] - p.cu_seqlens[r];
   if (n <= 0) return -1;
   const int lo = p.window > 0 && start - p.window + 1 > 0 ? (start - p.window + 1) / p.page_size : 0;
-  const int place = lo + ordinal;
-  if (place > (start + n - 1) / p.page_size) return -1;
+  const int place = lo + ordinal, last = (start + n - 1) / p.page_size;
+  if (place > last) return -1;
+  if (ordinal == (int)gridDim.x - 1 && place < last && threadIdx.x == 0) atomicExch(p.status, 6);    // the rest stays as it was
   const int page = place >= p.max_pages ? -1 : p.block_table[(size_t)r * p.max_pages + place];
   if (page < 0 || page >= p.num_pages) {
     if (threadIdx.x == 0) atomicExch(p.status, 3);
@@ -549,7 +550,7 @@ GLINT_API int glint_rope_append(const float* qkv, const int* positions, const in
 
 // Codes of the pages that the new tokens of each request can reach (from the page of the first key that the first of
 // them sees, to the page of the last of them) as values of `dtype`, at the same places of the wide pools.
-// `most_pages`: at least the pages of any request's range.
+// `most_pages`: at least the pages of any request's range (status 6 where it is less).
 GLINT_API int glint_cache8_unpack(const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
                                   const int* seq_start, const int* cu_seqlens, const int* block_table, int max_pages,
                                   void* k_out, void* v_out, int dtype, int n_seqs, int most_pages, int window, int nkv,

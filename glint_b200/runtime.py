@@ -13,7 +13,8 @@ _STATUS_TEXT = {1: "a token id lies outside the embedding table",
                 2: "a token's position has no page in its block table (cache write)",
                 3: "a key's position has no page in its block table (attention read)",
                 4: "a bounded device-side wait ran out",
-                5: "a request's tokens do not stand together in ascending positions (cache write)"}
+                5: "a request's tokens do not stand together in ascending positions (cache write)",
+                6: "a request holds more tokens than its step was made for (attention read)"}
 
 
 def parse_dtype(dtype):

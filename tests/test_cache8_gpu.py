@@ -261,6 +261,11 @@ def test_bad_pages_and_orders_are_reported_and_nothing_is_written(rts):
     with pytest.raises(KernelError, match="attention read"):
         rt.check_status()
     assert not s.cache.k_wide.any() and not s.cache.v_wide.any()
+    s = Setup(rt, [2, 3], [3, 20], nkv, hd, 16, seed=3)
+    short = ops_cache8.StepArrays(*[s.step.tensors[m] for m in ("positions", "token_seq", "seq_start", "cu_seqlens", "block_table")], 3, 16)
+    ops_cache8.unpack(rt, s.cache, short)
+    with pytest.raises(KernelError, match="more tokens than its step"):
+        rt.check_status()
     q = torch.zeros(2, nh * hd, dtype=torch.bfloat16, device=DEV)
     s = Setup(rt, [1, 1], [3, 20], nkv, hd, 16, seed=3)
     s.step.tensors["block_table"].fill_(10 ** 6)
@@ -336,6 +341,13 @@ ATTENDS = [  # lens, starts, nh, nkv, hd, page, window, cap
     ([130, 65], [1000, 64], 6, 3, 80, 32, 200, 0.0),
     ([40], [100], 4, 4, 96, 64, 0, 0.0),
     ([40, 1], [100, 3], 4, 2, 64, 48, 30, 10.0),                  # pages that the tiled kernel does not take
+    ([2 + i % 7 for i in range(75)], [(5 * i) % 200 for i in range(75)], 4, 2, 64, 16, 0, 50.0),     # more requests than a warp has lanes
+    ([1] * 3 + [3] * 40 + [90, 20], [9, 100, 40] + [(11 * i) % 90 for i in range(40)] + [70, 130], 12, 4, 112, 32, 0, 0.0),
+    ([130], [1500], 4, 2, 64, 16, 0, 50.0),                       # keys split over blocks, ...
+    ([130], [1500], 4, 2, 64, 16, 0, 56.0),                       # ... with a running maximum
+    ([100, 40], [2000, 1000], 6, 2, 128, 16, 0, 0.0),
+    ([150, 3], [1700, 1200], 2, 1, 256, 64, 900, 0.0),            # ... through a window
+    ([90] + [2] * 40, [2600] + [700 + i for i in range(40)], 10, 2, 48, 16, 0, 30.0),
 ]
 
 
@@ -378,6 +390,32 @@ def test_attention_against_the_definition(rts, dtype, case):
                     bound = (2e-4 if dtype == "float32" else 0.012) * np.abs(v[lo:p + 1]).max()
                     err = np.abs(got[s.cu[r] + i, head] - want).max()
                     assert err <= bound, (r, i, head, err, bound)
+
+
+@pytest.mark.parametrize("lens,starts,hd,cap", [([150], [0], 256, 50.0), ([150], [0], 64, 55.0), ([130], [1500], 128, 55.0), ([1], [70], 128, 55.0)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("e", [-43, 0, 28])
+def test_scores_that_all_reach_the_cap(rts, lens, starts, hd, cap, sign, e):
+    """Every score at +cap or at -cap, over values of up to 2^-36, 2^7 and 2^35: the mean of the values.  Probabilities are
+    equal, so that only their own rounding and the result's is left (2^-9 each), and tanh.approx does not matter: 0.012 of the
+    largest value as elsewhere."""
+    from glint_b200 import ops_cache8
+    rt, nh, nkv, P = rts["bfloat16"], 4, 2, 16
+    s = Setup(rt, lens, starts, nkv, hd, P, seed=9)
+    s.codes[0][:] = 255
+    s.cache.k.fill_(255)
+    s.e[0][:], s.e[1][:] = 0, e
+    s.cache.k_scale.fill_(1.0)
+    s.cache.v_scale.fill_(2.0 ** e)
+    q = torch.full((sum(lens), nh * hd), 8.0 * sign, dtype=torch.bfloat16, device=DEV)
+    out = ops_cache8.attention(rt, s.cache, s.step, q, nh, 1.0, softcap=cap)
+    rt.check_status()
+    got = out.double().cpu().numpy().reshape(-1, nh, hd)
+    for i in sorted({0, lens[0] // 2, lens[0] - 1}):
+        for head in range(nh):
+            v = s.values(1, 0, head // 2)[:starts[0] + i + 1]
+            err = np.abs(got[i, head] - v.mean(axis=0)).max()
+            assert err <= 0.012 * np.abs(v).max(), (i, head, err / np.abs(v).max())
 
 
 @pytest.mark.parametrize("case", [2, 4, 8, 14])
