@@ -16,8 +16,8 @@
 // So do their products with values of up to 2^36 (a row of 2^20 keys that all reach +cap) and down to 2^-36 (one whose
 // keys all stay at -cap).  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that
 // has grown by more than 8 log2 units, and O is rescaled then).
-// When there are fewer blocks than SMs (a few rows over a long context) the key tiles of a row are split over several
-// blocks, whose partial results a second kernel adds up in order.
+// Where SMs would stay empty (fewer blocks than SMs, or a few blocks behind the last full round of them) the keys of a tile of
+// rows are split over several blocks, whose partial results a second kernel adds up in order.
 // Blocks are found from the portions' lengths, so that short portions beside long ones cost no empty blocks.
 // Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx; keys of a token at position p from
 // max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the second product, and their sum
@@ -33,6 +33,8 @@ constexpr int AT_THREADS = 384;
 constexpr int AT_Q_SUB = AT_M * 128;  // bytes of a 64-column slice of the query tile
 constexpr int AT_KV_SUB = AT_N * 128;
 constexpr int AT_STAGES = 4;          // most tiles of keys, or of values, in shared memory
+constexpr int AT_LEAST = 4;           // key tiles of a split
+constexpr int AT_TAIL = 8;            // key tiles from which those behind the last full round are split
 constexpr float AT_GROW = 8.f;        // log2 units
 constexpr float AT_FIXED_CAP = 55.f;  // largest soft cap whose exponentials need no maximum
 constexpr float AT_FIXED_REF = 10.f;  // log2 units: their reference
@@ -42,11 +44,14 @@ struct PortionParams {
   const int* seq_start;
   const int* block_table;
   __nv_bfloat16* out;
-  float* part_o;                // [splits][T * nh][hd], null: one split
-  float2* part_ml;              // [splits][T * nh] (reference in log2 units, sum)
+  float* part_o;                // [splits][split tiles][128][hd]
+  float2* part_ml;              // [splits][split tiles][128] (reference in log2 units, sum)
+  int4* part_info;              // [split tiles]: parts (below 2: nothing to add up), rows, first token, kv head
   int* status;
   float multiplier, cap;
-  int max_pages, T, nh, nkv, hd, page_size, num_pages, window, n_seqs, whole, per_split, k_stages, v_stages;
+  int max_pages, nh, nkv, hd, page_size, num_pages, window, n_seqs, whole, k_stages, v_stages;
+  int split_from, splits;       // tiles (query tile, kv head) from there on have their keys split over that many blocks
+  int split_tiles;              // and are that many
 };
 
 struct PortionShared {
@@ -55,6 +60,7 @@ struct PortionShared {
   uint64_t k_full[AT_STAGES], k_empty[AT_STAGES], v_full[AT_STAGES], v_empty[AT_STAGES];
   uint32_t tmem_base;
   int abort_flag;
+  int part_tile;                // where this block's partial results go, in tiles of rows (-1: it has all keys)
   float row_ref[AT_M];
   float row_sum[2][AT_M];
   float row_own[2][AT_M];
@@ -112,6 +118,23 @@ __device__ __forceinline__ bool portion_tile(const PortionParams& p, int tok_per
   return false;
 }
 
+// The keys of a query tile, and what a split of them takes: tiles of 64, an even share of at least AT_LEAST.
+struct PortionKeys {
+  int pos0, pos_last, kv_first, begin, tiles, per, parts;
+};
+__device__ __forceinline__ PortionKeys portion_keys(const PortionParams& p, const PortionTile& w, int tok_per_tile, bool split) {
+  PortionKeys k;
+  const int tok0 = w.tile * tok_per_tile;
+  k.pos0 = w.start + tok0;
+  k.pos_last = k.pos0 + min(tok_per_tile, w.len - tok0) - 1;
+  k.kv_first = p.window > 0 ? max(0, k.pos0 - p.window + 1) : 0;
+  k.begin = k.kv_first & ~(AT_N - 1);
+  k.tiles = (k.pos_last - k.begin + AT_N) / AT_N;
+  k.per = split ? max(AT_LEAST, (k.tiles + p.splits - 1) / p.splits) : k.tiles;
+  k.parts = split ? (k.tiles + k.per - 1) / k.per : 1;
+  return k;
+}
+
 // FIXED: the soft cap spares the running maximum.  PAIR: two blocks on an SM (head sizes up to 128): each has half of the
 // tensor memory, so that P is written over the scores it came from and the scores two tiles on wait for the product that
 // reads it; one block's beginning and end pass under the other's tiles.
@@ -159,20 +182,30 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 0) atomicExch(p.status, 4);
     return;
   }
-  // blockIdx.x counts (query tile from the last, kv head), blockIdx.y the splits
-  const int kvh = (int)blockIdx.x % p.nkv, split = blockIdx.y;
+  // blocks count (query tile from the last, kv head); from split_from on every such tile has `splits` blocks
+  const bool may_split = (int)blockIdx.x >= p.split_from;
+  const int behind = may_split ? (int)blockIdx.x - p.split_from : 0;
+  const int split = may_split ? behind / p.split_tiles : 0, split_tile = behind - split * p.split_tiles;
+  const int index = may_split ? p.split_from + split_tile : (int)blockIdx.x;
+  const int kvh = index % p.nkv;
   PortionTile work;
-  if (!portion_tile(p, tok_per_tile, (int)blockIdx.x / p.nkv, work)) return;
+  if (!portion_tile(p, tok_per_tile, index / p.nkv, work)) {
+    if (may_split && threadIdx.x == 0) p.part_info[split_tile] = make_int4(0, 0, 0, 0);
+    return;
+  }
   const int seq = work.seq, tile = work.tile, t_begin = work.begin, q_len = work.len;
   const int tok0 = tile * tok_per_tile;
   const int n_tok = min(tok_per_tile, q_len - tok0);
   const int n_rows = n_tok * G;
-  const int pos0 = work.start + tok0;
-  const int pos_last = pos0 + n_tok - 1;
-  const int kv_first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
-  const int kv_begin = (kv_first & ~(AT_N - 1)) + split * p.per_split * AT_N;     // this split's first tile
-  const int n_tiles = min(p.per_split, (pos_last - kv_begin + AT_N) / AT_N);
-  if (kv_begin > pos_last) return;                       // the rows' keys end before this split (the same for all threads)
+  const PortionKeys keys = portion_keys(p, work, tok_per_tile, may_split);
+  const int pos0 = keys.pos0, pos_last = keys.pos_last, kv_first = keys.kv_first;
+  const int kv_begin = keys.begin + split * keys.per * AT_N;                      // this split's first tile
+  const int n_tiles = min(keys.per, keys.tiles - split * keys.per);
+  if (n_tiles <= 0) return;                              // fewer parts than blocks (the same for all threads)
+  if (threadIdx.x == 4 * 32) {
+    sh->part_tile = keys.parts > 1 ? split * p.split_tiles + split_tile : -1;
+    if (may_split && split == 0) p.part_info[split_tile] = make_int4(keys.parts, n_rows, t_begin + tok0, kvh);
+  }
   if (warp != 0 && warp != 3) {                          // the producers begin at once
     if (warp == 1) tc::tmem_alloc(&sh->tmem_base, TMEM_COLS);
     tc::fence_before_thread_sync();
@@ -443,6 +476,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     sh->row_sum[group][r] = l;
     sh->row_own[group][r] = ref;
     asm volatile("bar.sync 2, 256;" ::: "memory");
+    const bool partial = sh->part_tile >= 0;
+    const size_t part_row = (size_t)max(sh->part_tile, 0) * AT_M;
     if (ok) ok = warp_wait(&sh->o_full, 0, abort_flag);
     if (ok) {
       tc::fence_after_thread_sync();
@@ -456,15 +491,12 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           else total += sh->row_sum[b][r];               // 0, or NaN where every score was
       }
       const int o_lo = group ? ((hd16 + 1) >> 1) * 16 : 0, o_hi = group ? hd : ((hd16 + 1) >> 1) * 16;
-      const float inv = p.part_o ? 1.f : total == 0.f ? 0.f : 1.0f / total;
-      if (p.part_o && rv && group == 0) {
-        const size_t row = (size_t)(t_begin + tok0 + r / G) * p.nh + kvh * G + r % G;
-        p.part_ml[(size_t)split * p.T * p.nh + row] = make_float2(last, total);
-      }
+      const float inv = total == 0.f ? 0.f : 1.0f / total;
+      if (partial && rv && group == 0) p.part_ml[part_row + r] = make_float2(last, total);
       // Rows go out by way of shared memory, which all copies and products have left: a thread has a row of O, but a
       // warp should write rows as a whole (a thread writing its own row's 32 bytes at a time took 5 us).  16-byte chunk c of
       // row r sits at c ^ (r mod 8), as far as the chunks of a row are a multiple of a power of two.
-      const int chunk_shift = p.part_o ? 2 : 3;          // elements of a chunk: 4 floats, 8 bfloat16
+      const int chunk_shift = partial ? 2 : 3;          // elements of a chunk: 4 floats, 8 bfloat16
       const int chunks = hd >> chunk_shift, swizzle = r & 7 & ((chunks & -chunks) - 1);
       uint4* row_at = reinterpret_cast<uint4*>(smem) + (size_t)r * chunks;
       for (int c0 = o_lo; c0 < o_hi; c0 += 32) {
@@ -477,7 +509,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           if (c0 + 16 * half >= o_hi) break;
           const uint32_t* v = o + 16 * half;
           const int c = (c0 + 16 * half) >> chunk_shift;
-          if (p.part_o) {
+          if (partial) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) row_at[(c + i) ^ swizzle] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           } else {
@@ -496,10 +528,10 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     asm volatile("bar.sync 2, 256;" ::: "memory");
     if (ok) {
       // 8, 16 or 32 lanes to a row; a warp's rows are 8 x (rows at once) apart, their (token, head) counted without division
-      const int chunks = hd >> (p.part_o ? 2 : 3);
+      const int chunks = hd >> (partial ? 2 : 3);
       const int lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32, at_once = 32 / lanes, step = 8 * at_once;
       const int step_tok = step / G, step_head = step - step_tok * G, wrap = (chunks & -chunks) - 1;
-      uint4* to = p.part_o ? reinterpret_cast<uint4*>(p.part_o + (size_t)split * p.T * p.nh * hd) : reinterpret_cast<uint4*>(p.out);
+      uint4* to = partial ? reinterpret_cast<uint4*>(p.part_o + part_row * hd) : reinterpret_cast<uint4*>(p.out);
       int row = (warp - 4) * at_once + lane / lanes;
       int tok = row / G, head = row - tok * G;
       const int c0 = lane & (lanes - 1);
@@ -523,7 +555,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           int t_ = tok, h_ = head;
 #pragma unroll
           for (int k = 0; k < AHEAD; ++k) {
-            if (row + k * step < n_rows) to[((size_t)(t_begin + tok0 + t_) * p.nh + kvh * G + h_) * chunks + c] = v[k];
+            const size_t to_row = partial ? (size_t)(row + k * step) : (size_t)(t_begin + tok0 + t_) * p.nh + kvh * G + h_;
+            if (row + k * step < n_rows) to[to_row * chunks + c] = v[k];
             advance(t_, h_);
           }
         }
@@ -541,32 +574,23 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (threadIdx.x == 0 && sh->abort_flag) atomicExch(p.status, 4);
 }
 
-// Adds up the splits of every row, in order: a warp per row.
+// Adds up the parts of every row of the split tiles, in order: a warp per row, 16 blocks per tile.  Short and bound by its
+// round trips (7 us for 32 tiles of 4 parts, 16.8 MB): few registers, so that its blocks wait beside the last ones of
+// the kernel in front (with four parts in flight, 70 registers, they did not fit and the two took 1 us more).
 __global__ void __launch_bounds__(256) attention_portion_merge_kernel(const PortionParams p) {
   pdl_wait_release();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int t = row / p.nh;
-  // the request of the token: portions are few, and their offsets ascend
-  int seq = -1;
-  for (int b = 0; b < p.n_seqs && seq < 0; b += 32) {
-    const bool here = b + lane < p.n_seqs && p.cu_seqlens[b + lane] <= t && t < p.cu_seqlens[b + lane + 1];
-    const unsigned hit = __ballot_sync(0xffffffffu, here);
-    if (hit) seq = b + __ffs(hit) - 1;
-  }
-  if (t >= p.T || seq < 0) return;                       // a token in front of the portions
-  const int G = p.nh / p.nkv, tok_per_tile = AT_M / G;
-  const int tok0 = (t - p.cu_seqlens[seq]) / tok_per_tile * tok_per_tile;
-  const int q_len = p.cu_seqlens[seq + 1] - p.cu_seqlens[seq];
-  const int pos0 = p.seq_start[seq] + tok0, pos_last = pos0 + min(tok_per_tile, q_len - tok0) - 1;
-  const int kv_begin = (p.window > 0 ? max(0, pos0 - p.window + 1) : 0) & ~(AT_N - 1);
-  const int parts = ((pos_last - kv_begin) / AT_N + p.per_split) / p.per_split;
-  const size_t stride = (size_t)p.T * p.nh;
+  const int split_tile = blockIdx.x >> 4, r = (blockIdx.x & 15) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int4 info = p.part_info[split_tile];
+  const int parts = info.x, G = p.nh / p.nkv;
+  if (parts < 2 || r >= info.y) return;
+  const size_t from = (size_t)split_tile * AT_M + r, stride = (size_t)p.split_tiles * AT_M;
+  const size_t row = (size_t)(info.z + r / G) * p.nh + info.w * G + r % G;
   float M = -INFINITY;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.part_ml[s * stride + row].x);
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.part_ml[s * stride + from].x);
   float L = 0.f;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int s = 0; s < parts; ++s) {
-    const float2 ml = p.part_ml[s * stride + row];
+    const float2 ml = p.part_ml[s * stride + from];
     // a split whose keys are all masked for this row has no reference and L = 0; one whose scores were NaN has L = NaN
     const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : tc::exp2_approx(ml.x - M);
     L += ml.y * w;
@@ -574,7 +598,7 @@ __global__ void __launch_bounds__(256) attention_portion_merge_kernel(const Port
     for (int k = 0; k < 2; ++k) {
       const int d = lane * 4 + k * 128;
       if (d < p.hd) {
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * stride + row) * p.hd + d);
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * stride + from) * p.hd + d);
         acc[k].x += v.x * w; acc[k].y += v.y * w; acc[k].z += v.z * w; acc[k].w += v.w * w;
       }
     }
@@ -585,7 +609,7 @@ __global__ void __launch_bounds__(256) attention_portion_merge_kernel(const Port
     const int d = lane * 4 + k * 128;
     if (d < p.hd) {
       const __nv_bfloat162 a = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv), b = __floats2bfloat162_rn(acc[k].z * inv, acc[k].w * inv);
-      *reinterpret_cast<uint2*>(p.out + (size_t)row * p.hd + d) =
+      *reinterpret_cast<uint2*>(p.out + row * p.hd + d) =
           make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
   }
@@ -630,14 +654,14 @@ GLINT_API int glint_attention_portion_supported(int nh, int nkv, int hd, int pag
 }
 
 // q, out: [T, nh * hd] bf16; pools [pages][nkv][page_size][hd] bf16, finite everywhere; cu_seqlens (absolute token offsets),
-// seq_start and block_table of the n_seqs portions, of which none is longer than max_q_len or attends more than
+// seq_start and block_table of the n_seqs portions, which have `tokens` tokens in all and of which none is longer than max_q_len or attends more than
 // max_context keys.  `scratch`: floats for partial results, 16-byte aligned (none, or too few: the keys are not split).
 GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const void* v_pool, const int* cu_seqlens,
                                       const int* seq_start, const int* block_table, int max_pages, void* out, int T,
-                                      int n_seqs, int max_q_len, int max_context, int nh, int nkv, int hd, int page_size,
+                                      int tokens, int n_seqs, int max_q_len, int max_context, int nh, int nkv, int hd, int page_size,
                                       int num_pages, float multiplier, float cap, int window, int sms, float* scratch,
                                       long long scratch_floats, int* status, cudaStream_t stream) {
-  if (n_seqs <= 0 || max_q_len <= 0 || T <= 0) return GLINT_OK;
+  if (n_seqs <= 0 || max_q_len <= 0 || tokens <= 0 || T < tokens) return GLINT_OK;
   if (!glint_attention_portion_supported(nh, nkv, hd, page_size)) return GLINT_ERR_UNSUPPORTED_SIZE;
   if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) return GLINT_ERR_UNSUPPORTED_SIZE;
   if ((long long)num_pages * nkv * page_size > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
@@ -672,7 +696,7 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   }
   if (rc != GLINT_OK) return rc;
   PortionParams p = {};
-  p.cu_seqlens = cu_seqlens; p.seq_start = seq_start; p.block_table = block_table; p.max_pages = max_pages; p.T = T;
+  p.cu_seqlens = cu_seqlens; p.seq_start = seq_start; p.block_table = block_table; p.max_pages = max_pages;
   p.out = (__nv_bfloat16*)out; p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.num_pages = num_pages;
   p.multiplier = multiplier; p.cap = cap; p.window = window; p.whole = whole; p.status = status; p.n_seqs = n_seqs;
   const int nsub = (hd + 63) / 64;
@@ -685,27 +709,45 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
     else --p.k_stages;
   }
   const int smem = bytes(p.k_stages, p.v_stages);
-  // at most a tile more than whole ones for every portion
-  const long long blocks = ((long long)T / tok_per_tile + n_seqs) * nkv;
-  if (blocks > 0x7fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
-  // Fewer blocks than SMs: their keys are split, as far as that makes work for all SMs and leaves a split four tiles.
-  const long long reach = window > 0 && (long long)window + max_q_len < max_context ? (long long)window + max_q_len + AT_N : max_context;
-  const int most_tiles = (int)((reach + AT_N - 1) / AT_N);
-  int splits = (int)(sms * (pair ? 2 : 1) / blocks);
-  if (splits > most_tiles / 4) splits = most_tiles / 4;
-  const long long part = (long long)T * nh * (hd + 2);
-  if (splits > 1 && (!scratch || ((uintptr_t)scratch & 15) || part * splits > scratch_floats))
-    splits = scratch && !((uintptr_t)scratch & 15) ? (int)(scratch_floats / part) : 1;
-  if (splits < 1) splits = 1;
-  p.per_split = (most_tiles + splits - 1) / splits;
-  splits = (most_tiles + p.per_split - 1) / p.per_split;
-  if (splits > 1) {
-    p.part_o = scratch;
-    p.part_ml = reinterpret_cast<float2*>(scratch + (long long)splits * T * nh * hd);
-  } else {
-    p.per_split = 0x7fffff;                              // all of them, whatever max_context said
+  // n tokens make at most (n - 1) / tok_per_tile + 1 tiles of a portion
+  const long long blocks = ((tokens > n_seqs ? ((long long)tokens - n_seqs) / tok_per_tile : 0) + n_seqs) * nkv;
+  if (blocks > 0x3fffffffLL) return GLINT_ERR_UNSUPPORTED_SIZE;
+  // Keys are split where SMs would stay empty: those of all tiles when these are fewer than the SMs, else of the tiles
+  // behind the last full round.  A key tile takes about 1 us of an SM, 1.75 us when two blocks share it; partial results and
+  // their sum cost about as much as 9 key tiles (12 behind full rounds, whose blocks do not all end together; 16 with two
+  // blocks to an SM).  Measured (us, unsplit / one split block to an SM / two): heads of 128, 96 tiles (one part only fits)
+  // over 7,000 keys 116 / - / 84, over 1,024 keys 24 / - / 30; 64 tiles over 7,000 - / 71 / 66, 16 tiles - / 29 / 33; 304 tiles
+  // over 7,000 keys 278 / 208 and over 1,024 53 / 46; heads of 256, 152 tiles over 3,000 keys 95 / 74, over 500 32 / 36.
+  const long long before = ((long long)max_context - max_q_len) / (n_seqs > 1 ? 2 : 1);     // cached tokens, of several portions half the most
+  const bool tail = blocks > sms;
+  const long long keys = tail ? (window > 0 && window < before ? window : before) + tok_per_tile
+                              : window > 0 && (long long)window + tok_per_tile + AT_N < max_context ? (long long)window + tok_per_tile + AT_N : max_context;
+  const int tiles = (int)((keys + AT_N - 1) / AT_N);
+  p.split_from = tail ? (int)(blocks / sms * sms) : 0;
+  p.split_tiles = (int)blocks - p.split_from;
+  p.splits = 1;
+  if (p.split_tiles) {
+    const int most = tiles / AT_LEAST, one = min(sms / p.split_tiles, most), two = min(2 * sms / p.split_tiles, most);
+    float least = (float)tiles;
+    if (one > 1 && (float)tiles / one + (tail ? 12.f : 9.f) < least) {
+      p.splits = one;
+      least = (float)tiles / one + 9.f;
+    }
+    if (pair && !tail && two > one && 1.75f * tiles / two + 16.f < least) p.splits = two;
   }
-  const dim3 grid((unsigned)blocks, splits);
+  const long long part = (long long)p.split_tiles * (AT_M * (hd + 2) + 4);      // floats of a split, and of what is said of its tiles
+  if (p.splits > 1 && (!scratch || ((uintptr_t)scratch & 15) || part * p.splits > scratch_floats))
+    p.splits = scratch && !((uintptr_t)scratch & 15) ? (int)(scratch_floats / part) : 1;
+  if (p.splits < 2) {
+    p.splits = 1;
+    p.split_tiles = 0;
+    p.split_from = (int)blocks;
+  } else {
+    p.part_info = reinterpret_cast<int4*>(scratch);
+    p.part_o = scratch + (long long)p.split_tiles * 4;
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (long long)p.splits * p.split_tiles * AT_M * hd);
+  }
+  const dim3 grid((unsigned)(p.split_from + p.split_tiles * p.splits));
   const bool fixed = cap > 0.f && cap <= AT_FIXED_CAP;
   cudaError_t e = cudaSuccess;
 #define LAUNCH(FIXED, PAIR)                                                                                             \
@@ -720,7 +762,7 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
     if (fixed) LAUNCH(true, false) else LAUNCH(false, false)
   }
 #undef LAUNCH
-  if (e == cudaSuccess && splits > 1)
-    e = launch_kernel(attention_portion_merge_kernel, dim3((unsigned)(((long long)T * nh + 7) / 8)), dim3(256), 0, stream, p);
+  if (e == cudaSuccess && p.split_tiles)
+    e = launch_kernel(attention_portion_merge_kernel, dim3((unsigned)(p.split_tiles * (AT_M / 8))), dim3(256), 0, stream, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }

@@ -345,7 +345,7 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
   if (rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_portion && rest.max_seq_len > 1 &&
       t.attention_portion_supported(nh, nkv, hd, page))
     return counted(t.attention_portion(q, wide.k, wide.v, rest.cu_seqlens, rest.seq_start, rest.block_table[g], rest.max_pages[g],
-                                       out, step->num_tokens, rest.num_seqs, rest.max_seq_len, rest.max_context, nh, nkv, hd, page,
+                                       out, step->num_tokens, step->num_tokens - lead, rest.num_seqs, rest.max_seq_len, rest.max_context, nh, nkv, hd, page,
                                        view->num_pages, multiplier, cap, window, rt->sms, view->partials, view->partial_floats,
                                        rt->status, stream));
   return glint_op_attention(rt, lead ? &rest : step, q, &wide, out, nh, nkv, hd, multiplier, cap, window, stream);

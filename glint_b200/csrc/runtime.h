@@ -56,7 +56,7 @@ struct GlintTensorEntries {
                            int, int*, cudaStream_t);
   int (*attention_decode8_supported)(int, int, int, int);
   long long (*attention_decode8_workspace)(int, int, int, int);
-  int (*attention_portion)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int, int, int,
+  int (*attention_portion)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int, int, int, int,
                            int, int, int, int, int, int, float, float, int, int, float*, long long, int*, cudaStream_t);
   int (*attention_portion_supported)(int, int, int, int);
   int (*attention_prefill)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int,

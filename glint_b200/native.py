@@ -75,7 +75,7 @@ def cache8_scratch(num_kv_heads, head_dim, device):
     blocks of 128 rows as the SMs hold.  It belongs to one cache, like the wide pages: launches on one stream share it."""
     sms = torch.cuda.get_device_properties(device).multi_processor_count if torch.device(device).type == "cuda" else 1
     rows = 128 * sms * (2 if head_dim <= 128 else 1)
-    return (torch.empty(max(2 * sms * 2 * 8 * (head_dim + 4), rows * (head_dim + 2)), dtype=torch.float32, device=device),
+    return (torch.empty(max(2 * sms * 2 * 8 * (head_dim + 4), rows * (head_dim + 2) + 4 * rows // 128), dtype=torch.float32, device=device),
             torch.zeros(CACHE8_ARRIVE, dtype=torch.int32, device=device))
 
 
