@@ -293,8 +293,8 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     tc::tma_prefetch_desc(&map_k);
     tc::tma_prefetch_desc(&map_v);
   }
-  pdl_wait_release();
-  // ---- where this block begins: every warp scans the tokens' units for itself, some consecutive tokens per lane -----
+  // ---- where this block begins: every warp scans the tokens' units for itself, some consecutive tokens per lane.  Positions,
+  // requests and block tables come by copies, no kernel writes them: all this passes under the kernel in front. ---------
   const int per = (p.T + 31) >> 5;
   const int r0 = min(lane * per, p.T), r1 = min(r0 + per, p.T);
   int mine = 0, row_first = 0;
@@ -400,6 +400,7 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   // arrive 5 us later.
   {
     const int at = look_up(0, t, pos, row, pair, voff, remaining);
+    pdl_wait_release();
     const float ks = at >= 0 ? p.k_scale[at] : 0.f, vs = at >= 0 ? p.v_scale[at] : 1.f;
     __syncthreads();
     for (int s = warp; s < p.stages; s += D8_WARPS) fetch(s, s);          // a stage is always the same warp's

@@ -177,11 +177,6 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 66) tc::tma_prefetch_desc(&map_v);
   }
   __syncthreads();
-  pdl_wait_release();
-  if (tc::smem_u32(at_raw) & 1023) {                     // the operands' swizzle wants it
-    if (threadIdx.x == 0) atomicExch(p.status, 4);
-    return;
-  }
   // blocks count (query tile from the last, kv head); from split_from on every such tile has `splits` blocks
   const bool may_split = (int)blockIdx.x >= p.split_from;
   const int behind = may_split ? (int)blockIdx.x - p.split_from : 0;
@@ -189,7 +184,13 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int index = may_split ? p.split_from + split_tile : (int)blockIdx.x;
   const int kvh = index % p.nkv;
   PortionTile work;
-  if (!portion_tile(p, tok_per_tile, index / p.nkv, work)) {
+  const bool found = portion_tile(p, tok_per_tile, index / p.nkv, work);         // no kernel writes what this reads
+  pdl_wait_release();
+  if (tc::smem_u32(at_raw) & 1023) {                     // the operands' swizzle wants it
+    if (threadIdx.x == 0) atomicExch(p.status, 4);
+    return;
+  }
+  if (!found) {
     if (may_split && threadIdx.x == 0) p.part_info[split_tile] = make_int4(0, 0, 0, 0);
     return;
   }

@@ -91,7 +91,6 @@ template <typename S, int NP, bool FULL>
 __global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const AppendParams p, int cache_blocks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int width = (p.nh + 2 * p.nkv) * p.hd, half = p.rot >> 1, pairs = p.hd >> 1;
-  pdl_wait_release();
   int2 at[NP];
   double turns[NP];
 #pragma unroll
@@ -107,6 +106,11 @@ __global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const App
     const long long unit = (long long)(blockIdx.x - cache_blocks) * AP_WARPS + warp;
     const int t = (int)(unit / groups), h0 = (int)(unit - (long long)t * groups) * AP_HEADS;
     if (t >= p.T) return;
+    const int pos = p.positions[t];
+    float2 turned_by[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) turned_by[k] = FULL || lane + 32 * k < half ? rope_angle(pos, turns[k], p.amplitude) : make_float2(1.f, 0.f);
+    pdl_wait_release();
     const float* src = p.qkv + (size_t)t * width + (size_t)h0 * p.hd;
     S* dst = (S*)p.q_out + ((size_t)t * p.nh + h0) * p.hd;
     float a[AP_HEADS][NP], b[AP_HEADS][NP];
@@ -118,12 +122,11 @@ __global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const App
           a[h][k] = src[h * p.hd + at[k].x];
           b[h][k] = src[h * p.hd + at[k].y];
         }
-    const int pos = p.positions[t];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       if (!FULL && lane + 32 * k >= pairs) continue;
       const bool turned = FULL || lane + 32 * k < half;
-      const float2 cs = turned ? rope_angle(pos, turns[k], p.amplitude) : make_float2(1.f, 0.f);
+      const float2 cs = turned_by[k];
 #pragma unroll
       for (int h = 0; h < AP_HEADS; ++h)
         if (h0 + h < p.nh) {
@@ -135,7 +138,8 @@ __global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const App
     return;
   }
 
-  // ---- keys and values -----------------------------------------------------------------------------------------------
+  // ---- keys and values.  Positions, requests and block tables come by copies, no kernel writes them: all that follows from
+  // them passes under the kernel in front. ---------------------------------------------------------------------------------
   // Of the window's tokens and those behind it that may belong to its runs: what a thread finds out for all.
   __shared__ unsigned starts[AP_WARPS], bad[AP_WARPS];    // does a run begin there; does it break the order
   __shared__ int poss[AP_WARPS * 32], offs[AP_WARPS * 32];
@@ -194,12 +198,9 @@ __global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const App
       b[k] = in ? row[at[k].y] : 0.f;
     }
   };
-  float a[AP_HELD][NP], b[AP_HELD][NP];
-#pragma unroll
-  for (int c = 0; c < AP_HELD; ++c)
-    if (first + warp + c * AP_WARPS < last) load(first + warp + c * AP_WARPS, a[c], b[c]);
   const bool coded = p.k_scale != nullptr;
   float* scale = is_v ? p.v_scale : p.k_scale;
+  int owned = -2;                                         // page of the run that this thread's token begins
   if (me >= first && me < last) {
     int w = me >> 5;
     unsigned m = starts[w] & (0xffffffffu >> (31 - (me & 31)));
@@ -216,10 +217,16 @@ __global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const App
         }
       }
       pages[me] = page;
-      olds[me] = coded && page >= 0 && offs[me] ? __float_as_uint(scale[(size_t)page * p.nkv + h]) & 0x7fffffffu : 0u;
       tops[me] = 0u;
+      owned = page;
     }
   }
+  pdl_wait_release();
+  float a[AP_HELD][NP], b[AP_HELD][NP];
+#pragma unroll
+  for (int c = 0; c < AP_HELD; ++c)
+    if (first + warp + c * AP_WARPS < last) load(first + warp + c * AP_WARPS, a[c], b[c]);
+  if (owned > -2) olds[me] = coded && owned >= 0 && offs[me] ? __float_as_uint(scale[(size_t)owned * p.nkv + h]) & 0x7fffffffu : 0u;
   __syncthreads();
   // rotates token i's values and brings their largest magnitude to its run
   auto prepare = [&](int i, float (&x)[NP], float (&y)[NP]) {
@@ -461,8 +468,8 @@ constexpr int UP_EACH = 2;                        // sixteens of a thread
 
 template <typename S>
 __global__ void __launch_bounds__(UP_THREADS) cache8_unpack_kernel(const UnpackParams p, int parts) {
+  const int page = unpack_page(p, blockIdx.y, blockIdx.x);     // no kernel writes what this reads
   pdl_wait_release();
-  const int page = unpack_page(p, blockIdx.y, blockIdx.x);
   if (page < 0) return;
   const int is_v = (int)blockIdx.z >= parts;
   const int first = ((int)blockIdx.z - (is_v ? parts : 0)) * (UP_THREADS * UP_EACH) + (int)threadIdx.x;
