@@ -36,6 +36,8 @@ constexpr int D8_MAX_STAGES = 24;                 // a multiple of the warps (se
 constexpr int D8_CHUNK = 128;                     // pages looked up at a time
 constexpr int D8_BLOCK_SMEM = 113 * 1024;         // of an SM's 228 KB: two blocks with 1 KB each of the system's
 constexpr int D8_HEADS = 8;                       // query heads of a pair (the MMA's N); larger groups are several pairs
+constexpr long long D8_BRIEF = 768 * 1024;        // bytes of a block's codes below which ...
+constexpr long long D8_BRIEF_FLIGHT = 49152;      // ... so many of them are in flight
 constexpr int D8_ROW = 128;                       // bytes of a swizzled row
 constexpr int D8_MAX_TOKENS = 1024;               // of a launch
 constexpr float D8_P_BASE = 64.f;                 // probabilities are multiplied by this before they become halves
@@ -749,10 +751,6 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
   if (rc == GLINT_OK) rc = d8_map(&map_v, v_pool, rows, hd, page_size, whole_page);
   if (rc != GLINT_OK) return rc;
   const long long page_bytes = page_size * row_bytes;
-  int stages = (int)((D8_BLOCK_SMEM - fixed) / (2 * page_bytes * D8_WARPS)) * D8_WARPS;
-  if (stages > D8_MAX_STAGES) stages = D8_MAX_STAGES;
-  if (stages < D8_WARPS) stages = D8_WARPS;
-  const long long smem = stages * 2 * page_bytes + fixed;
   // what a pair costs a block beside its pages, and the least a block is given, in pages of this size
   const long long unit = 2ll * page_size * hd;
   const int pair_cost = (int)((96 * 1024 + unit / 2) / unit) + 1;
@@ -769,6 +767,16 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
   if (fits < 1) return GLINT_ERR_UNSUPPORTED_SIZE;
   int step = arrive_ints / pairs < D8_MAX_TOKENS ? arrive_ints / pairs : D8_MAX_TOKENS;
   if (fits < step) step = (int)fits;
+  if (step > T) step = T;
+  // Shared memory for copies in flight: all of it for launches that stream long, 48 KB where a block has less than 768 KB to
+  // read; the kernels on either side then find room beside it.  16 requests of 2,000 keys (16 heads in 8 groups of 256, 444 KB
+  // a block) take 35.2 us with 48 KB and 36.8 with 96, 32 of them (886 KB) 57.8 and 56.3; a decode step of the 9B sizes
+  // (21 layers) at one request 2.27 and 2.35 ms, at 32 requests 3.66 and 3.58.
+  const bool brief = step * pairs * most_pages * unit < blocks * D8_BRIEF;
+  int stages = (int)((brief ? (D8_BRIEF_FLIGHT < D8_BLOCK_SMEM - fixed ? D8_BRIEF_FLIGHT : D8_BLOCK_SMEM - fixed) : D8_BLOCK_SMEM - fixed) / (2 * page_bytes * D8_WARPS)) * D8_WARPS;
+  if (stages > D8_MAX_STAGES) stages = D8_MAX_STAGES;
+  if (stages < D8_WARPS) stages = D8_WARPS;
+  const long long smem = stages * 2 * page_bytes + fixed;
   for (int t0 = 0; t0 < T; t0 += step) {
     const int n = T - t0 < step ? T - t0 : step;
     Decode8Params p = {(const __nv_bfloat16*)q + (size_t)t0 * nh * hd, positions + t0, token_seq + t0, block_table, k_scale, v_scale,
