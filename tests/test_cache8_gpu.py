@@ -89,6 +89,13 @@ APPENDS = [  # lens, starts, nh, nkv, hd, page, pairs, interleaved, amplitude
     ([9], [0], 2, 1, 6, 3, 1, True, 1.0),                   # odd pages, one pair of three turned
     ([5, 6], [2, 0], 2, 2, 64, 16, 0, False, 1.0),          # nothing turned
     ([300], [250], 4, 2, 256, 256, 128, False, 1.0),        # pages of 256
+    ([40, 1], [5, 7], 6, 2, 128, 16, 32, True, 1.2),        # heads of 64, 128 and 256, all or some of them turned
+    ([20, 1], [5, 14], 2, 1, 128, 16, 24, False, 0.9),
+    ([1, 30], [9, 3], 4, 2, 256, 16, 32, False, 1.0),
+    ([30], [3], 4, 2, 256, 32, 33, False, 1.0),
+    ([30], [3], 5, 1, 256, 16, 128, True, 1.0),
+    ([30], [30], 3, 1, 64, 16, 7, True, 1.0),
+    ([30], [30], 3, 1, 256, 16, 0, False, 1.0),
 ]
 
 
