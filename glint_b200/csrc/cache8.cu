@@ -74,6 +74,11 @@ __device__ __forceinline__ float2 rope_angle(int pos, double turns, float amplit
 // largest magnitude of a run, and with it the page's new scale, is found in one block whatever the windows cut: a warp
 // per token, values kept in registers (two tokens a warp) between the maximum and the codes.  Query blocks: a warp
 // rotates four heads of a token with one set of sines and cosines.
+// Measured, 2,048 tokens of 8 heads in 4 groups of 256 with the widening behind it (34 MB of float read, 4 MB of codes and 8 MB
+// of queries written; 11.3 + 4.2 us) / a mixed step of 997 tokens, 32 heads in 16 groups of 128: 16.6 / 22.9 us; two or eight
+// heads a warp 17.4 / 24.6 and 23.1 / 23.9; one or four tokens held 18.0 / 24.2 and 17.4 / 23.6; room for three, five or
+// six blocks an SM instead of four 18.5 / 22.8, 17.8 / 21.4 and 20.7 / 21.9, so that heads of 256 take four, smaller ones five.
+// One token takes 2.4 us behind a kernel that it can begin under.
 constexpr int AP_WARPS = 8;
 constexpr int AP_WINDOW = 16;                     // tokens
 constexpr int AP_HELD = 2;                        // tokens of a warp whose values stay in registers
@@ -228,7 +233,7 @@ struct RopeLane {
 };
 
 template <typename S, int NP, bool FULL>
-__global__ void __launch_bounds__(AP_WARPS * 32, 4) rope_append_kernel(const AppendParams p, int cache_blocks) {
+__global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_kernel(const AppendParams p, int cache_blocks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int width = (p.nh + 2 * p.nkv) * p.hd, pairs = p.hd >> 1;
   const RopeLane<NP, FULL> mine = {lane, p.rot >> 1, pairs, p.rot, p.interleaved};
@@ -570,11 +575,12 @@ __device__ __forceinline__ void store16(float* to, const float4 (&v)[4]) {
   for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(to)[i] = v[i];
 }
 
-// Memory-bound: a byte read and two written per element.  Grid (pages of the longest range, requests, parts of 8192
+// Memory-bound: a byte read and two written per element (8,150 keys of 8 heads of 256, 100 MB: 16.9 us = 5.9 TB/s, the part of
+// it that stays in L2 included; 4,096 keys 10.5 us, of which 3 are the launch's start and end).  Grid (pages of the longest range, requests, parts of 8192
 // elements of a page's keys, then of its values): a page's heads lie one behind the other, a thread takes 16 codes at a
 // time of one of them (a page of a head is a multiple of 16 elements).
-constexpr int UP_THREADS = 256;
-constexpr int UP_EACH = 2;                        // sixteens of a thread
+constexpr int UP_THREADS = 256;                   // 128: a mixed step 8.1 instead of 6.4 us; 512: 2,282 tokens 13.7 instead of 13.0
+constexpr int UP_EACH = 2;                        // sixteens of a thread; 1: 16.5 instead of 13.0, 4: 15.0
 
 template <typename S>
 __global__ void __launch_bounds__(UP_THREADS) cache8_unpack_kernel(const UnpackParams p, int parts) {
