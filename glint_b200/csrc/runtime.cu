@@ -82,13 +82,14 @@ bool tiled_attention_supported(int nh, int nkv, int hd, int page) {
 }
 // Tokens of portions over coded pages that take the single-token kernel all the same.  It reads the codes again for every
 // token, a (token, kv head) pair costs it about 96 KB beside them, but it needs no wide pages and spreads over all SMs: bytes
-// that count as much as 32 MB and seven readings of the longest context.  Measured on both sides of that (us, this kernel
-// against wide pages and the tiled one), 8 heads in 4 groups of 256: 8 tokens at 2,000 keys 15.4 / 17.9, 32 at 2,000 26 / 19,
-// 8 at 8,000 25.7 / 31, 16 at 8,000 40 / 32; 32 heads in 16 groups of 128: 8 at 500 12.8 / 16.1, 32 at 500 22.7 / 18.8.
-// Below 256 keys the tiled kernel's one or two tiles are as fast (64 tokens at 100 keys 17 / 12).
+// that count as much as 43 MB and seven readings of the longest context.  Measured on both sides of that (us, this kernel
+// against wide pages and the tiled one), 8 heads in 4 groups of 256: 16 tokens at 2,000 keys 16.8 / 18.0, 32 at 2,000 24.8 /
+// 18.3, 8 at 8,000 24.2 / 31.4, 16 at 8,000 37.9 / 31.9; 32 heads in 16 groups of 128: 16 at 500 14.7 / 17.7, 32 at 500 21.1 /
+// 17.5, 8 at 8,000 47.1 / 44.3.  Below 256 keys the tiled kernel's few tiles are as fast or faster: 32 tokens at 100 keys 12.1 /
+// 11.3 and 12.1 / 10.4.
 bool few_tokens(long long tokens, int reach, int nkv, int hd) {
   const long long context = (long long)reach * nkv * hd * 2;
-  return reach > 256 && tokens * (context + nkv * (96ll << 10)) <= (32ll << 20) + 7 * context;
+  return reach > 256 && tokens * (context + nkv * (96ll << 10)) <= (43ll << 20) + 7 * context;
 }
 constexpr int SPLIT_SINGLES_FROM = 4096;   // context from which single tokens in front of portions leave the tiled kernel
 constexpr int SPLIT_SINGLES_UP_TO = 8;     // so few of them leave it at any context
