@@ -78,6 +78,7 @@ class Cache8:
                                         self.v_wide.data_ptr(), partials.data_ptr(), partials.numel(), arrive.data_ptr(),
                                         arrive.numel())
         self.addr, self.dtype, self.device_index = ctypes.addressof(self.struct), self.k_wide.dtype, self.k.get_device()
+        self.device = self.k.device
 
     @classmethod
     def empty(cls, num_pages, num_kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda:0"):
@@ -186,11 +187,11 @@ def append(rt, cache, step, qkv, turns, num_heads, q_out=None, layout="half", am
     T, hd, index = step.num_tokens, cache.hd, rt.device_index
     _rows(qkv, T, (num_heads + 2 * cache.nkv) * hd, torch.float32, "qkv", index)
     pairs = turns.numel()
-    if turns.dtype is not torch.float64 or turns.get_device() != index or turns.dim() != 1 or 2 * pairs > hd:
+    if turns.dtype is not torch.float64 or turns.get_device() != index or turns.dim() != 1 or 2 * pairs > hd or not turns.is_contiguous():
         ops.require(turns, torch.float64, "turns")
         raise KernelError(f"turns {tuple(turns.shape)} on device {turns.get_device()} do not fit heads of {hd} on device {index}")
     if q_out is None:
-        q_out = qkv.new_empty((T, num_heads * hd), dtype=rt.dtype)
+        q_out = torch.empty_strided((T, num_heads * hd), (num_heads * hd, 1), dtype=rt.dtype, device=cache.device)   # the cheapest
     else:
         _rows(q_out, T, num_heads * hd, rt.dtype, "q_out", index)
     _call(rt, "cache8 append", _lib().glint_op_rope_append_with, ctypes.addressof(rt.native), step.addr, qkv.data_ptr(),

@@ -145,6 +145,7 @@ def test_call_refusals(monkeypatch):
                            ((qkv[:, :-32].contiguous(), turns, 4), {}, "qkv"), ((qkv[:2], turns, 4), {}, "qkv"),
                            ((qkv.double(), turns, 4), {}, "float32"), ((qkv, turns.float(), 4), {}, "float64"),
                            ((qkv, torch.zeros(17, dtype=torch.float64), 4), {}, "turns"),
+                           ((qkv, torch.zeros(32, dtype=torch.float64)[::2], 4), {}, "contiguous"),
                            ((qkv, turns, 4), dict(layout="pairs"), "layout"), ((qkv, turns, 4), dict(q_out=q.float()), "q_out"),
                            ((qkv, turns, 4), dict(q_out=q[:2]), "q_out")]:
         with pytest.raises(KernelError, match=what):
