@@ -69,7 +69,7 @@ class Setup:
 def _qkv(T, nh, nkv, hd, seed, spread=1.0):
     g = torch.Generator().manual_seed(seed)
     x = torch.randn(T, nh + 2 * nkv, hd, generator=g) * torch.exp(spread * torch.randn(T, nh + 2 * nkv, 1, generator=g))
-    return x.reshape(T, -1).contiguous()
+    return x.reshape(T, (nh + 2 * nkv) * hd).contiguous()
 
 
 def _turns(pairs, theta=10000.0):
@@ -355,6 +355,14 @@ ATTENDS = [  # lens, starts, nh, nkv, hd, page, window, cap
     ([100, 40], [2000, 1000], 6, 2, 128, 16, 0, 0.0),
     ([150, 3], [1700, 1200], 2, 1, 256, 64, 900, 0.0),            # ... through a window
     ([90] + [2] * 40, [2600] + [700 + i for i in range(40)], 10, 2, 48, 16, 0, 30.0),
+    ([70, 3], [100, 7], 40, 1, 64, 16, 0, 50.0),                  # groups that do not divide 128, or fill it
+    ([20], [60], 128, 1, 32, 16, 0, 0.0),
+    ([80], [40], 4, 2, 16, 16, 0, 50.0),                          # head sizes between the usual ones
+    ([80], [140], 4, 2, 240, 64, 0, 50.0),
+    ([80], [140], 2, 1, 192, 32, 0, 0.0),
+    ([150, 1, 1], [30, 4, 200], 4, 2, 64, 16, 1, 0.0),            # a window of one
+    ([700], [1500], 34, 17, 48, 32, 0, 50.0),                     # a few blocks more than SMs
+    ([1100], [900], 16, 16, 128, 16, 0, 56.0),
 ]
 
 
@@ -425,6 +433,40 @@ def test_scores_that_all_reach_the_cap(rts, lens, starts, hd, cap, sign, e):
             assert err <= 0.012 * np.abs(v).max(), (i, head, err / np.abs(v).max())
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("lens,starts", [([0, 5, 0, 70, 1], [10, 3, 0, 20, 6]), ([1, 0, 0, 130], [400, 500, 0, 900]), ([1, 0, 1], [30, 9, 700]),
+                                         ([0, 0], [5, 0]), ([], [])])
+def test_requests_without_tokens_and_steps_without_requests(rts, dtype, lens, starts):
+    """Requests that bring no token of a step, and steps without any: the others as the definition has them (tolerances as
+    above)."""
+    from glint_b200 import ops_cache8
+    rt, nh, nkv, hd, P = rts[dtype], 4, 2, 64, 16
+    T = sum(lens)
+    if not lens:
+        i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=DEV)
+        cache = ops_cache8.Cache8.empty(2, nkv, P, hd, rt.dtype)
+        step = ops_cache8.StepArrays(i32(0), i32(0), i32(0), i32(1), i32(0, 2), 0, 0)
+    else:
+        s = Setup(rt, lens, starts, nkv, hd, P, seed=3)
+        cache, step = s.cache, s.step
+    q = (0.1 * torch.randn(T, nh * hd, generator=torch.Generator().manual_seed(1))).to(rt.dtype)
+    out = ops_cache8.attention(rt, cache, step, q.to(DEV), nh, 0.125, softcap=30.0)
+    ops_cache8.unpack(rt, cache, step)
+    rt.check_status()
+    assert out.shape == q.shape
+    got, qd = (t.double().cpu().numpy().reshape(-1, nh, hd) for t in (out, q))
+    for r, (n, start) in enumerate(zip(lens, starts)):
+        for i in sorted({0, n - 1}) if n else ():
+            for head in range(nh):
+                k, v = s.values(0, r, head // 2), s.values(1, r, head // 2)
+                want = plain.attend(qd[s.cu[r] + i, head], k, v, 0.125, 30.0, 0, start + i + 1)
+                bound = (2e-4 if dtype == "float32" else 0.012) * np.abs(v[:start + i + 1]).max()
+                assert np.abs(got[s.cu[r] + i, head] - want).max() <= bound, (r, i, head)
+    q2 = ops_cache8.append(rt, cache, step, _qkv(T, nh, nkv, hd, 1).to(DEV), _turns(32).to(DEV), nh)
+    rt.check_status()
+    assert q2.shape == q.shape
+
+
 @pytest.mark.parametrize("case", [2, 4, 8, 14])
 def test_attention_repeats_itself(rts, case):
     _, _, a = _attention_case(rts, "bfloat16", case)
@@ -462,6 +504,64 @@ def test_attention_over_pages_of_very_different_scales(rts):
                 err = np.abs(got.double().cpu().numpy()[0, head * hd:(head + 1) * hd] - want).max()
                 # rounding of the probabilities and of the result, as above; the large page's weight is e^-60 or less
                 assert err <= 0.012 * np.abs(want).max(), (big_page, gap, head, err)
+
+
+@pytest.mark.parametrize("lens,starts,cap", [([90], [40], 50.0), ([90], [40], 0.0), ([130], [1500], 0.0), ([1] * 4, [40, 700, 3, 90], 50.0)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_not_finite_reaches_its_own_row_only(rts, lens, starts, cap, bad):
+    """Bit for bit: the other heads and tokens are what they are without it; its own row is not a number (infinity times codes
+    of both signs is none either)."""
+    from glint_b200 import ops_cache8
+    rt, nh, nkv, hd = rts["bfloat16"], 4, 2, 64
+    s = Setup(rt, lens, starts, nkv, hd, 16, seed=2)
+    q = (0.1 * torch.randn(sum(lens), nh * hd, generator=torch.Generator().manual_seed(1))).to(DEV, torch.bfloat16)
+    want = ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.125, softcap=cap).view(-1, nh, hd)
+    t, head = min(2, sum(lens) - 1), 1
+    q.view(-1, nh, hd)[t, head, 5:7] = bad
+    got = ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.125, softcap=cap).view(-1, nh, hd)
+    rt.check_status()
+    assert got[t, head].isnan().all()
+    got[t, head] = want[t, head]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("cap", [50.0, 0.0])
+def test_portions_replayed_from_a_graph(rts, cap):
+    """Append and attention of portions captured once for contexts of up to 2,000 tokens and replayed at others."""
+    from glint_b200 import ops_cache8
+    rt, nh, nkv, hd, P, lens = rts["bfloat16"], 4, 2, 128, 16, [70, 33]
+    turns = _turns(hd // 2).to(DEV)
+    s = Setup(rt, lens, [1900, 1800], nkv, hd, P, seed=6)
+    qkv = _qkv(sum(lens), nh, nkv, hd, 1).to(DEV)
+    names = ("k", "v", "k_scale", "v_scale")
+    fresh = [getattr(s.cache, m).clone() for m in names]
+    t = s.step.tensors
+
+    def once():
+        q = ops_cache8.append(rt, s.cache, s.step, qkv, turns, nh)
+        return ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.1, softcap=cap)
+
+    def reset(starts, seed):
+        t["positions"].copy_(torch.cat([torch.arange(a, a + n, dtype=torch.int32) for a, n in zip(starts, lens)]))
+        t["seq_start"].copy_(torch.tensor(starts, dtype=torch.int32))
+        qkv.copy_(_qkv(sum(lens), nh, nkv, hd, seed))
+        for m, f in zip(names, fresh):
+            getattr(s.cache, m).copy_(f)
+        s.step.begin()
+    once()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for starts, seed in (([1900, 1800], 2), ([0, 5], 3), ([700, 1799], 4)):
+        reset(starts, seed)
+        graph.replay()
+        replayed = [out.clone()] + [getattr(s.cache, m).clone() for m in names]
+        reset(starts, seed)
+        eager = [once()] + [getattr(s.cache, m) for m in names]
+        for a, b in zip(replayed, eager):
+            assert torch.equal(a, b)
+    rt.check_status()
 
 
 def test_more_single_tokens_than_a_launch_takes(rts):
