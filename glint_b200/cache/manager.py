@@ -115,6 +115,10 @@ class CodedKVNeed(PagedKVNeed):
     attention of prompt portions reads, and scratch for single tokens (all layers take turns: a step's kernels run
     in order on one stream)."""
 
+    def __post_init__(self):
+        if self.head_dim % 2:
+            raise GlintError(f"a cache in 8 bits takes even head sizes, not {self.head_dim}")
+
     def group_key(self):
         return ("coded",) + super().group_key()
 

@@ -60,6 +60,12 @@ def test_declaration_and_accounting():
         CacheManager([wide, a], [None, 0], 2, 6, 16, 64, torch.bfloat16, "cpu")
 
 
+def test_odd_heads_are_refused_when_declared():
+    PagedKVNeed(4, 33, None)
+    with pytest.raises(GlintError, match="even"):
+        CodedKVNeed(4, 33, None)
+
+
 def test_cache_dtype_names():
     from glint_b200.runtime import parse_cache_dtype
     assert parse_cache_dtype(None) is None and parse_cache_dtype("auto") is None and parse_cache_dtype("int8") == "int8"
