@@ -43,7 +43,7 @@ constexpr int D8_CHUNK = 128;                     // pages looked up at a time
 constexpr int D8_BLOCK_SMEM = 113 * 1024;         // of an SM's 228 KB: two blocks with 1 KB each of the system's
 constexpr int D8_HEADS = 8;                       // query heads of a pair (the MMA's N); larger groups are several pairs
 constexpr long long D8_BRIEF = 768 * 1024;        // bytes of a block's codes below which ...
-constexpr long long D8_BRIEF_FLIGHT = 49152;      // ... so many of them are in flight
+constexpr long long D8_BRIEF_FLIGHT = 48 * 1024;  // ... so many of them are in flight
 constexpr int D8_ROW = 128;                       // bytes of a swizzled row
 constexpr int D8_MAX_TOKENS = 1024;               // of a launch
 constexpr float D8_P_BASE = 64.f;                 // probabilities are multiplied by this before they become halves
@@ -783,7 +783,9 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
   // a block) take 35.2 us with 48 KB and 36.8 with 96, 32 of them (886 KB) 57.8 and 56.3; a decode step of the 9B sizes
   // (21 layers) at one request 2.27 and 2.35 ms, at 32 requests 3.66 and 3.58.
   const bool brief = step * pairs * most_pages * unit < blocks * D8_BRIEF;
-  int stages = (int)((brief ? (D8_BRIEF_FLIGHT < D8_BLOCK_SMEM - fixed ? D8_BRIEF_FLIGHT : D8_BLOCK_SMEM - fixed) : D8_BLOCK_SMEM - fixed) / (2 * page_bytes * D8_WARPS)) * D8_WARPS;
+  long long flight = D8_BLOCK_SMEM - fixed;
+  if (brief && flight > D8_BRIEF_FLIGHT) flight = D8_BRIEF_FLIGHT;
+  int stages = (int)(flight / (2 * page_bytes * D8_WARPS)) * D8_WARPS;
   if (stages > D8_MAX_STAGES) stages = D8_MAX_STAGES;
   if (stages < D8_WARPS) stages = D8_WARPS;
   const long long smem = stages * 2 * page_bytes + fixed;

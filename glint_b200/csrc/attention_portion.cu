@@ -23,8 +23,8 @@
 // large product reaches; the tensor pipe is busy 54 % of the time and the special-function unit 55 %.  Neither binds alone:
 // what is left is the hand-over between the warps of a tile.
 // Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx; keys of a token at position p from
-// max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the second product, and their sum
-// is that of the rounded ones.
+// max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the
+// second product, and their sum is that of the rounded ones.
 #include "common.cuh"
 #include "tcgen05.cuh"
 

@@ -131,7 +131,8 @@ __device__ __forceinline__ void store_values(__nv_bfloat16* to, const float* fro
   } else if constexpr (N == 4) {
     *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(from[0], from[1]), pack_bf16(from[2], from[3]));
   } else {
-    *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(from[0], from[1]), pack_bf16(from[2], from[3]), pack_bf16(from[4], from[5]), pack_bf16(from[6], from[7]));
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(from[0], from[1]), pack_bf16(from[2], from[3]), pack_bf16(from[4], from[5]),
+                                              pack_bf16(from[6], from[7]));
   }
 }
 template <int N>
@@ -576,9 +577,9 @@ __device__ __forceinline__ void store16(float* to, const float4 (&v)[4]) {
 }
 
 // Memory-bound: a byte read and two written per element (8,150 keys of 8 heads of 256, 100 MB: 16.9 us = 5.9 TB/s, the part of
-// it that stays in L2 included; 4,096 keys 10.5 us, of which 3 are the launch's start and end).  Grid (pages of the longest range, requests, parts of 8192
-// elements of a page's keys, then of its values): a page's heads lie one behind the other, a thread takes 16 codes at a
-// time of one of them (a page of a head is a multiple of 16 elements).
+// it that stays in L2 included; 4,096 keys 10.5 us, of which 3 are the launch's start and end).  Grid (pages of the longest range,
+// requests, parts of 8192 elements of a page's keys, then of its values): a page's heads lie one behind the other, a thread
+// takes 16 codes at a time of one of them (a page of a head is a multiple of 16 elements).
 constexpr int UP_THREADS = 256;                   // 128: a mixed step 8.1 instead of 6.4 us; 512: 2,282 tokens 13.7 instead of 13.0
 constexpr int UP_EACH = 2;                        // sixteens of a thread; 1: 16.5 instead of 13.0, 4: 15.0
 
@@ -608,8 +609,8 @@ __global__ void __launch_bounds__(UP_THREADS) cache8_unpack_kernel(const UnpackP
   }
 }
 
-// Any size, element by element.  Grid (pages of the longest request, kv heads, requests): the pages that the request's new tokens can reach, each to
-// its own place in the wide pools.
+// Any size, element by element.  Grid (pages of the longest request, kv heads, requests): the pages that the request's new
+// tokens can reach, each to its own place in the wide pools.
 template <typename S>
 __global__ void __launch_bounds__(256) cache8_unpack_simple_kernel(const UnpackParams p) {
   pdl_wait_release();
