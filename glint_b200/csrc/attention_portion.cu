@@ -7,7 +7,10 @@
 // never pauses.  So nothing waits that need not:
 //   warps 0, 3 TMA: the query tile once and key tiles; value tiles: page by page into rings as deep as shared memory allows
 //              (head size 256: three tiles of keys, two of values)
-//   warp 1     tcgen05.mma: S = Q K^T into one of two score buffers of tensor memory, as soon as that has been read
+//   warp 1     tcgen05.mma: S = Q K^T into one of two score buffers of tensor memory, as soon as that has been read.  With
+//              64 keys a tile, products from shared memory alone read Q again for every tile (head size 256: 64 KB beside 64
+//              of K and V read and 64 written, 1,536 cycles of shared memory, about the tile's time), so the first 128 dims
+//              of Q lie in tensor memory where there is room (4,096 tokens 136.6 -> 133.6 us)
 //   warp 2     tcgen05.mma: O += P V, P (bfloat16 pairs) from one of two buffers of tensor memory
 //   warps 4-7  softmax of the even tiles, warps 8-11 of the odd ones, one thread per row: no maximum or sum is exchanged
 //              within a tile, and one group computes while the other loads, stores and waits
@@ -19,8 +22,8 @@
 // Where SMs would stay empty (fewer blocks than SMs, or a few blocks behind the last full round of them) the keys of a tile of
 // rows are split over several blocks, whose partial results a second kernel adds up in order.
 // Blocks are found from the portions' lengths, so that short portions beside long ones cost no empty blocks.
-// 4,096 tokens, 16 heads in 8 groups of 256: 137 GFLOP in 127 us (and 10 for the wide pages) = 1.08 PFLOP/s, 0.66 of what a
-// large product reaches; the tensor pipe is busy 54 % of the time and the special-function unit 55 %.  Neither binds alone:
+// 4,096 tokens, 16 heads in 8 groups of 256: 137 GFLOP in 123 us (and 10 for the wide pages) = 1.11 PFLOP/s, 0.68 of what a
+// large product reaches (call after call 144 us: the power cap); tensor pipe and special-function unit are busy 55 % of the time.  Neither binds alone:
 // what is left is the hand-over between the warps of a tile.
 // Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx; keys of a token at position p from
 // max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the
@@ -57,7 +60,7 @@ struct PortionParams {
 };
 
 struct PortionShared {
-  uint64_t q_full, o_full;
+  uint64_t q_full, o_full, q_ready;
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], turn[2];
   uint64_t k_full[AT_STAGES], k_empty[AT_STAGES], v_full[AT_STAGES], v_empty[AT_STAGES];
   uint32_t tmem_base;
@@ -137,7 +140,7 @@ __device__ __forceinline__ PortionKeys portion_keys(const PortionParams& p, cons
   return k;
 }
 
-// FIXED: the soft cap spares the running maximum (4,096 tokens, 16 heads in 8 groups of 256: 137 us, 187 without; 2,282 ragged
+// FIXED: the soft cap spares the running maximum (4,096 tokens, 16 heads in 8 groups of 256: 134 us, 187 without; 2,282 ragged
 // ones, 32 heads in 16 groups of 128: 92 and 179, where the columns that do not fit the registers are computed twice).
 // PAIR: two blocks on an SM (head sizes up to 128): each has half of the tensor memory, so that P is written over the scores
 // it came from and the scores two tiles on wait for the product that reads it; one block's beginning and end pass under the
@@ -162,7 +165,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // a barrier per thread; arrivals of a group's rows where threads arrive, of one thread or copy elsewhere
     uint64_t* const single[] = {&sh->q_full, &sh->o_full, sh->s_full, sh->pv_done, sh->k_full, sh->k_empty, sh->v_full, sh->v_empty};
     const int many[] = {1, 1, 2, 2, AT_STAGES, AT_STAGES, AT_STAGES, AT_STAGES};
-    uint64_t* const rows[] = {sh->s_free, sh->p_ready, sh->turn};
+    uint64_t* const rows[] = {sh->s_free, sh->p_ready, sh->turn, &sh->q_ready};
+    const int rows_many[] = {2, 2, 2, 1};
     int i = threadIdx.x;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -170,9 +174,9 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       i -= many[k];
     }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      if (i >= 0 && i < 2) tc::mbar_init(rows[k] + i, AT_M);
-      i -= 2;
+    for (int k = 0; k < 4; ++k) {
+      if (i >= 0 && i < rows_many[k]) tc::mbar_init(rows[k] + i, AT_M);
+      i -= rows_many[k];
     }
     if (i == 0) sh->abort_flag = 0;
     if (threadIdx.x < 32) tc::fence_barrier_init();
@@ -221,6 +225,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   // two of P as bfloat16 pairs, 32 columns each; O, up to 256 columns (PAIR: 128)
   const uint32_t tmem_p = PAIR ? tmem_s : tmem_s + 2 * AT_N, p_step = PAIR ? AT_N : AT_N / 2;
   const uint32_t tmem_o = tmem_s + (PAIR ? 2 * AT_N : 3 * AT_N);
+  const uint32_t tmem_q = tmem_s + 448;                  // not PAIR: the first 128 dims of the queries
   volatile int* abort_flag = &sh->abort_flag;
 
   if (warp == 0 || warp == 3) {
@@ -306,6 +311,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const uint64_t kd0 = tc::smem_desc_k_sw128_sbo(tc::smem_u32(sk), k_sbo);
       const uint32_t k_tile = ((uint32_t)nsub * AT_KV_SUB) >> 4;
       bool ok = tc::mbar_wait(&sh->q_full, 0, abort_flag);
+      if (!PAIR && ok) ok = tc::mbar_wait(&sh->q_ready, 0, abort_flag);
       for (int j = 0, stage = 0, phase = 0; j < n_tiles && ok; ++j) {
         const int b = j & 1;
         ok = tc::mbar_wait(&sh->k_full[stage], phase, abort_flag);
@@ -319,7 +325,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           if (ks < hd16) {
             const uint32_t oq = ((ks >> 2) * AT_Q_SUB + (ks & 3) * 32) >> 4;
             const uint32_t ok_ = ((ks >> 2) * k_slice + (ks & 3) * 32) >> 4;
-            tc::mma_bf16_ss(d, qd + oq, kd + ok_, idesc, ks > 0 ? 1u : 0u);
+            if (!PAIR && ks < 8) tc::mma_bf16_ts(d, tmem_q + 8 * ks, kd + ok_, idesc, ks > 0 ? 1u : 0u);
+            else tc::mma_bf16_ss(d, qd + oq, kd + ok_, idesc, ks > 0 ? 1u : 0u);
           }
         }
         tc::mma_commit(&sh->s_full[b]);
@@ -378,8 +385,27 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const float out_scale = p.cap > 0.f ? p.cap * LOG2E : LOG2E;   // scores are kept in log2 units
     float ref = -INFINITY, l = 0.f;
     bool ok = true;                                      // the same in all lanes of a warp
+    if (!PAIR && group == 0) {                           // the queries' first 128 dims, as pairs, into tensor memory
+      ok = warp_wait(&sh->q_full, 0, abort_flag);
+      if (ok) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int chunk = (c & 1) * 4 + i;
+            const uint4 x = *reinterpret_cast<const uint4*>(sq + (size_t)(c >> 1) * AT_Q_SUB + r * 128 + ((chunk ^ (r & 7)) << 4));
+            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+          }
+          tc::tmem_st_16(tmem_q + lane_base + 16 * c, v);
+        }
+        tc::tmem_st_wait();
+        tc::fence_before_thread_sync();
+        tc::mbar_arrive(&sh->q_ready);
+      }
+    }
     constexpr int CH = PAIR ? 32 : AT_N;                 // columns in registers at a time
-    for (int j = group; j < n_tiles; j += 2) {
+    for (int j = group; j < n_tiles && ok; j += 2) {
       ok = warp_wait(&sh->s_full[group], (j >> 1) & 1, abort_flag);
       if (!ok) break;
       tc::fence_after_thread_sync();
