@@ -24,6 +24,8 @@ from .errors import KernelError
 
 LAYOUTS = {"half": False, "interleaved": True}
 
+_F32, _F64 = torch.float32, torch.float64
+
 _routed = None
 
 
@@ -158,20 +160,24 @@ def _rows(t, rows, width, dtype, name, index):
     raise KernelError(f"{name} belongs to device {t.get_device()}, the runtime to {index}")
 
 
+_current_device = ops._raw_device or torch.cuda.current_device
+_current_stream = ops._raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(rt, what, fn, *args):
     """One routed operation on the current stream of the runtime's device."""
-    if torch._C._cuda_getDevice() == rt.device_index:
-        rc = fn(*args, ops.stream())
+    index = rt.device_index
+    if _current_device() == index:
+        rc = fn(*args, _current_stream(index))
     else:
-        with torch.cuda.device(rt.device_index):
-            rc = fn(*args, ops.stream())
+        with torch.cuda.device(index):
+            rc = fn(*args, _current_stream(index))
     if rc != 0:
         raise KernelError(f"{what}: {ops.error_string(rc)} (code {rc})")
 
 
 def _heads(num_heads, cache):
-    if num_heads < 1 or num_heads % cache.nkv:
-        raise KernelError(f"{num_heads} query heads do not share {cache.nkv} kv heads evenly")
+    raise KernelError(f"{num_heads} query heads do not share {cache.nkv} kv heads evenly")
 
 
 def append(rt, cache, step, qkv, turns, num_heads, q_out=None, layout="half", amplitude=1.0):
@@ -181,21 +187,24 @@ def append(rt, cache, step, qkv, turns, num_heads, q_out=None, layout="half", am
     paired (j, j + pairs) in the layout "half" and (2j, 2j + 1) in the layout "interleaved"; the angles are computed
     in 64 bits.  ``amplitude`` scales the turned dims.  A key or value that is not finite makes its page's scale NaN."""
     _check(rt, cache, step)
-    _heads(num_heads, cache)
+    if num_heads < 1 or num_heads % cache.nkv:
+        _heads(num_heads, cache)
     interleaved = LAYOUTS.get(layout)
     if interleaved is None:
         raise KernelError(f"rotary layout {layout!r} is none of {sorted(LAYOUTS)}")
     T, hd, index = step.num_tokens, cache.hd, rt.device_index
-    _rows(qkv, T, (num_heads + 2 * cache.nkv) * hd, torch.float32, "qkv", index)
+    width = num_heads * hd
+    if qkv.dtype is not _F32 or qkv.get_device() != index or qkv.shape != (T, width + 2 * cache.nkv * hd) or not qkv.is_contiguous():
+        _rows(qkv, T, width + 2 * cache.nkv * hd, _F32, "qkv", index)
     pairs = turns.numel()
-    if turns.dtype is not torch.float64 or turns.get_device() != index or turns.dim() != 1 or 2 * pairs > hd or not turns.is_contiguous():
+    if turns.dtype is not _F64 or turns.get_device() != index or turns.dim() != 1 or 2 * pairs > hd or not turns.is_contiguous():
         ops.require(turns, torch.float64, "turns")
         raise KernelError(f"turns {tuple(turns.shape)} on device {turns.get_device()} do not fit heads of {hd} on device {index}")
     if q_out is None:
-        q_out = torch.empty_strided((T, num_heads * hd), (num_heads * hd, 1), dtype=rt.dtype, device=cache.device)   # the cheapest
+        q_out = torch.empty_strided((T, width), (width, 1), dtype=rt.dtype, device=cache.device)   # the cheapest
     else:
-        _rows(q_out, T, num_heads * hd, rt.dtype, "q_out", index)
-    _call(rt, "cache8 append", _lib().glint_op_rope_append_with, ctypes.addressof(rt.native), step.addr, qkv.data_ptr(),
+        _rows(q_out, T, width, rt.dtype, "q_out", index)
+    _call(rt, "cache8 append", (_routed or _lib()).glint_op_rope_append_with, rt.native_addr, step.addr, qkv.data_ptr(),
           q_out.data_ptr(), cache.addr, num_heads, cache.nkv, hd, turns.data_ptr(), 2 * pairs, interleaved, amplitude)
     return q_out
 
@@ -205,7 +214,7 @@ def unpack(rt, cache, step, window=0):
     places of the wide pools (returned); other places are left as they were."""
     window = window or 0
     _check(rt, cache, step, window)
-    _call(rt, "cache8 unpack", _lib().glint_op_cache8_unpack, ctypes.addressof(rt.native), step.addr, cache.addr, cache.nkv,
+    _call(rt, "cache8 unpack", (_routed or _lib()).glint_op_cache8_unpack, rt.native_addr, step.addr, cache.addr, cache.nkv,
           cache.hd, window)
     return cache.k_wide, cache.v_wide
 
@@ -216,13 +225,14 @@ def attention(rt, cache, step, q, num_heads, multiplier, softcap=0.0, window=0, 
     all).  Returns ``out`` [tokens, heads * head size]."""
     window = window or 0
     _check(rt, cache, step, window)
-    _heads(num_heads, cache)
+    if num_heads < 1 or num_heads % cache.nkv:
+        _heads(num_heads, cache)
     T, hd, index = step.num_tokens, cache.hd, rt.device_index
     _rows(q, T, num_heads * hd, rt.dtype, "q", index)
     if out is None:
         out = torch.empty_like(q)
     else:
         _rows(out, T, num_heads * hd, rt.dtype, "out", index)
-    _call(rt, "cache8 attention", _lib().glint_op_attention, ctypes.addressof(rt.native), step.addr, q.data_ptr(), cache.addr,
+    _call(rt, "cache8 attention", (_routed or _lib()).glint_op_attention, rt.native_addr, step.addr, q.data_ptr(), cache.addr,
           out.data_ptr(), num_heads, cache.nkv, hd, multiplier, softcap or 0.0, window)
     return out

@@ -1,6 +1,8 @@
 """The device, the dtype and the kernel choice that all parts of one model share."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import ops
@@ -58,6 +60,7 @@ class Runtime:
         self.shared = {}          # what several parts of a model share (a table of rotation angles), by key
         from . import native
         self.native = native.make_runtime_struct(self)     # the C++ side's view of this runtime
+        self.native_addr = ctypes.addressof(self.native)
         self._backing = {}        # (role, dtype) -> flat tensor
         self._views = {}          # (role, shape, dtype) -> view of the backing tensor
         self._retired = []        # outgrown backing tensors: captured launches may still point into them
