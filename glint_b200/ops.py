@@ -190,9 +190,14 @@ def rope_append(qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_
     pool = torch.uint8 if k_scale is not None else q_out.dtype
     require(k_pool, pool, "k_pool"); require(v_pool, pool, "v_pool")
     require(k_scale, torch.float32, "k_scale"); require(v_scale, torch.float32, "v_scale")
-    if qkv.shape[1] != (nh + 2 * nkv) * hd or 2 * turns.numel() > hd or q_out.numel() != T * nh * hd:
+    if (qkv.shape[1] != (nh + 2 * nkv) * hd or 2 * turns.numel() > hd or q_out.numel() != T * nh * hd
+            or positions.numel() != T or token_seq.numel() != T):
         raise KernelError(f"rope_append shapes do not fit: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)}, "
-                          f"{turns.numel()} pairs, heads {nh}/{nkv} x {hd}")
+                          f"{positions.numel()} positions, {turns.numel()} pairs, heads {nh}/{nkv} x {hd}")
+    if k_pool is not None and any(t.numel() != n for t, n in ((k_pool, num_pages * nkv * page_size * hd), (v_pool, k_pool.numel()))):
+        raise KernelError(f"pools {tuple(k_pool.shape)} and {tuple(v_pool.shape)} are not {num_pages} pages of {nkv} x {page_size} x {hd}")
+    if k_scale is not None and not k_scale.numel() == v_scale.numel() == num_pages * nkv:
+        raise KernelError(f"scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)} are not {num_pages} x {nkv}")
     check(core().glint_rope_append(ptr(qkv), ptr(positions), ptr(token_seq), ptr(block_table), block_table.shape[1],
                                    ptr(turns), 2 * turns.numel(), int(bool(interleaved)), amplitude, ptr(q_out),
                                    dtype_code(q_out.dtype), ptr(k_pool), ptr(v_pool), ptr(k_scale), ptr(v_scale), T, nh,

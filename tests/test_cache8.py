@@ -176,6 +176,20 @@ def test_call_refusals(monkeypatch):
 FREQ = 10000.0 ** (-np.arange(0, 64, 2) / 64.0)
 
 
+def test_single_operation_refusals(monkeypatch):
+    _pretend(monkeypatch)
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)
+    good = dict(qkv=torch.zeros(3, 8 * 32), positions=i32(3), token_seq=i32(3), block_table=i32((1, 3)), turns=torch.zeros(16, dtype=torch.float64),
+                q_out=torch.zeros(3, 4 * 32), k_pool=torch.zeros(3, 2, 16, 32, dtype=torch.uint8), v_pool=torch.zeros(3, 2, 16, 32, dtype=torch.uint8),
+                nh=4, nkv=2, hd=32, page_size=16, num_pages=3, status=None, k_scale=torch.zeros(3, 2), v_scale=torch.zeros(3, 2))
+    for name, bad, what in [("positions", i32(2), "fit"), ("token_seq", i32(4), "fit"), ("q_out", torch.zeros(2, 4 * 32), "fit"),
+                            ("turns", torch.zeros(17, dtype=torch.float64), "fit"), ("num_pages", 4, "pages"),
+                            ("v_pool", torch.zeros(2, 2, 16, 32, dtype=torch.uint8), "pages"), ("v_scale", torch.zeros(2, 2), "scales"),
+                            ("k_pool", torch.zeros(3, 2, 16, 32), "uint8")]:
+        with pytest.raises(KernelError, match=what):
+            ops_cache8.ops.rope_append(**dict(good, **{name: bad}))
+
+
 def test_bands_keep_the_fast_and_slow_the_slow():
     from glint_b200.parts.positions import scaled_frequencies
     got, amplitude = scaled_frequencies(FREQ, {"kind": "bands", "factor": 8.0, "original_context": 4096}, 10000.0, 64)
