@@ -410,8 +410,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ok) break;
       tc::fence_after_thread_sync();
       const int key0 = kv_begin + j * AT_N;
-      // most tiles lie wholly inside every row's range
-      const bool inside = __all_sync(0xffffffffu, rv && key0 >= lo && key0 + AT_N - 1 <= qpos);
+      // most tiles lie wholly inside every row's range (lanes without a row compute what nobody reads)
+      const bool inside = __all_sync(0xffffffffu, !rv || (key0 >= lo && key0 + AT_N - 1 <= qpos));
       uint32_t raw[CH];
       // scores of columns c0 .. c0 + CH - 1 in log2 units, masked; FIXED: less the fixed reference
       auto scores = [&](int c0) {
