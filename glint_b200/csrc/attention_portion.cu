@@ -140,11 +140,11 @@ __device__ __forceinline__ PortionKeys portion_keys(const PortionParams& p, cons
   return k;
 }
 
-// FIXED: the soft cap spares the running maximum (4,096 tokens, 16 heads in 8 groups of 256: 134 us, 187 without; 2,282 ragged
-// ones, 32 heads in 16 groups of 128: 92 and 179, where the columns that do not fit the registers are computed twice).
+// FIXED: the soft cap spares the running maximum (4,096 tokens, 16 heads in 8 groups of 256: 134 us, 211 without; 2,282 ragged
+// ones, 32 heads in 16 groups of 128: 90 and 174, where the columns that do not fit the registers are computed twice).
 // PAIR: two blocks on an SM (head sizes up to 128): each has half of the tensor memory, so that P is written over the scores
 // it came from and the scores two tiles on wait for the product that reads it; one block's beginning and end pass under the
-// other's tiles (the ragged portions 92 us, 107 with one block).
+// other's tiles (the ragged portions 90 us, 105 with one block).
 template <bool FIXED, bool PAIR>
 __global__ void __launch_bounds__(AT_THREADS, PAIR ? 2 : 1)
 attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -410,7 +410,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ok) break;
       tc::fence_after_thread_sync();
       const int key0 = kv_begin + j * AT_N;
-      // most tiles lie wholly inside every row's range (lanes without a row compute what nobody reads)
+      // Most tiles lie wholly inside every row's range.  Lanes without a row compute what nobody reads: asked for the mask in
+      // every tile, they made 250 tokens behind 7,900 take 67.3 us instead of 59.7.
       const bool inside = __all_sync(0xffffffffu, !rv || (key0 >= lo && key0 + AT_N - 1 <= qpos));
       uint32_t raw[CH];
       // scores of columns c0 .. c0 + CH - 1 in log2 units, masked; FIXED: less the fixed reference
@@ -731,8 +732,9 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   p.out = (__nv_bfloat16*)out; p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.num_pages = num_pages;
   p.multiplier = multiplier; p.cap = cap; p.window = window; p.whole = whole; p.status = status; p.n_seqs = n_seqs;
   const int nsub = (hd + 63) / 64;
-  // As many tiles ahead as fit, up to four: two of each do nearly as well (ragged portions, heads of 128: 93 against 92 us;
-  // 4,096 tokens, heads of 256, which have room for three of keys and two of values: no difference)
+  // As many tiles ahead as fit, up to four: two of each do nearly as well (ragged portions, heads of 128: 91 against 90 us;
+  // heads of 256, which have room for three of keys and two of values: 4,096 tokens 134.5 against 133.9, 250 behind 7,900 61.6
+  // against 59.8)
   auto bytes = [&](int k, int v) { return nsub * AT_Q_SUB + (k + v) * nsub * AT_KV_SUB + (int)sizeof(PortionShared); };
   const bool pair = hd <= 128;                           // two blocks on an SM
   p.k_stages = p.v_stages = AT_STAGES;

@@ -20,6 +20,14 @@ constexpr unsigned C8_NOT_FINITE = 0x7f800000u;   // |x| as bits: from here on i
 // exponent of the scale for a largest magnitude given as the bits of |x|
 __device__ __forceinline__ int c8_exponent(unsigned bits) { return max((int)(bits >> 23) - 133, C8_LOWEST); }
 __device__ __forceinline__ float c8_pow2(int e) { return __int_as_float((e + 127) << 23); }    // -126 <= e <= 127
+// Steps by which the 32-bit rotation can be off: 4 ulp (2^-22) of a pair of length 128 sqrt(2).  Keys nearer than that to a
+// border between codes are rotated again in 64 bits (one in 10,000), so that codes are those of the definition to the last
+// (2,048 tokens 16.6 -> 17.4 us; in 32 bits alone about one code in a million was the one beside it).
+constexpr float C8_NEAR = 4.5e-5f;
+__device__ __forceinline__ float c8_distance(float x, float inv) {
+  const float h = x * inv, magic = 12582912.f;           // 1.5 * 2^23: the nearest whole number
+  return fabsf(h - ((h + magic) - magic));
+}
 // floor(x / s) + 128.  The product is exact, but for the smallest numbers under the largest scales, where it may become
 // -0: the floor of any negative number is at most -1.
 __device__ __forceinline__ unsigned c8_code(float x, float inv) {
@@ -65,6 +73,28 @@ __device__ __forceinline__ float2 rope_angle(int pos, double turns, float amplit
   const float cs = (n & 1) ? s : c, sn = (n & 1) ? c : s;
   return make_float2((((n + 1) & 2) ? -cs : cs) * amplitude, ((n & 2) ? -sn : sn) * amplitude);
 }
+
+// The pair (a, b) turned, in 64 bits: Taylor polynomials to x^17 and x^16, which leave out less than 1e-15.
+__device__ __noinline__ double2 rope_exact(int pos, double turns, float amplitude, float a, float b) {
+  const double quarters = 4.0 * turns * (double)pos;
+  const double n = rint(quarters);
+  const double x = (quarters - n) * 1.5707963267948966, y = x * x;
+  double s = 0.0, c = 0.0, f = 1.0 / 355687428096000.0, g = 1.0 / 20922789888000.0;      // 1 / 17!, 1 / 16!
+#pragma unroll
+  for (int i = 17; i >= 3; i -= 2) {
+    s = fma(s, y, ((i >> 1) & 1) ? -f : f);
+    c = fma(c, y, ((i >> 1) & 1) ? -g : g);
+    f *= (double)(i * (i - 1));
+    g *= (double)((i - 1) * (i - 2));
+  }
+  s = fma(s * y, x, x);
+  c = fma(c, y, 1.0);
+  const int q = (int)((long long)n & 3);
+  const double cs = ((q + 1) & 2 ? -1.0 : 1.0) * (q & 1 ? s : c) * amplitude, sn = (q & 2 ? -1.0 : 1.0) * (q & 1 ? c : s) * amplitude;
+  return make_double2(a * cs - b * sn, a * sn + b * cs);
+}
+// The scale was found in 32 bits: in 64 a value may reach 128 s.
+__device__ __forceinline__ unsigned c8_code(double x, double inv) { return (unsigned)(max(-128, min(127, (int)floor(x * inv))) + 128); }
 
 // ---- heads of up to 256: a lane holds NP pairs of a head ------------------------------------------------------------
 //
@@ -167,6 +197,10 @@ struct RopeLane {
   // FULL, not interleaved: where the pairs' first and second dims begin (those that are not turned pair up as they like)
   __device__ __forceinline__ int first() const { return lane * NP < half ? lane * NP : lane * 2 * NP; }
   __device__ __forceinline__ int second() const { return lane * NP < half ? half + lane * NP : lane * 2 * NP + NP; }
+  __device__ __forceinline__ int2 dims(int k) const {
+    if (!FULL) return at(k);
+    return interleaved ? make_int2(2 * pair(k), 2 * pair(k) + 1) : make_int2(first() + k, second() + k);
+  }
   __device__ __forceinline__ int2 at(int k) const { return rope_pair(lane + 32 * k, rot, interleaved); }
   __device__ __forceinline__ void load(const float* row, float (&a)[NP], float (&b)[NP]) const {
     if constexpr (FULL) {
@@ -385,13 +419,14 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
     if (lane == 0) atomicMax(&tops[runs[i]], m);
   }
   __syncthreads();
-  auto store = [&](int i, const float (&x)[NP], const float (&y)[NP]) {
+  // returns the pairs whose codes have to be looked at again
+  auto store = [&](int i, const float (&x)[NP], const float (&y)[NP]) -> unsigned {
     const int s = runs[i], page = pages[s];
-    if (page < 0) return;
+    if (page < 0) return 0u;
     const size_t row = ((size_t)page * p.nkv + h) * p.page_size;
     if (!coded) {
       mine.store((S*)(is_v ? p.v_pool : p.k_pool) + (row + offs[i]) * p.hd, x, y);
-      return;
+      return 0u;
     }
     const unsigned m = tops[s], before = olds[s];
     const int off0 = offs[s];
@@ -423,29 +458,57 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
       cx[k] = finite ? c8_code(x[k], inv) : 128u;
       cy[k] = finite ? c8_code(y[k], inv) : 128u;
     }
+    unsigned near = 0;
+    if (!is_v && finite) {
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        if (fminf(c8_distance(x[k], inv), c8_distance(y[k], inv)) < C8_NEAR) near |= 1u << k;
+    }
     mine.store(dst, cx, cy);
+    return near;
   };
+  auto again = [&](int i, unsigned near) {
+    const int r = runs[i];
+    const float* row = src + (size_t)i * width;
+    uint8_t* dst = (uint8_t*)p.k_pool + (((size_t)pages[r] * p.nkv + h) * p.page_size + offs[i]) * p.hd;
+    const int e = max(c8_exponent(tops[r]), offs[r] > 0 ? (int)(olds[r] >> 23) - 127 : C8_LOWEST);
+    const double inv = (double)c8_pow2(-e);
+    for (; near; near &= near - 1) {
+      const int k = __ffs(near) - 1;
+      if (!mine.turned(k)) continue;
+      const int2 d = mine.dims(k);
+      const float a = row[d.x], b = row[d.y];
+      if (a == 0.f && b == 0.f) continue;
+      const double2 u = rope_exact(poss[i], p.turns[mine.pair(k)], p.amplitude, a, b);
+      dst[d.x] = (uint8_t)c8_code(u.x, inv);
+      dst[d.y] = (uint8_t)c8_code(u.y, inv);
+    }
+  };
+  unsigned near[AP_HELD] = {};
 #pragma unroll
   for (int c = 0; c < AP_HELD; ++c)
-    if (first + warp + c * AP_WARPS < last) store(first + warp + c * AP_WARPS, a[c], b[c]);
+    if (first + warp + c * AP_WARPS < last) near[c] = store(first + warp + c * AP_WARPS, a[c], b[c]);
+#pragma unroll
+  for (int c = 0; c < AP_HELD; ++c)
+    if (near[c]) again(first + warp + c * AP_WARPS, near[c]);
   for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {
     float x[NP], y[NP];
     load(i, x, y);
     prepare(i, x, y);
-    store(i, x, y);
+    const unsigned some = store(i, x, y);
+    if (some) again(i, some);
   }
 }
 
 // ---- any head size -------------------------------------------------------------------------------------------------
-// Element d of a head of token t (row of hd floats), rotated.
-__device__ __forceinline__ float rope_element(const AppendParams& p, const float* row, int pos, int d) {
+// Element d of a head of token t (row of hd floats), rotated (in 64 bits: these sizes are not those that count).
+__device__ __forceinline__ double rope_element(const AppendParams& p, const float* row, int pos, int d) {
   if (d >= p.rot) return row[d];
   const int half = p.rot >> 1;
   const int j = p.interleaved ? d >> 1 : (d < half ? d : d - half);
   const int ia = p.interleaved ? 2 * j : j, ib = p.interleaved ? 2 * j + 1 : j + half;
-  const float2 cs = rope_angle(pos, p.turns[j], p.amplitude);
-  const float a = row[ia], b = row[ib];
-  return d == ia ? a * cs.x - b * cs.y : a * cs.y + b * cs.x;
+  const double2 r = rope_exact(pos, p.turns[j], p.amplitude, row[ia], row[ib]);
+  return d == ia ? r.x : r.y;
 }
 
 // Grid (tokens, 1 + 2 kv heads): y = 0 rotates the token's queries; y = 1 + 2 h + w writes keys (w = 0) or values
@@ -462,7 +525,7 @@ __global__ void __launch_bounds__(128) rope_append_simple_kernel(const AppendPar
     S* q = (S*)p.q_out + (size_t)t0 * p.nh * p.hd;
     for (int i = threadIdx.x; i < p.nh * p.hd; i += blockDim.x) {
       const int head = i / p.hd;
-      q[i] = from_float<S>(rope_element(p, row + head * p.hd, pos0, i - head * p.hd));
+      q[i] = from_float<S>((float)rope_element(p, row + head * p.hd, pos0, i - head * p.hd));
     }
     return;
   }
@@ -486,19 +549,19 @@ __global__ void __launch_bounds__(128) rope_append_simple_kernel(const AppendPar
   while (off0 + n < p.page_size && t0 + n < p.T && p.token_seq[t0 + n] == seq && p.positions[t0 + n] == pos0 + n) ++n;
   const float* src = p.qkv + (size_t)t0 * width + (size_t)(p.nh + (is_v ? p.nkv : 0) + h) * p.hd;
   const size_t at = ((size_t)page * p.nkv + h) * p.page_size;              // row of the pool
-  auto element = [&](int i) -> float {
+  auto element = [&](int i) -> double {
     const int r = i / p.hd, d = i - r * p.hd;
-    return is_v ? src[(size_t)r * width + d] : rope_element(p, src + (size_t)r * width, pos0 + r, d);
+    return is_v ? (double)src[(size_t)r * width + d] : rope_element(p, src + (size_t)r * width, pos0 + r, d);
   };
   if (!p.k_scale) {
     S* dst = (S*)(is_v ? p.v_pool : p.k_pool) + (at + off0) * p.hd;
-    for (int i = threadIdx.x; i < n * p.hd; i += blockDim.x) dst[i] = from_float<S>(element(i));
+    for (int i = threadIdx.x; i < n * p.hd; i += blockDim.x) dst[i] = from_float<S>((float)element(i));
     return;
   }
   uint8_t* dst = (uint8_t*)(is_v ? p.v_pool : p.k_pool) + at * p.hd;
   float* scale = (is_v ? p.v_scale : p.k_scale) + (size_t)page * p.nkv + h;
   unsigned mine = 0;
-  for (int i = threadIdx.x; i < n * p.hd; i += blockDim.x) mine = max(mine, __float_as_uint(element(i)) & 0x7fffffffu);
+  for (int i = threadIdx.x; i < n * p.hd; i += blockDim.x) mine = max(mine, __float_as_uint(__double2float_rz(element(i))) & 0x7fffffffu);
   mine = __reduce_max_sync(0xffffffffu, mine);
   if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = mine;
   const unsigned old = off0 > 0 ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
@@ -514,7 +577,7 @@ __global__ void __launch_bounds__(128) rope_append_simple_kernel(const AppendPar
   }
   const float inv = c8_pow2(-e);
   for (int i = threadIdx.x; i < n * p.hd; i += blockDim.x)
-    dst[off0 * p.hd + i] = finite ? (uint8_t)c8_code(element(i), inv) : (uint8_t)128;
+    dst[off0 * p.hd + i] = finite ? (uint8_t)c8_code(element(i), (double)inv) : (uint8_t)128;
 }
 
 struct UnpackParams {

@@ -150,6 +150,35 @@ def test_append_against_the_definition(rts, dtype, case):
                 assert np.array_equal(scales[which][i], 2.0 ** s.e[which][i])
 
 
+@pytest.mark.parametrize("nkv,hd,P,pairs,inter,amp", [(4, 256, 16, 128, False, 1.0), (4, 128, 16, 32, True, 1.3), (4, 64, 32, 32, False, 0.7),
+                                                      (3, 96, 16, 48, True, 1.0), (3, 256, 16, 33, False, 1.0), (2, 10, 8, 5, False, 1.0)])
+def test_codes_are_those_of_the_definition_to_the_last(rts, nkv, hd, P, pairs, inter, amp):
+    """Codes of rotated keys next to a border between two are decided in 64 bits: 400 tokens at far positions, every code as the
+    definition has it.  (The scale comes from 32 bits: pages whose largest magnitude lies within 2^-20 of a power of two are left out.)"""
+    from glint_b200 import ops_cache8
+    rt, T, start, nh = rts["bfloat16"], 400, 90001, nkv
+    s = Setup(rt, [T], [start], nkv, hd, P, seed=hd, window=1)
+    qkv, turns = _qkv(T, nh, nkv, hd, 3, 0.5), _turns(pairs)
+    ops_cache8.append(rt, s.cache, s.step, qkv.to(DEV), turns.to(DEV), nh, layout="interleaved" if inter else "half", amplitude=amp)
+    rt.check_status()
+    codes = s.cache.k.cpu().numpy()
+    x, n = qkv.double().numpy().reshape(T, nh + 2 * nkv, hd), 0
+    for h in range(nkv):
+        y = np.stack([plain.rotate(x[t, nh + h], start + t, turns.numpy(), inter, amp) for t in range(T)])
+        first = -(-start // P) * P - start                       # the first page begun in this step
+        for t in range(first, T, P):
+            part = y[t:t + P]
+            mantissa = math.frexp(np.abs(part).max())[0]
+            if min(mantissa - 0.5, 1.0 - mantissa) < 2.0 ** -20:
+                continue
+            e = plain.exponent(np.abs(part).max())
+            want = (np.floor(part * 2.0 ** -e) + 128).astype(np.int64)
+            got = codes[s.table[0, (start + t) // P], h, :len(part)]
+            assert np.array_equal(got, want), (h, t, np.abs(got - want).max(), (got != want).sum())
+            n += 1
+    assert n > 0.9 * nkv * ((T - first) // P)
+
+
 @pytest.mark.parametrize("P,hd", [(16, 64), (32, 256), (8, 10)])
 def test_append_does_not_depend_on_the_cuts(rts, P, hd):
     """75 tokens at once, one by one, and in odd portions leave the same codes and scales, bit for bit."""
