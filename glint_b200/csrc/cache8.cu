@@ -47,7 +47,7 @@ struct AppendParams {
   float* k_scale;                // null: pools of the activations' type
   float* v_scale;
   int* status;
-  float amplitude;
+  double amplitude;
   int T, nh, nkv, hd, rot, interleaved, page_size, num_pages, max_pages;
 };
 
@@ -75,7 +75,7 @@ __device__ __forceinline__ float2 rope_angle(int pos, double turns, float amplit
 }
 
 // The pair (a, b) turned, in 64 bits: Taylor polynomials to x^17 and x^16, which leave out less than 1e-15.
-__device__ __noinline__ double2 rope_exact(int pos, double turns, float amplitude, float a, float b) {
+__device__ __noinline__ double2 rope_exact(int pos, double turns, double amplitude, float a, float b) {
   const double quarters = 4.0 * turns * (double)pos;
   const double n = rint(quarters);
   const double x = (quarters - n) * 1.5707963267948966, y = x * x;
@@ -108,7 +108,8 @@ __device__ __forceinline__ unsigned c8_code(double x, double inv) { return (unsi
 // of queries written; 11.3 + 4.2 us) / a mixed step of 997 tokens, 32 heads in 16 groups of 128: 16.6 / 22.9 us; two or eight
 // heads a warp 17.4 / 24.6 and 23.1 / 23.9; one or four tokens held 18.0 / 24.2 and 17.4 / 23.6; room for three, five or
 // six blocks an SM instead of four 18.5 / 22.8, 17.8 / 21.4 and 20.7 / 21.9, so that heads of 256 take four, smaller ones five.
-// One token takes 2.4 us behind a kernel that it can begin under.
+// (All before keys next to a border were decided in 64 bits, which adds 0.8 / 1.0.)  One token takes 2.4 us behind a kernel
+// that it can begin under.
 constexpr int AP_WARPS = 8;
 constexpr int AP_WINDOW = 16;                     // tokens
 constexpr int AP_HELD = 2;                        // tokens of a warp whose values stay in registers
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
     const int pos = p.positions[t];
     float2 turned_by[NP];
 #pragma unroll
-    for (int k = 0; k < NP; ++k) turned_by[k] = mine.turned(k) ? rope_angle(pos, turns[k], p.amplitude) : make_float2(1.f, 0.f);
+    for (int k = 0; k < NP; ++k) turned_by[k] = mine.turned(k) ? rope_angle(pos, turns[k], (float)p.amplitude) : make_float2(1.f, 0.f);
     pdl_wait_release();
     const float* src = p.qkv + (size_t)t * width + (size_t)h0 * p.hd;
     S* dst = (S*)p.q_out + ((size_t)t * p.nh + h0) * p.hd;
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       if (!is_v && mine.turned(k)) {
-        const float2 cs = rope_angle(poss[i], turns[k], p.amplitude);
+        const float2 cs = rope_angle(poss[i], turns[k], (float)p.amplitude);
         const float u = x[k], v = y[k];
         x[k] = u * cs.x - v * cs.y;
         y[k] = u * cs.y + v * cs.x;
@@ -702,7 +703,7 @@ using namespace glint;
 // q_out, keys and values to the pages: coded when there are scales, else in `dtype`.  k_pool null: queries only.
 // The tokens of a request stand together in ascending positions (status 5 otherwise).
 GLINT_API int glint_rope_append(const float* qkv, const int* positions, const int* token_seq, const int* block_table,
-                                int max_pages, const double* turns, int rot, int interleaved, float amplitude, void* q_out,
+                                int max_pages, const double* turns, int rot, int interleaved, double amplitude, void* q_out,
                                 int dtype, void* k_pool, void* v_pool, float* k_scale, float* v_scale, int T, int nh,
                                 int nkv, int hd, int page_size, int num_pages, int* status, cudaStream_t stream) {
   if (T <= 0) return GLINT_OK;

@@ -20,7 +20,7 @@ int glint_rope_kv_write(const float* qkv, const int* positions, const int* token
                         void* v_pool, int dtype, int T, int nh, int nkv, int hd, int page_size, int num_pages,
                         int* status, cudaStream_t stream);
 int glint_rope_append(const float* qkv, const int* positions, const int* token_seq, const int* block_table,
-                      int max_pages, const double* turns, int rot, int interleaved, float amplitude, void* q_out,
+                      int max_pages, const double* turns, int rot, int interleaved, double amplitude, void* q_out,
                       int dtype, void* k_pool, void* v_pool, float* k_scale, float* v_scale, int T, int nh, int nkv,
                       int hd, int page_size, int num_pages, int* status, cudaStream_t stream);
 int glint_cache8_unpack(const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
@@ -194,7 +194,7 @@ extern "C" int glint_op_rope_append(const GlintRuntime* rt, const GlintStep* ste
 // For callers with a rotary encoding at hand that is not kept in a GlintRope.
 extern "C" int glint_op_rope_append_with(const GlintRuntime* rt, const GlintStep* step, const float* qkv, void* q_out,
                                          const GlintView* view, int nh, int nkv, int hd, const double* turns,
-                                         int rotary_dim, int interleaved, float amplitude, cudaStream_t stream) {
+                                         int rotary_dim, int interleaved, double amplitude, cudaStream_t stream) {
   const GlintRope rope = {turns, rotary_dim, interleaved, amplitude, 1};
   return glint_op_rope_append(rt, step, qkv, q_out, view, nh, nkv, hd, &rope, stream);
 }

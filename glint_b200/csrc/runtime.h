@@ -119,7 +119,7 @@ struct GlintRope {
   const double* turns;          // [rotary_dim / 2] turns per position
   int rotary_dim;
   int interleaved;              // pairs (2 j, 2 j + 1) instead of (j, j + rotary_dim / 2)
-  float amplitude;              // of the rotated dims
+  double amplitude;             // of the rotated dims
   int only;                     // 1: always this kernel (interleaved pairs or an amplitude: no other takes them)
 };
 

@@ -11,7 +11,7 @@ short program and runs it at once.  Which kernel an operation takes is decided i
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, Structure, c_float, c_int, c_longlong, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -81,7 +81,7 @@ def cache8_scratch(num_kv_heads, head_dim, device):
 
 class RopeStruct(Structure):
     """``GlintRope`` of csrc/runtime.h."""
-    _fields_ = [("turns", c_void_p), ("rotary_dim", c_int), ("interleaved", c_int), ("amplitude", c_float),
+    _fields_ = [("turns", c_void_p), ("rotary_dim", c_int), ("interleaved", c_int), ("amplitude", c_double),
                 ("only", c_int)]
 
 

@@ -6,7 +6,7 @@ loaded, or a tensor is not on a CUDA device, the call raises ``KernelError``.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -57,7 +57,7 @@ _CORE_SIGNATURES = {
     "glint_add_rmsnorm": [_P, _P, _P, _F, _F, _P, _I, _P, _F, _F, _I, _I, _P],
     "glint_rope_table": [_P, _P, _F, _P, _I, _I, _P],
     "glint_rope_kv_write": [_P, _P, _P, _P, _I, _P, _F, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
-    "glint_rope_append": [_P, _P, _P, _P, _I, _P, _I, _I, _F, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
+    "glint_rope_append": [_P, _P, _P, _P, _I, _P, _I, _I, c_double, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
     "glint_gated_act": [_P, _P, _I, _I, _I, _I, _P],
     "glint_softcap": [_P, _L, _F, _P],
     "glint_place_tokens": [_P, _P, _P, _P, _I, _P],

@@ -14,7 +14,7 @@ one ``Cache8`` belong on one stream, or on streams that wait for each other, gra
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_void_p
+from ctypes import c_double, c_float, c_int, c_void_p
 from dataclasses import dataclass
 
 import torch
@@ -35,7 +35,7 @@ def _lib():
     if _routed is None:
         lib = native.lib()
         P, I, F = c_void_p, c_int, c_float
-        lib.glint_op_rope_append_with.argtypes = [P, P, P, P, P, I, I, I, P, I, I, F, P]
+        lib.glint_op_rope_append_with.argtypes = [P, P, P, P, P, I, I, I, P, I, I, c_double, P]
         lib.glint_op_cache8_unpack.argtypes = [P, P, P, I, I, I, P]
         lib.glint_op_attention.argtypes = [P, P, P, P, P, I, I, I, F, F, I, P]
         for f in (lib.glint_op_rope_append_with, lib.glint_op_cache8_unpack, lib.glint_op_attention):
