@@ -313,7 +313,9 @@ static int decode_attention(const GlintRuntime* rt, const GlintStep* step, const
 
 // Attention over coded pages.  Single tokens (all, or those in front of portions) read the codes; portions read wide
 // pages, which a kernel in front writes once for all their query tiles: inside the tiled kernel every block of 128 query
-// rows would widen the same keys again.  Sizes that no tensor-core kernel takes are widened whole.
+// rows would widen the same keys again.  Sizes that no tensor-core kernel takes are widened whole.  Single tokens in front
+// of portions leave only where the kernel behind finds its tokens by their request's offsets: one that goes by the step's
+// tokens (more than 64 query heads a kv head over pages that the portion kernel does not take, or more than 128) takes all.
 static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const void* q, const GlintView* view, void* out,
                            int nh, int nkv, int hd, float multiplier, float cap, int window, cudaStream_t stream) {
   const GlintTensorEntries& t = rt->tensor;
@@ -323,7 +325,9 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
                       t.attention_decode8_workspace(blocks, nh, nkv, hd) <= view->partial_floats;
   const int reach = window > 0 && window < step->max_context ? window : step->max_context;
   const bool each_alone = step->max_seq_len == 1 || few_tokens(step->num_tokens, reach, nkv, hd);
-  const int lead = !single ? 0 : each_alone ? step->num_tokens : step->leading_single;
+  const bool portion = rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_portion && step->max_seq_len > 1 &&
+                       t.attention_portion_supported(nh, nkv, hd, page);
+  const int lead = !single ? 0 : each_alone ? step->num_tokens : portion || prefill_supported(nh, nkv, hd) ? step->leading_single : 0;
   if (lead > 0) {
     const int rc = counted(t.attention_decode8(
         q, (const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale, step->positions, step->token_seq,
@@ -343,8 +347,7 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
   wide.k = view->k_wide;
   wide.v = view->v_wide;
   wide.k_scale = wide.v_scale = nullptr;
-  if (rt->tensor_cores && rt->dtype == GLINT_DTYPE_BF16 && t.attention_portion && rest.max_seq_len > 1 &&
-      t.attention_portion_supported(nh, nkv, hd, page))
+  if (portion)
     return counted(t.attention_portion(q, wide.k, wide.v, rest.cu_seqlens, rest.seq_start, rest.block_table[g], rest.max_pages[g],
                                        out, step->num_tokens, step->num_tokens - lead, rest.num_seqs, rest.max_seq_len, rest.max_context, nh, nkv, hd, page,
                                        view->num_pages, multiplier, cap, window, rt->sms, view->partials, view->partial_floats,
