@@ -61,6 +61,7 @@ struct Decode8Params {
   int* status;
   float multiplier, cap;
   int T, nh, nkv, hd, groups, page_size, splits, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units;
+  int early;                    // positions, requests and tables are no kernel's work: read before the wait
 };
 
 // Rows that a block reads: the first of them in the pools (-1: none), their scales.
@@ -302,8 +303,9 @@ attention_decode8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     tc::tma_prefetch_desc(&map_k);
     tc::tma_prefetch_desc(&map_v);
   }
-  // ---- where this block begins: every warp scans the tokens' units for itself, some consecutive tokens per lane.  Positions,
-  // requests and block tables come by copies, no kernel writes them: all this passes under the kernel in front. ---------
+  // ---- where this block begins: every warp scans the tokens' units for itself, some consecutive tokens per lane.  Where
+  // positions, requests and block tables come by copies, all this passes under the kernel in front. ---------------------
+  if (!p.early) pdl_wait();
   const int per = (p.T + 31) >> 5;
   const int r0 = min(lane * per, p.T), r1 = min(r0 + per, p.T);
   int mine = 0, row_first = 0;
@@ -731,12 +733,13 @@ GLINT_API long long glint_attention_decode8_workspace(int blocks, int nh, int nk
 // q, out [T][nh][hd] bfloat16, pages of codes with their scales; T single tokens of which none attends more than
 // `max_context` keys.  `partials`: glint_attention_decode8_workspace floats, 16-byte aligned; `arrive`: `arrive_ints`
 // counters that are zero before the first launch (every launch leaves them zero).  Launches of more tokens than
-// the counters or 1024 allow are cut.  `blocks`: at most that many blocks (two per SM).
+// the counters or 1024 allow are cut.  `blocks`: at most that many blocks (two per SM).  `early`: positions, requests and
+// block tables were on the device before the kernel in front began (copies, not a kernel's results).
 GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, const uint8_t* v_pool, const float* k_scale,
                                       const float* v_scale, const int* positions, const int* token_seq, const int* block_table,
                                       int max_pages, void* out, int T, int nh, int nkv, int hd, int page_size, int num_pages,
                                       float multiplier, float cap, int window, int max_context, int blocks, float* partials,
-                                      int* arrive, int arrive_ints, int* status, cudaStream_t stream) {
+                                      int* arrive, int arrive_ints, int* status, int early, cudaStream_t stream) {
   if (T <= 0) return GLINT_OK;
   if (!partials || !arrive || blocks < 1 || max_pages < 1 || ((uintptr_t)partials & 15)) return GLINT_ERR_BAD_ARG;
   if (!glint_attention_decode8_supported(nh, nkv, hd, page_size)) return GLINT_ERR_UNSUPPORTED_SIZE;
@@ -793,7 +796,8 @@ GLINT_API int glint_attention_decode8(const void* q, const uint8_t* k_pool, cons
     const int n = T - t0 < step ? T - t0 : step;
     Decode8Params p = {(const __nv_bfloat16*)q + (size_t)t0 * nh * hd, positions + t0, token_seq + t0, block_table, k_scale, v_scale,
                        (__nv_bfloat16*)out + (size_t)t0 * nh * hd, partials, arrive, status, multiplier, cap,
-                       n, nh, nkv, hd, groups, page_size, splits, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units};
+                       n, nh, nkv, hd, groups, page_size, splits, num_pages, max_pages, window, stages, whole_page, pair_cost, min_units,
+                       early};
     const long long most = (long long)n * pairs * (most_pages + pair_cost);
     const long long useful = (most + min_units - 1) / min_units;
     const int grid = useful < blocks ? (int)useful : blocks;

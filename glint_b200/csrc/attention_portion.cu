@@ -57,6 +57,7 @@ struct PortionParams {
   int max_pages, nh, nkv, hd, page_size, num_pages, window, n_seqs, whole, k_stages, v_stages;
   int split_from, splits;       // tiles (query tile, kv head) from there on have their keys split over that many blocks
   int split_tiles;              // and are that many
+  int early;                    // offsets and starts are no kernel's work: read before the wait
 };
 
 struct PortionShared {
@@ -191,8 +192,9 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int split = may_split ? behind / p.split_tiles : 0, split_tile = behind - split * p.split_tiles;
   const int index = may_split ? p.split_from + split_tile : (int)blockIdx.x;
   const int kvh = index % p.nkv;
+  if (!p.early) pdl_wait();
   PortionTile work;
-  const bool found = portion_tile(p, tok_per_tile, index / p.nkv, work);         // no kernel writes what this reads
+  const bool found = portion_tile(p, tok_per_tile, index / p.nkv, work);
   pdl_wait_release();
   if (tc::smem_u32(at_raw) & 1023) {                     // the operands' swizzle wants it
     if (threadIdx.x == 0) atomicExch(p.status, 4);
@@ -688,11 +690,12 @@ GLINT_API int glint_attention_portion_supported(int nh, int nkv, int hd, int pag
 // q, out: [T, nh * hd] bf16; pools [pages][nkv][page_size][hd] bf16, finite everywhere; cu_seqlens (absolute token offsets),
 // seq_start and block_table of the n_seqs portions, which have `tokens` tokens in all and of which none is longer than max_q_len or attends more than
 // max_context keys.  `scratch`: floats for partial results, 16-byte aligned (none, or too few: the keys are not split).
+// `early`: cu_seqlens and seq_start were on the device before the kernel in front began (copies, not a kernel's results).
 GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const void* v_pool, const int* cu_seqlens,
                                       const int* seq_start, const int* block_table, int max_pages, void* out, int T,
                                       int tokens, int n_seqs, int max_q_len, int max_context, int nh, int nkv, int hd, int page_size,
                                       int num_pages, float multiplier, float cap, int window, int sms, float* scratch,
-                                      long long scratch_floats, int* status, cudaStream_t stream) {
+                                      long long scratch_floats, int* status, int early, cudaStream_t stream) {
   if (n_seqs <= 0 || max_q_len <= 0 || tokens <= 0 || T < tokens) return GLINT_OK;
   if (!glint_attention_portion_supported(nh, nkv, hd, page_size)) return GLINT_ERR_UNSUPPORTED_SIZE;
   if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) return GLINT_ERR_UNSUPPORTED_SIZE;
@@ -730,7 +733,7 @@ GLINT_API int glint_attention_portion(const void* q, const void* k_pool, const v
   PortionParams p = {};
   p.cu_seqlens = cu_seqlens; p.seq_start = seq_start; p.block_table = block_table; p.max_pages = max_pages;
   p.out = (__nv_bfloat16*)out; p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.num_pages = num_pages;
-  p.multiplier = multiplier; p.cap = cap; p.window = window; p.whole = whole; p.status = status; p.n_seqs = n_seqs;
+  p.multiplier = multiplier; p.cap = cap; p.window = window; p.whole = whole; p.status = status; p.n_seqs = n_seqs; p.early = early;
   const int nsub = (hd + 63) / 64;
   // As many tiles ahead as fit, up to four: two of each do nearly as well (ragged portions, heads of 128: 91 against 90 us;
   // heads of 256, which have room for three of keys and two of values: 4,096 tokens 134.5 against 133.9, 250 behind 7,900 61.6

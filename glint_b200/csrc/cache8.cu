@@ -49,6 +49,7 @@ struct AppendParams {
   int* status;
   double amplitude;
   int T, nh, nkv, hd, rot, interleaved, page_size, num_pages, max_pages;
+  int early;                     // positions, requests, tables and turns are no kernel's work: read before the wait
 };
 
 // (cos, sin) of 2 pi pos turns, times the amplitude.  The product is taken in 64 bits and reduced to an eighth of a turn
@@ -273,6 +274,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int width = (p.nh + 2 * p.nkv) * p.hd, pairs = p.hd >> 1;
   const RopeLane<NP, FULL> mine = {lane, p.rot >> 1, pairs, p.rot, p.interleaved};
+  if (!p.early) pdl_wait();
   double turns[NP];
 #pragma unroll
   for (int k = 0; k < NP; ++k) turns[k] = mine.turned(k) ? p.turns[mine.pair(k)] : 0.0;
@@ -309,8 +311,8 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
     return;
   }
 
-  // ---- keys and values.  Positions, requests and block tables come by copies, no kernel writes them: all that follows from
-  // them passes under the kernel in front. ---------------------------------------------------------------------------------
+  // ---- keys and values.  Where positions, requests and block tables come by copies (`early`), all that follows from them
+  // passes under the kernel in front. --------------------------------------------------------------------------------------
   // Of the window's tokens and those behind it that may belong to its runs: what a thread finds out for all.
   __shared__ unsigned starts[AP_WARPS], bad[AP_WARPS];    // does a run begin there; does it break the order
   __shared__ int poss[AP_WARPS * 32], offs[AP_WARPS * 32];
@@ -592,7 +594,7 @@ struct UnpackParams {
   void* k_out;
   void* v_out;
   int* status;
-  int max_pages, window, nkv, page_elems, page_size, num_pages;
+  int max_pages, window, nkv, page_elems, page_size, num_pages, early;
 };
 
 // A page that a request can reach: its place in the pools, -1 if there is none.
@@ -649,7 +651,8 @@ constexpr int UP_EACH = 2;                        // sixteens of a thread; 1: 16
 
 template <typename S>
 __global__ void __launch_bounds__(UP_THREADS) cache8_unpack_kernel(const UnpackParams p, int parts) {
-  const int page = unpack_page(p, blockIdx.y, blockIdx.x);     // no kernel writes what this reads
+  if (!p.early) pdl_wait();
+  const int page = unpack_page(p, blockIdx.y, blockIdx.x);
   pdl_wait_release();
   if (page < 0) return;
   const int is_v = (int)blockIdx.z >= parts;
@@ -701,18 +704,19 @@ using namespace glint;
 // qkv [T][nh + 2 nkv][hd] float32: the first `rot` dims of every query and key head are turned in pairs, (j, j + rot/2)
 // or, interleaved, (2 j, 2 j + 1), by positions[t] * turns[j] of a full turn, scaled by `amplitude`; queries go to
 // q_out, keys and values to the pages: coded when there are scales, else in `dtype`.  k_pool null: queries only.
-// The tokens of a request stand together in ascending positions (status 5 otherwise).
+// The tokens of a request stand together in ascending positions (status 5 otherwise).  `early`: positions, requests, block
+// tables and turns were on the device before the kernel in front began (copies, not a kernel's results).
 GLINT_API int glint_rope_append(const float* qkv, const int* positions, const int* token_seq, const int* block_table,
                                 int max_pages, const double* turns, int rot, int interleaved, double amplitude, void* q_out,
                                 int dtype, void* k_pool, void* v_pool, float* k_scale, float* v_scale, int T, int nh,
-                                int nkv, int hd, int page_size, int num_pages, int* status, cudaStream_t stream) {
+                                int nkv, int hd, int page_size, int num_pages, int* status, int early, cudaStream_t stream) {
   if (T <= 0) return GLINT_OK;
   if (hd <= 0 || hd % 2 || rot % 2 || rot < 0 || rot > hd || nh <= 0 || nkv <= 0 || page_size <= 0) return GLINT_ERR_BAD_ARG;
   if (!k_pool != !v_pool || !k_scale != !v_scale || (k_scale && !k_pool)) return GLINT_ERR_BAD_ARG;
   if (k_scale && (((uintptr_t)k_pool | (uintptr_t)v_pool) & 1)) return GLINT_ERR_BAD_ARG;      // codes are moved in pairs
   if (nkv > 32767) return GLINT_ERR_UNSUPPORTED_SIZE;
   AppendParams p = {qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_pool, k_scale, v_scale, status, amplitude,
-                    T, nh, nkv, hd, rot, interleaved ? 1 : 0, page_size, num_pages, max_pages};
+                    T, nh, nkv, hd, rot, interleaved ? 1 : 0, page_size, num_pages, max_pages, early};
   cudaError_t e = cudaSuccess;
   if (hd <= 256 && page_size <= AP_MOST_PAGE) {
     const long long cache_blocks = k_pool ? (long long)((T + AP_WINDOW - 1) / AP_WINDOW) * 2 * nkv : 0;
@@ -739,16 +743,16 @@ GLINT_API int glint_rope_append(const float* qkv, const int* positions, const in
 
 // Codes of the pages that the new tokens of each request can reach (from the page of the first key that the first of
 // them sees, to the page of the last of them) as values of `dtype`, at the same places of the wide pools.
-// `most_pages`: at least the pages of any request's range (status 6 where it is less).
+// `most_pages`: at least the pages of any request's range (status 6 where it is less).  `early` as for glint_rope_append.
 GLINT_API int glint_cache8_unpack(const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
                                   const int* seq_start, const int* cu_seqlens, const int* block_table, int max_pages,
                                   void* k_out, void* v_out, int dtype, int n_seqs, int most_pages, int window, int nkv,
-                                  int hd, int page_size, int num_pages, int* status, cudaStream_t stream) {
+                                  int hd, int page_size, int num_pages, int* status, int early, cudaStream_t stream) {
   if (n_seqs <= 0 || most_pages <= 0) return GLINT_OK;
   if (nkv <= 0 || hd <= 0 || page_size <= 0 || (long long)page_size * hd > 0x7fffffffLL) return GLINT_ERR_BAD_ARG;
   if (nkv > 65535 || n_seqs > 65535) return GLINT_ERR_UNSUPPORTED_SIZE;
   UnpackParams p = {k, v, k_scale, v_scale, seq_start, cu_seqlens, block_table, k_out, v_out, status, max_pages, window, nkv,
-                    page_size * hd, page_size, num_pages};
+                    page_size * hd, page_size, num_pages, early};
   cudaError_t e = cudaSuccess;
   const long long parts = ((long long)nkv * page_size * hd / 16 + UP_THREADS * UP_EACH - 1) / (UP_THREADS * UP_EACH);
   const bool aligned = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_out | (uintptr_t)v_out) & 15);

@@ -22,11 +22,11 @@ int glint_rope_kv_write(const float* qkv, const int* positions, const int* token
 int glint_rope_append(const float* qkv, const int* positions, const int* token_seq, const int* block_table,
                       int max_pages, const double* turns, int rot, int interleaved, double amplitude, void* q_out,
                       int dtype, void* k_pool, void* v_pool, float* k_scale, float* v_scale, int T, int nh, int nkv,
-                      int hd, int page_size, int num_pages, int* status, cudaStream_t stream);
+                      int hd, int page_size, int num_pages, int* status, int early, cudaStream_t stream);
 int glint_cache8_unpack(const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
                         const int* seq_start, const int* cu_seqlens, const int* block_table, int max_pages,
                         void* k_out, void* v_out, int dtype, int n_seqs, int most_pages, int window, int nkv, int hd,
-                        int page_size, int num_pages, int* status, cudaStream_t stream);
+                        int page_size, int num_pages, int* status, int early, cudaStream_t stream);
 int glint_gated_act(const float* gu, void* out, int dtype, int T, int I, int act, cudaStream_t stream);
 int glint_gemm_plain(const void* A, const void* W, int dtype, float* out, int M, int N, int K, float cap,
                      cudaStream_t stream);
@@ -188,7 +188,8 @@ extern "C" int glint_op_rope_append(const GlintRuntime* rt, const GlintStep* ste
                                    rope->turns, rope->rotary_dim, rope->interleaved, rope->amplitude, q_out, rt->dtype,
                                    view->writes ? view->k : nullptr, view->writes ? view->v : nullptr,
                                    view->writes ? view->k_scale : nullptr, view->writes ? view->v_scale : nullptr,
-                                   step->num_tokens, nh, nkv, hd, view->page_size, view->num_pages, rt->status, stream));
+                                   step->num_tokens, nh, nkv, hd, view->page_size, view->num_pages, rt->status, step->copied,
+                                   stream));
 }
 
 // For callers with a rotary encoding at hand that is not kept in a GlintRope.
@@ -213,7 +214,7 @@ extern "C" int glint_op_cache8_unpack(const GlintRuntime* rt, const GlintStep* s
   return counted(glint_cache8_unpack((const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale,
                                      step->seq_start, step->cu_seqlens, step->block_table[g], step->max_pages[g],
                                      view->k_wide, view->v_wide, rt->dtype, step->num_seqs, (int)most, window, nkv, hd, page,
-                                     view->num_pages, rt->status, stream));
+                                     view->num_pages, rt->status, step->copied, stream));
 }
 
 extern "C" int glint_op_qkv_rope(const GlintRuntime* rt, const GlintStep* step, const void* x, const void* w,
@@ -332,7 +333,7 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
     const int rc = counted(t.attention_decode8(
         q, (const uint8_t*)view->k, (const uint8_t*)view->v, view->k_scale, view->v_scale, step->positions, step->token_seq,
         step->block_table[g], step->max_pages[g], out, lead, nh, nkv, hd, page, view->num_pages, multiplier, cap, window,
-        step->max_context, blocks, view->partials, view->arrive, view->arrive_ints, rt->status, stream));
+        step->max_context, blocks, view->partials, view->arrive, view->arrive_ints, rt->status, step->copied, stream));
     if (rc != GLINT_OK || lead == step->num_tokens) return rc;
   }
   GlintStep rest = *step;                        // the requests behind; their tokens keep their absolute offsets
@@ -351,7 +352,7 @@ static int coded_attention(const GlintRuntime* rt, const GlintStep* step, const 
     return counted(t.attention_portion(q, wide.k, wide.v, rest.cu_seqlens, rest.seq_start, rest.block_table[g], rest.max_pages[g],
                                        out, step->num_tokens, step->num_tokens - lead, rest.num_seqs, rest.max_seq_len, rest.max_context, nh, nkv, hd, page,
                                        view->num_pages, multiplier, cap, window, rt->sms, view->partials, view->partial_floats,
-                                       rt->status, stream));
+                                       rt->status, step->copied, stream));
   return glint_op_attention(rt, lead ? &rest : step, q, &wide, out, nh, nkv, hd, multiplier, cap, window, stream);
 }
 

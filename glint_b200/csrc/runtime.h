@@ -33,6 +33,8 @@ struct GlintStep {
   const int* logit_rows;        // [logit rows]
   const int* block_table[GLINT_MAX_GROUPS];   // per cache group: [requests][max_pages]
   int max_pages[GLINT_MAX_GROUPS];
+  int copied;                   // 1: the device arrays came by a copy, which is over before any kernel behind it begins: kernels may
+                                // read them before they wait for the kernel in front.  0: a kernel in front may have written them
 };
 
 // Entry points of the tensor-core library, bound at run time (a float32 process never loads it).
@@ -53,11 +55,11 @@ struct GlintTensorEntries {
                                  int*, cudaStream_t);
   int (*attention_decode8)(const void*, const uint8_t*, const uint8_t*, const float*, const float*, const int*, const int*,
                            const int*, int, void*, int, int, int, int, int, int, float, float, int, int, int, float*, int*,
-                           int, int*, cudaStream_t);
+                           int, int*, int, cudaStream_t);
   int (*attention_decode8_supported)(int, int, int, int);
   long long (*attention_decode8_workspace)(int, int, int, int);
   int (*attention_portion)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int, int, int, int,
-                           int, int, int, int, int, int, float, float, int, int, float*, long long, int*, cudaStream_t);
+                           int, int, int, int, int, int, float, float, int, int, float*, long long, int*, int, cudaStream_t);
   int (*attention_portion_supported)(int, int, int, int);
   int (*attention_prefill)(const void*, const void*, const void*, const int*, const int*, const int*, int, void*, int,
                            int, int, int, int, int, int, float, float, int, int*, cudaStream_t);

@@ -30,7 +30,7 @@ class StepStruct(Structure):
                 ("num_groups", c_int), ("uneven", c_int),
                 ("token_ids", c_void_p), ("positions", c_void_p), ("token_seq", c_void_p), ("seq_slot", c_void_p),
                 ("seq_start", c_void_p), ("cu_seqlens", c_void_p), ("logit_rows", c_void_p),
-                ("block_table", c_void_p * MAX_GROUPS), ("max_pages", c_int * MAX_GROUPS)]
+                ("block_table", c_void_p * MAX_GROUPS), ("max_pages", c_int * MAX_GROUPS), ("copied", c_int)]
 
 
 class TensorEntries(Structure):
@@ -158,7 +158,8 @@ def make_runtime_struct(rt):
 
 
 def fill_step(step, ctx, step_id):
-    """Copy a ``StepContext`` into the structure the executor reads."""
+    """Copy a ``StepContext`` into the structure the executor reads.  Its arrays come by one copy in front of the step's kernels."""
+    step.copied = 1
     step.id = step_id
     step.num_tokens, step.num_seqs = ctx.num_tokens, ctx.num_seqs
     step.max_seq_len, step.max_context = ctx.max_seq_len, ctx.max_context

@@ -57,7 +57,7 @@ _CORE_SIGNATURES = {
     "glint_add_rmsnorm": [_P, _P, _P, _F, _F, _P, _I, _P, _F, _F, _I, _I, _P],
     "glint_rope_table": [_P, _P, _F, _P, _I, _I, _P],
     "glint_rope_kv_write": [_P, _P, _P, _P, _I, _P, _F, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
-    "glint_rope_append": [_P, _P, _P, _P, _I, _P, _I, _I, c_double, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
+    "glint_rope_append": [_P, _P, _P, _P, _I, _P, _I, _I, c_double, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _P],
     "glint_gated_act": [_P, _P, _I, _I, _I, _I, _P],
     "glint_softcap": [_P, _L, _F, _P],
     "glint_place_tokens": [_P, _P, _P, _P, _I, _P],
@@ -201,7 +201,7 @@ def rope_append(qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_
     check(core().glint_rope_append(ptr(qkv), ptr(positions), ptr(token_seq), ptr(block_table), block_table.shape[1],
                                    ptr(turns), 2 * turns.numel(), int(bool(interleaved)), amplitude, ptr(q_out),
                                    dtype_code(q_out.dtype), ptr(k_pool), ptr(v_pool), ptr(k_scale), ptr(v_scale), T, nh,
-                                   nkv, hd, page_size, num_pages, ptr(status), stream()), "rope_append")
+                                   nkv, hd, page_size, num_pages, ptr(status), 0, stream()), "rope_append")
 
 
 def rope_table(positions, inv_freq, factor, out):

@@ -1,0 +1,52 @@
+"""The coded cache's operators behind kernels that write a step's arrays: what they read is what those kernels leave."""
+import pytest
+import torch
+
+from tests.test_cache8_gpu import DEV, Setup, _qkv, _turns, rts  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("lens,starts", [([1] * 8, [40 * i + 3 for i in range(8)]), ([60, 20], [7, 300])])
+def test_arrays_written_by_a_kernel_that_lets_its_successor_begin(rts, lens, starts):
+    """Positions, starts, table and turns come from kernels directly in front of every call (the ones that place values release
+    their successor before they write); attention, append and widening give, bit for bit, what they give once the device is idle."""
+    from glint_b200 import ops, ops_cache8
+    rt, nh, nkv, hd, P = rts["bfloat16"], 8, 4, 128, 16
+    T, R = sum(lens), len(lens)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    qkv = _qkv(T, nh, nkv, hd, 1, 0.3).to(DEV)
+    turns = _turns(hd // 2).to(DEV)
+    results = []
+    for idle in (True, False):
+        s = Setup(rt, lens, [a + 40 for a in starts], nkv, hd, P, seed=6)
+        t = s.step.tensors
+        table = t["block_table"].clone()
+        rows = {n: torch.arange(t[n].numel(), dtype=torch.int32, device=DEV) for n in ("positions", "seq_start", "block_table")}
+        own = torch.empty_like(turns)
+        wait = torch.cuda.synchronize if idle else (lambda: None)
+        got = []
+        for at in range(40):
+            sources = {"positions": i32([a + at + k for a, n in zip(starts, lens) for k in range(n)]),
+                       "seq_start": i32([a + at for a in starts]), "block_table": table.view(-1)}
+            torch.cuda.synchronize()
+            def behind_the_writers(call):
+                own.zero_()
+                for n in rows:
+                    t[n].zero_()
+                own.copy_(turns)
+                for n in rows:
+                    ops.place_tokens(t[n].view(-1), rows[n], sources[n], rows[n])
+                s.step.begin()
+                wait()
+                got.append(call())
+                wait()
+                return got[-1]
+            q = behind_the_writers(lambda: ops_cache8.append(rt, s.cache, s.step, qkv, own, nh))
+            behind_the_writers(lambda: ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.1, softcap=50.0))
+            behind_the_writers(lambda: torch.stack(ops_cache8.unpack(rt, s.cache, s.step)))
+        got += [t.clone() for t in (s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale)]
+        rt.check_status()
+        results.append(got)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
