@@ -50,3 +50,38 @@ def test_arrays_written_by_a_kernel_that_lets_its_successor_begin(rts, lens, sta
         results.append(got)
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_portions_between_products_and_beside_others(rts, hd):
+    """Portions in front of tiled products, which take tensor memory of their own while they wait, and at the same time portions
+    over another cache on another stream: bit for bit what each gives alone."""
+    from glint_b200 import ops_cache8, ops_tensor
+    rt, nh, nkv, P = rts["bfloat16"], 8, 4, 16
+    g = torch.Generator().manual_seed(hd)
+    setups = [Setup(rt, [300, 40], [150, 900], nkv, hd, P, seed=s) for s in (1, 2)]
+    q = (0.2 * torch.randn(340, nh * hd, generator=g)).to(DEV, torch.bfloat16)
+    w = (0.05 * torch.randn(256, nh * hd, generator=g)).to(DEV, torch.bfloat16)
+
+    def once(s, product):
+        out = ops_cache8.attention(rt, s.cache, s.step, q, nh, 0.1, softcap=50.0)
+        y = torch.empty(340, 256, dtype=torch.float32, device=DEV)
+        if product:
+            ops_tensor.gemm(out, w, y, status=rt.status, force_splits=1, path="tcgen05")
+        return (out, y) if product else (out,)
+    want = []
+    for k, s in enumerate(setups):
+        want.append(once(s, k == 0))
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in setups]
+    got = [[], []]
+    for _ in range(20):
+        for k, (s, stream) in enumerate(zip(setups, streams)):
+            with torch.cuda.stream(stream):
+                got[k].append(once(s, k == 0))
+    torch.cuda.synchronize()
+    rt.check_status()
+    for k in range(2):
+        for outs in got[k]:
+            for a, b in zip(outs, want[k]):
+                assert torch.equal(a, b)
