@@ -28,6 +28,11 @@ __device__ __forceinline__ float c8_distance(float x, float inv) {
   const float h = x * inv, magic = 12582912.f;           // 1.5 * 2^23: the nearest whole number
   return fabsf(h - ((h + magic) - magic));
 }
+// A largest magnitude, given as bits, so near a power of two (16 steps of 32 bits, where 10 are the most that the rotation can be
+// off) that 64 bits have to say which exponent it has.
+__device__ __forceinline__ bool c8_near_scale(unsigned bits) {
+  return bits >= 13u << 23 && bits < C8_NOT_FINITE && ((bits + 16u) & 0x7fffffu) < 32u;
+}
 // floor(x / s) + 128.  The product is exact, but for the smallest numbers under the largest scales, where it may become
 // -0: the floor of any negative number is at most -1.
 __device__ __forceinline__ unsigned c8_code(float x, float inv) {
@@ -94,7 +99,7 @@ __device__ __noinline__ double2 rope_exact(int pos, double turns, double amplitu
   const double cs = ((q + 1) & 2 ? -1.0 : 1.0) * (q & 1 ? s : c) * amplitude, sn = (q & 2 ? -1.0 : 1.0) * (q & 1 ? c : s) * amplitude;
   return make_double2(a * cs - b * sn, a * sn + b * cs);
 }
-// The scale was found in 32 bits: in 64 a value may reach 128 s.
+// (A value turned beyond what 32 bits hold is held to the largest code.)
 __device__ __forceinline__ unsigned c8_code(double x, double inv) { return (unsigned)(max(-128, min(127, (int)floor(x * inv))) + 128); }
 
 // ---- heads of up to 256: a lane holds NP pairs of a head ------------------------------------------------------------
@@ -393,9 +398,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
     if (first + warp + c * AP_WARPS < last) load(first + warp + c * AP_WARPS, a[c], b[c]);
   if (owned > -2) olds[me] = coded && owned >= 0 && offs[me] ? __float_as_uint(scale[(size_t)owned * p.nkv + h]) & 0x7fffffffu : 0u;
   __syncthreads();
-  // rotates token i's values and brings their largest magnitude to its run
-  auto prepare = [&](int i, float (&x)[NP], float (&y)[NP]) {
-    unsigned m = 0;
+  auto rotate = [&](int i, float (&x)[NP], float (&y)[NP]) {
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       if (!is_v && mine.turned(k)) {
@@ -404,7 +407,24 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
         x[k] = u * cs.x - v * cs.y;
         y[k] = u * cs.y + v * cs.x;
       }
-      m = max(m, max(__float_as_uint(x[k]) & 0x7fffffffu, __float_as_uint(y[k]) & 0x7fffffffu));
+    }
+  };
+  // The largest magnitude of token i's values in this lane, as bits.  Next to a power of two, where it decides the scale,
+  // that of the pairs turned in 64 bits, cut to 32 (which keeps its exponent).
+  auto magnitude = [&](int i, const float (&x)[NP], const float (&y)[NP]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) m = max(m, max(__float_as_uint(x[k]) & 0x7fffffffu, __float_as_uint(y[k]) & 0x7fffffffu));
+    if (!is_v && coded && c8_near_scale(m)) {
+      const float* row = src + (size_t)i * width;
+      m = 0;
+      for (int k = 0; k < NP; ++k) {
+        if (!mine.in(k)) continue;
+        const int2 d = mine.dims(k);
+        double2 u = make_double2(row[d.x], row[d.y]);
+        if (mine.turned(k)) u = rope_exact(poss[i], p.turns[mine.pair(k)], p.amplitude, row[d.x], row[d.y]);
+        m = max(m, __float_as_uint(__double2float_rz(fmax(fabs(u.x), fabs(u.y)))));
+      }
     }
     return m;
   };
@@ -412,13 +432,15 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
   for (int c = 0; c < AP_HELD; ++c) {
     const int i = first + warp + c * AP_WARPS;
     if (i >= last) continue;
-    const unsigned m = __reduce_max_sync(0xffffffffu, prepare(i, a[c], b[c]));
+    rotate(i, a[c], b[c]);
+    const unsigned m = __reduce_max_sync(0xffffffffu, magnitude(i, a[c], b[c]));
     if (lane == 0) atomicMax(&tops[runs[i]], m);
   }
   for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {    // a run cut by the window, pages of many rows
     float x[NP], y[NP];
     load(i, x, y);
-    const unsigned m = __reduce_max_sync(0xffffffffu, prepare(i, x, y));
+    rotate(i, x, y);
+    const unsigned m = __reduce_max_sync(0xffffffffu, magnitude(i, x, y));
     if (lane == 0) atomicMax(&tops[runs[i]], m);
   }
   __syncthreads();
@@ -497,7 +519,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32, NP == 4 ? 4 : 5) rope_append_ke
   for (int i = first + warp + AP_HELD * AP_WARPS; i < last; i += AP_WARPS) {
     float x[NP], y[NP];
     load(i, x, y);
-    prepare(i, x, y);
+    rotate(i, x, y);
     const unsigned some = store(i, x, y);
     if (some) again(i, some);
   }
