@@ -20,16 +20,17 @@ constexpr unsigned C8_NOT_FINITE = 0x7f800000u;   // |x| as bits: from here on i
 // exponent of the scale for a largest magnitude given as the bits of |x|
 __device__ __forceinline__ int c8_exponent(unsigned bits) { return max((int)(bits >> 23) - 133, C8_LOWEST); }
 __device__ __forceinline__ float c8_pow2(int e) { return __int_as_float((e + 127) << 23); }    // -126 <= e <= 127
-// Steps by which the 32-bit rotation can be off: 4 ulp (2^-22) of a pair of length 128 sqrt(2).  Keys nearer than that to a
-// border between codes are rotated again in 64 bits (one in 10,000), so that codes are those of the definition to the last
-// (2,048 tokens 16.6 -> 17.4 us; in 32 bits alone about one code in a million was the one beside it).
-constexpr float C8_NEAR = 4.5e-5f;
+// Steps by which the 32-bit rotation can be off, in units u = 2^-24 of a pair's length (at most 128 sqrt(2) steps): the angle, two
+// roundings and a constant of at most pi / 4, 1.9; sine and cosine 0.8 and 1.0, together 1.3; a product and a sum 2; an
+// amplitude and its product 2: 7.2 u = 7.8e-5 (4.1 u is the most that a search found).  Keys nearer than that to a border
+// between codes are rotated again in 64 bits (one in 6,000), so that codes are those of the definition to the last.
+constexpr float C8_NEAR = 8e-5f;
 __device__ __forceinline__ float c8_distance(float x, float inv) {
   const float h = x * inv, magic = 12582912.f;           // 1.5 * 2^23: the nearest whole number
   return fabsf(h - ((h + magic) - magic));
 }
-// A largest magnitude, given as bits, so near a power of two (16 steps of 32 bits, where 10 are the most that the rotation can be
-// off) that 64 bits have to say which exponent it has.
+// A largest magnitude, given as bits, so near a power of two (16 steps of 32 bits; the rotation's 7.2 u of a pair's length
+// are 10.2 of its larger part) that 64 bits have to say which exponent it has.
 __device__ __forceinline__ bool c8_near_scale(unsigned bits) {
   return bits >= 13u << 23 && bits < C8_NOT_FINITE && ((bits + 16u) & 0x7fffffu) < 32u;
 }
