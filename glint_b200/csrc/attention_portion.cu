@@ -25,7 +25,9 @@
 // 4,096 tokens, 16 heads in 8 groups of 256: 137 GFLOP in 123 us (and 10 for the wide pages) = 1.11 PFLOP/s, 0.68 of what a
 // large product reaches (call after call 144 us: the power cap); tensor pipe and special-function unit are busy 55 % of the time.  Neither binds alone:
 // what is left is the hand-over between the warps of a tile.
-// Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx; keys of a token at position p from
+// Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx: 2^-11 of a capped score, so up to 0.02 in the exponent of
+// a score of 40, beside the 2^-8 of a probability's rounding.  The single-token kernel has its cap to 32 bits; exponential and
+// reciprocal in place of tanh.approx would be a third special-function operation a score where two of them bind.  Keys of a token at position p from
 // max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the
 // second product, and their sum is that of the rounded ones.
 #include "common.cuh"
