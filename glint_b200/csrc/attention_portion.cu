@@ -17,7 +17,7 @@
 // With a soft cap of up to 55 the exponentials need no running maximum at all: scores lie within +-cap (80 log2 units), and
 // probabilities relative to 2^10, between 2^-90 and 2^70, keep the precision they always have in float32 sums and as bfloat16.
 // So do their products with values of up to 2^36 (a row of 2^20 keys that all reach +cap) and down to 2^-36 (one whose
-// keys all stay at -cap).  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that
+// keys all stay at -cap); sums of larger ones that overflow are reported (status 7).  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that
 // has grown by more than 8 log2 units, and O is rescaled then).
 // Where SMs would stay empty (fewer blocks than SMs, or a few blocks behind the last full round of them) the keys of a tile of
 // rows are split over several blocks, whose partial results a second kernel adds up in order.
@@ -542,6 +542,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const int chunk_shift = partial ? 2 : 3;          // elements of a chunk: 4 floats, 8 bfloat16
       const int chunks = hd >> chunk_shift, swizzle = r & 7 & ((chunks & -chunks) - 1);
       uint4* row_at = reinterpret_cast<uint4*>(smem) + (size_t)r * chunks;
+      uint32_t largest = 0, pairs = 0;                   // magnitudes of 32 bits, of two times 16
       for (int c0 = o_lo; c0 < o_hi; c0 += 32) {
         uint32_t o[32];
         tc::tmem_ld_16(tmem_o + lane_base + c0, o);
@@ -555,18 +556,23 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           if (partial) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) row_at[(c + i) ^ swizzle] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) largest = max(largest, v[i] & 0x7fffffffu);
           } else {
             uint32_t h[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
               h[i] = *reinterpret_cast<const uint32_t*>(&x);
+              pairs = __vmaxu2(pairs, h[i] & 0x7fff7fffu);
             }
             row_at[c ^ swizzle] = make_uint4(h[0], h[1], h[2], h[3]);
             row_at[(c + 1) ^ swizzle] = make_uint4(h[4], h[5], h[6], h[7]);
           }
         }
       }
+      // values are finite, and a score that is not makes the row's sum NaN: what else is not finite has overflowed
+      if (rv && total < INFINITY && max(largest, max(pairs, pairs << 16)) >= 0x7f800000u) atomicExch(p.status, 7);
     }
     asm volatile("bar.sync 2, 256;" ::: "memory");
     if (ok) {
@@ -651,6 +657,8 @@ __global__ void __launch_bounds__(256) attention_portion_merge_kernel(const Port
   for (int k = 0; k < 2; ++k) {
     const int d = lane * 4 + k * 128;
     if (d < p.hd) {
+      if (L < INFINITY && !(fmaxf(fmaxf(fabsf(acc[k].x), fabsf(acc[k].y)), fmaxf(fabsf(acc[k].z), fabsf(acc[k].w))) < INFINITY))
+        atomicExch(p.status, 7);                          // (parts that are finite each)
       const __nv_bfloat162 a = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv), b = __floats2bfloat162_rn(acc[k].z * inv, acc[k].w * inv);
       *reinterpret_cast<uint2*>(p.out + row * p.hd + d) =
           make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));

@@ -223,7 +223,11 @@ def unpack(rt, cache, step, window=0):
 def attention(rt, cache, step, q, num_heads, multiplier, softcap=0.0, window=0, out=None):
     """Attention of the step's queries ``q`` [tokens, heads * head size] (the runtime's dtype) over the coded pages, keys
     and values of the step among them: scores times ``multiplier``, soft cap, keys of the last ``window`` positions (0:
-    all).  Returns ``out`` [tokens, heads * head size]."""
+    all).  Returns ``out`` [tokens, heads * head size].
+
+    Range in bfloat16: single tokens take whatever the pages hold.  Portions keep their precision for values between 2^-36 and
+    2^36 where there is a soft cap of up to 55, and of up to 2^90 without one; sums that overflow are reported by
+    ``Runtime.check_status`` (code 7).  Their capped scores are off by up to 2^-11 relative."""
     window = window or 0
     _check(rt, cache, step, window)
     if num_heads < 1 or num_heads % cache.nkv:

@@ -16,7 +16,8 @@ _STATUS_TEXT = {1: "a token id lies outside the embedding table",
                 3: "a key's position has no page in its block table (attention read)",
                 4: "a bounded device-side wait ran out",
                 5: "a request's tokens do not stand together in ascending positions (cache write)",
-                6: "a request holds more tokens than its step was made for (attention read)"}
+                6: "a request holds more tokens than its step was made for (attention read)",
+                7: "values so large that the sums of attention overflow (attention of portions over coded pages)"}
 
 
 def parse_dtype(dtype):

@@ -79,3 +79,43 @@ def test_scores_up_to_the_cap(rts, dtype, reach, case):
                         told += (np.abs(v[lo:hi].mean(axis=0) - want) > 2 * bound).any()
     # what a kernel without the cap, or one that does not look at its scores, would give lies outside
     assert told == rows and (not cap or capped >= (0.4 if reach > 1 else 0.05) * rows), (rows, capped, told)
+
+
+@pytest.mark.parametrize("lens,starts,hd", [([150], [0], 64), ([130], [1500], 128), ([150], [400], 256), ([130], [1500], 256)])
+def test_values_too_large_for_the_sums_of_portions_are_reported(rts, lens, starts, hd):
+    """Scores at +cap over values of up to 2^(7 + e): inside the range the mean of the values, beyond it a report, and the same values
+    without a cap, or as single tokens, are right.  A page that is not finite is no such report."""
+    from glint_b200 import ops_cache8
+    from glint_b200.errors import KernelError
+    rt, nh, nkv, P = rts["bfloat16"], 4, 2, 16
+    T = sum(lens)
+    s = Setup(rt, lens, starts, nkv, hd, P, seed=9)
+    s.cache.k.fill_(255)
+    s.cache.k_scale.fill_(1.0)
+    s.codes[1][:] = 255
+    s.cache.v.fill_(255)
+    q = torch.full((T, nh * hd), 8.0, dtype=torch.bfloat16, device=DEV)
+    one = ops_cache8.StepArrays(*[torch.tensor(a, dtype=torch.int32, device=DEV) for a in ([starts[0] + T - 1], [0], [starts[0] + T - 1], [0, 1])],
+                                s.step.tensors["block_table"], 1, starts[0] + T)
+    for e in (0, 28, 70, 100):
+        s.cache.v_scale.fill_(2.0 ** e)
+        value = 127.5 * 2.0 ** e
+        calls = [(s.step, q, 55.0, e < 30), (s.step, q, 0.0, e < 84), (one, q[:1], 55.0, True), (one, q[:1], 0.0, True)]
+        for step, rows, cap, fine in calls:
+            out = ops_cache8.attention(rt, s.cache, step, rows.contiguous(), nh, 1.0, softcap=cap).double()
+            if fine:
+                rt.check_status()
+                assert ((out - value).abs() <= 2.0 ** -6 * value).all(), (e, cap)
+            elif e == 70:
+                with pytest.raises(KernelError, match="overflow"):
+                    rt.check_status()
+            else:                                   # past what is promised: right, or reported
+                try:
+                    rt.check_status()
+                except KernelError:
+                    continue
+                assert ((out - value).abs() <= 2.0 ** -6 * value).all(), (e, cap)
+    s.cache.v_scale.fill_(float("nan"))
+    out = ops_cache8.attention(rt, s.cache, s.step, q, nh, 1.0, softcap=55.0)
+    assert out.isnan().all()
+    rt.check_status()
