@@ -41,7 +41,8 @@ class LLM:
     decode step with the previous step's sampled tokens still on the device and read them one step
     late, so that the host's work overlaps the GPU's (same tokens as without it).
     ``cache_dtype``: None keeps keys and values in ``dtype``; 'int8' keeps them in codes of 8 bits with a
-    scale per page and head, for twice the tokens in the same memory and half the bytes per decoded token.
+    scale per page and head: half the bytes per decoded token and, in bfloat16, 2 n / (n + 2) times the tokens in the
+    same memory for groups of n layers (a group keeps one layer's pages wide): 1.83 with 42 layers in two groups.
     """
 
     def __init__(self, model_path=None, dtype="bfloat16", device="cuda:0", cache_tokens=None, max_active=64,

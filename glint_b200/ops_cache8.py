@@ -8,8 +8,10 @@ only, not on how they were cut into steps; a value is off by at most half a step
 
 The calls launch on the current stream of the runtime's device, with the kernels the runtime chooses.  ``Cache8`` and
 ``StepArrays`` are made once for a layer's pages and a step's arrays and only point at them: what the arrays hold is
-read by the kernels.  A ``Cache8`` holds scratch (the wide pools for portions, partial results for single tokens): calls on
-one ``Cache8`` belong on one stream, or on streams that wait for each other, graphs among them.
+read by the kernels.  A ``Cache8`` holds scratch: wide pools for portions, twice the bytes of the codes, and partial results.  The
+layers of a model share one (``Cache8.empty(..., like=first)``); with its own each would hold more than pages of bfloat16.  Calls
+on one ``Cache8``, or on several that share scratch, belong on one stream, or on streams that wait for each other, graphs among
+them.
 """
 from __future__ import annotations
 
@@ -48,13 +50,14 @@ def _lib():
 class Cache8:
     """One layer's pages: ``k``, ``v`` uint8 [pages, kv heads, page size, head size], ``k_scale``, ``v_scale`` float32
     [pages, kv heads], and ``k_wide``, ``v_wide``, scratch of the codes' shape in the runtime's dtype.  The wide pools
-    have to be finite when the cache is made (zeros)."""
+    have to be finite when the cache is made (zeros).  ``scratch``: another cache's, of the same shape; made here unless given."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
     v_scale: torch.Tensor
     k_wide: torch.Tensor
     v_wide: torch.Tensor
+    scratch: tuple = None
 
     def __post_init__(self):
         for name in ("k", "v"):
@@ -74,7 +77,11 @@ class Cache8:
             raise KernelError("the tensors of a coded cache belong to one device")
         if any(t.data_ptr() % 16 for t in (self.k, self.v, self.k_wide, self.v_wide)):
             raise KernelError("the pools of a coded cache begin at multiples of 16 bytes")
-        self.scratch = partials, arrive = native.cache8_scratch(self.nkv, self.hd, self.k.device)
+        if self.scratch is None:
+            self.scratch = native.cache8_scratch(self.nkv, self.hd, self.k.device)
+        partials, arrive = self.scratch
+        if any(t.device != self.k.device for t in self.scratch):
+            raise KernelError("the tensors of a coded cache belong to one device")
         self.struct = native.ViewStruct(self.k.data_ptr(), self.v.data_ptr(), self.page_size, self.num_pages, 0, 1,
                                         self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.k_wide.data_ptr(),
                                         self.v_wide.data_ptr(), partials.data_ptr(), partials.numel(), arrive.data_ptr(),
@@ -83,13 +90,18 @@ class Cache8:
         self.device = self.k.device
 
     @classmethod
-    def empty(cls, num_pages, num_kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda:0"):
-        """A cache that holds nothing yet."""
+    def empty(cls, num_pages, num_kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda:0", like=None):
+        """A cache that holds nothing yet.  ``like``: a cache of the same sizes, dtype and device, say another layer's, whose wide
+        pools and scratch this one shares."""
         shape = (num_pages, num_kv_heads, page_size, head_dim)
         made = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2)]
         made += [torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)]
-        made += [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
-        return cls(*made)
+        if like is None:
+            return cls(*made, *[torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)])
+        if tuple(like.k.shape) != shape or like.dtype != dtype or like.device != made[0].device:
+            raise KernelError(f"a cache of {shape} with wide pools of {dtype} on {made[0].device} cannot share those of one of "
+                              f"{tuple(like.k.shape)}, {like.dtype} on {like.device}")
+        return cls(*made, like.k_wide, like.v_wide, like.scratch)
 
 
 class StepArrays:

@@ -85,3 +85,34 @@ def test_portions_between_products_and_beside_others(rts, hd):
         for outs in got[k]:
             for a, b in zip(outs, want[k]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lens,starts", [([1] * 6, [0] * 6), ([200, 1], [0, 0])])
+def test_layers_that_share_scratch(rts, lens, starts):
+    """Three layers' appends and attention, step after step on one stream, over caches that share their wide pages and scratch: bit for
+    bit what caches of their own give."""
+    from glint_b200 import ops_cache8
+    rt, nh, nkv, hd, P, layers = rts["bfloat16"], 4, 2, 128, 16, 3
+    R, pages = len(lens), 40
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(1))[:R * (pages // R)].view(R, -1).to(DEV, torch.int32)
+    turns = _turns(hd // 2).to(DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    results = []
+    for shared in (False, True):
+        caches = [ops_cache8.Cache8.empty(pages, nkv, P, hd)]
+        caches += [ops_cache8.Cache8.empty(pages, nkv, P, hd, like=caches[0] if shared else None) for _ in range(layers - 1)]
+        at, outs = list(starts), []
+        for step_no in range(4):
+            ns = lens if step_no == 0 else [1 + step_no % 2] * R
+            pos = [a + k for a, n in zip(at, ns) for k in range(n)]
+            cu = [sum(ns[:r]) for r in range(R + 1)]
+            step = ops_cache8.StepArrays(i32(pos), i32([r for r, n in enumerate(ns) for _ in range(n)]), i32(at), i32(cu), table, max(ns),
+                                         max(a + n for a, n in zip(at, ns)))
+            for layer, cache in enumerate(caches):
+                q = ops_cache8.append(rt, cache, step, _qkv(len(pos), nh, nkv, hd, 10 * step_no + layer, 0.3).to(DEV), turns, nh)
+                outs.append(ops_cache8.attention(rt, cache, step, q, nh, 0.1, softcap=50.0))
+            at = [a + n for a, n in zip(at, ns)]
+        rt.check_status()
+        results.append(outs + [getattr(c, n) for c in caches for n in ("k", "v", "k_scale", "v_scale")])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
