@@ -190,7 +190,9 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const int pos = positions[t];
   const int first = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
   // the split takes whole pages, counted from the page that holds the first key
-  const int page_lo = first / page_size, page_hi = pos / page_size;
+  // (a position that the block table has no room for is reported, and held to its last page)
+  const int page_lo = first / page_size, page_hi = min(pos / page_size, max_pages - 1);
+  if (page_hi < pos / page_size && threadIdx.x == 0) atomicExch(status, 3);
   const int pages_per_split = (page_hi - page_lo + splits) / splits;
   const int my_lo = page_lo + split * pages_per_split;
   const int my_hi = min(page_hi + 1, my_lo + pages_per_split);     // exclusive

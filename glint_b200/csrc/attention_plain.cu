@@ -41,7 +41,10 @@ attention_plain_kernel(const S* __restrict__ q, const S* __restrict__ k_pool,
     acc[i] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
-  for (int p = start; p <= pos; ++p) {
+  // a position that the block table has no room for is reported, and held to its last key
+  const int last = (int)min((long long)pos, (long long)max_pages * page_size - 1);
+  if (last < pos && lane == 0) atomicExch(status, 3);
+  for (int p = start; p <= last; ++p) {
     const int page = table[p / page_size];
     if (page < 0 || page >= num_pages) {  // a key the block table does not hold: report, skip
       if (lane == 0) atomicExch(status, 3);

@@ -134,7 +134,8 @@ __device__ __forceinline__ PortionKeys portion_keys(const PortionParams& p, cons
   PortionKeys k;
   const int tok0 = w.tile * tok_per_tile;
   k.pos0 = w.start + tok0;
-  k.pos_last = k.pos0 + min(tok_per_tile, w.len - tok0) - 1;
+  // a position that the block table has no room for (the widening in front has reported it) is held to its last page
+  k.pos_last = (int)min((long long)k.pos0 + min(tok_per_tile, w.len - tok0) - 1, (long long)p.max_pages * p.page_size - 1);
   k.kv_first = p.window > 0 ? max(0, k.pos0 - p.window + 1) : 0;
   k.begin = k.kv_first & ~(AT_N - 1);
   k.tiles = (k.pos_last - k.begin + AT_N) / AT_N;
@@ -224,7 +225,8 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int pos0 = keys.pos0, pos_last = keys.pos_last, kv_first = keys.kv_first;
   const int kv_begin = keys.begin + split * keys.per * AT_N;                      // this split's first tile
   const int n_tiles = min(keys.per, keys.tiles - split * keys.per);
-  if (n_tiles <= 0) {                                    // fewer parts than blocks (the same for all threads)
+  if (n_tiles <= 0) {                                    // fewer parts than blocks, or no key (the same for all threads)
+    if (may_split && split == 0 && threadIdx.x == 0) p.part_info[split_tile] = make_int4(0, 0, 0, 0);
     leave();
     return;
   }

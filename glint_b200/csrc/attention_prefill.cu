@@ -111,12 +111,15 @@ attention_prefill_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
   const int kv_first = window > 0 ? max(0, pos0 - window + 1) : 0;
-  for (int kv0 = kv_first & ~(PF_KEYS - 1); kv0 <= pos_last; kv0 += PF_KEYS) {
+  // a position that the block table has no room for is reported, and held to its last key
+  const int kv_last = (int)min((long long)pos_last, (long long)max_pages * page_size - 1);
+  if (kv_last < pos_last && tid == 0) atomicExch(status, 3);
+  for (int kv0 = kv_first & ~(PF_KEYS - 1); kv0 <= kv_last; kv0 += PF_KEYS) {
     __syncthreads();   // everyone is done with the previous tile
     for (int idx = tid; idx < PF_KEYS * pieces; idx += PF_THREADS) {
       const int r = idx / pieces, c = idx % pieces;
       const int key = kv0 + r;
-      bool valid = key >= kv_first && key <= pos_last;
+      bool valid = key >= kv_first && key <= kv_last;
       int page = 0;
       if (valid) {
         page = table[key / page_size];
