@@ -107,8 +107,8 @@ class Cache8:
 class StepArrays:
     """The arrays of a step (int32, on the device) for calls that bring their own: ``positions`` and ``token_seq`` per
     token (a request's tokens stand together, in ascending positions; requests in the order of their rows), ``seq_start``
-    (tokens cached before the step) and ``cu_seqlens`` (token offsets, one more) per request, ``block_table``
-    [requests, pages].  ``max_seq_len`` is the most tokens of a request, ``max_context`` at least the largest position
+    (tokens cached before the step) and ``cu_seqlens`` (token offsets, one more, the last of them the number of tokens) per
+    request, ``block_table`` [requests, pages].  Every token is a request's: a row of padding would be one like the others.  ``max_seq_len`` is the most tokens of a request, ``max_context`` at least the largest position
     plus one; ``contexts``: the contexts of the requests in front that bring a single token, for planning launches.
     A page that a step writes belongs to one of its requests; pages that are only read may be several requests'.
     ``begin()`` starts a new step: the arrays may hold other values, and what was planned for the old ones is not used.
@@ -128,10 +128,13 @@ class StepArrays:
                               f"{cu_seqlens.numel()} offsets, block table {tuple(block_table.shape)}")
         if T and not (1 <= max_seq_len <= T and max_context >= max_seq_len and R >= 1):
             raise KernelError(f"max_seq_len {max_seq_len} and max_context {max_context} do not fit {T} tokens")
-        if len(contexts) > R:
-            raise KernelError(f"{len(contexts)} contexts for {R} requests")
-        self.tensors, self.num_tokens, self.device_index = named, T, positions.get_device()
         contexts = [int(c) for c in contexts]
+        # the requests in front bring a token each; where some bring more, those stand behind
+        if len(contexts) > min(R, T) or (contexts and max_seq_len > 1 and len(contexts) == min(R, T)):
+            raise KernelError(f"{len(contexts)} contexts of single tokens do not fit {R} requests of {T} tokens, up to {max_seq_len} each")
+        if contexts and not 1 <= min(contexts) <= max(contexts) <= max_context:
+            raise KernelError(f"contexts from {min(contexts)} to {max(contexts)} do not lie within 1 and {max_context}")
+        self.tensors, self.num_tokens, self.device_index = named, T, positions.get_device()
         s = self.struct = native.StepStruct()
         s.num_tokens, s.num_seqs, s.max_seq_len, s.max_context = T, R, int(max_seq_len), int(max_context)
         s.leading_single, s.leading_single_context = (R if max_seq_len == 1 else len(contexts)), max(contexts or [0])
