@@ -194,10 +194,14 @@ def rope_append(qkv, positions, token_seq, block_table, turns, q_out, k_pool, v_
             or positions.numel() != T or token_seq.numel() != T):
         raise KernelError(f"rope_append shapes do not fit: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)}, "
                           f"{positions.numel()} positions, {turns.numel()} pairs, heads {nh}/{nkv} x {hd}")
+    if (k_pool is None) != (v_pool is None) or (k_scale is None) != (v_scale is None) or (k_scale is not None and k_pool is None):
+        raise KernelError("keys and values go into pools, and scales, of both or of neither")
     if k_pool is not None and any(t.numel() != n for t, n in ((k_pool, num_pages * nkv * page_size * hd), (v_pool, k_pool.numel()))):
         raise KernelError(f"pools {tuple(k_pool.shape)} and {tuple(v_pool.shape)} are not {num_pages} pages of {nkv} x {page_size} x {hd}")
     if k_scale is not None and not k_scale.numel() == v_scale.numel() == num_pages * nkv:
         raise KernelError(f"scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)} are not {num_pages} x {nkv}")
+    if status is None:
+        raise KernelError("rope_append wants a status word for positions without a page")
     check(core().glint_rope_append(ptr(qkv), ptr(positions), ptr(token_seq), ptr(block_table), block_table.shape[1],
                                    ptr(turns), 2 * turns.numel(), int(bool(interleaved)), amplitude, ptr(q_out),
                                    dtype_code(q_out.dtype), ptr(k_pool), ptr(v_pool), ptr(k_scale), ptr(v_scale), T, nh,

@@ -31,3 +31,15 @@ def test_contexts_that_do_not_fit_the_step(monkeypatch, contexts, lens):
 def test_contexts_that_do(monkeypatch, contexts, lens):
     _pretend(monkeypatch)
     assert _mixed(contexts, lens).struct.leading_single == (len(lens) if max(lens) == 1 else len(contexts))
+
+
+@pytest.mark.parametrize("missing", [("v_pool",), ("k_scale",), ("v_scale",), ("k_pool", "v_pool"), ("status",)])
+def test_an_operand_left_out_is_refused(monkeypatch, missing):
+    _pretend(monkeypatch)
+    z = lambda *shape, dtype=torch.float32: torch.zeros(*shape, dtype=dtype)
+    args = dict(qkv=z(3, 8 * 32), positions=i32(0, 1, 2), token_seq=i32(0, 0, 0), block_table=z(1, 3, dtype=torch.int32), turns=z(16, dtype=torch.float64),
+                q_out=z(3, 4 * 32), k_pool=z(3, 2, 16, 32, dtype=torch.uint8), v_pool=z(3, 2, 16, 32, dtype=torch.uint8),
+                nh=4, nkv=2, hd=32, page_size=16, num_pages=3, status=i32(0), k_scale=z(3, 2), v_scale=z(3, 2))
+    args.update({name: None for name in missing})
+    with pytest.raises(KernelError, match="pool|scale|status"):
+        ops_cache8.ops.rope_append(**args)
