@@ -188,15 +188,7 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 65) tc::tma_prefetch_desc(&map_k);
     if (threadIdx.x == 66) tc::tma_prefetch_desc(&map_v);
   }
-  // Tensor memory is taken before the successor is released: one that takes its own before it waits for this kernel could
-  // else leave a block here without.
-  if (warp == 1) tc::tmem_alloc(&sh->tmem_base, TMEM_COLS);
-  tc::fence_before_thread_sync();
   __syncthreads();
-  tc::fence_after_thread_sync();
-  auto leave = [&] {                                     // all threads together, before any product
-    if (warp == 1) tc::tmem_dealloc(sh->tmem_base, TMEM_COLS);
-  };
   // blocks count (query tile from the last, kv head); from split_from on every such tile has `splits` blocks
   const bool may_split = (int)blockIdx.x >= p.split_from;
   const int behind = may_split ? (int)blockIdx.x - p.split_from : 0;
@@ -206,15 +198,13 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (!p.early) pdl_wait();
   PortionTile work;
   const bool found = portion_tile(p, tok_per_tile, index / p.nkv, work);
-  pdl_wait_release();
+  pdl_wait();
   if (tc::smem_u32(at_raw) & 1023) {                     // the operands' swizzle wants it
     if (threadIdx.x == 0) atomicExch(p.status, 4);
-    leave();
     return;
   }
   if (!found) {
     if (may_split && threadIdx.x == 0) p.part_info[split_tile] = make_int4(0, 0, 0, 0);
-    leave();
     return;
   }
   const int seq = work.seq, tile = work.tile, t_begin = work.begin, q_len = work.len;
@@ -227,12 +217,20 @@ attention_portion_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int n_tiles = min(keys.per, keys.tiles - split * keys.per);
   if (n_tiles <= 0) {                                    // fewer parts than blocks, or no key (the same for all threads)
     if (may_split && split == 0 && threadIdx.x == 0) p.part_info[split_tile] = make_int4(0, 0, 0, 0);
-    leave();
     return;
   }
   if (threadIdx.x == 4 * 32) {
     sh->part_tile = keys.parts > 1 ? split * p.split_tiles + split_tile : -1;
     if (may_split && split == 0) p.part_info[split_tile] = make_int4(keys.parts, n_rows, t_begin + tok0, kvh);
+  }
+  if (warp != 0 && warp != 3) {                          // the producers begin at once
+    // Tensor memory is taken before the successor is released: one that takes its own before it waits for this kernel could
+    // else leave a block here without.  (With the allocation in front of everything the ragged portions took 1 us more.)
+    if (warp == 1) tc::tmem_alloc(&sh->tmem_base, TMEM_COLS);
+    tc::fence_before_thread_sync();
+    asm volatile("bar.sync 3, %0;" ::"n"(AT_THREADS - 64) : "memory");
+    tc::fence_after_thread_sync();
+    pdl_launch_dependents();
   }
   const uint32_t tmem_s = warp != 0 && warp != 3 ? sh->tmem_base : 0u;      // two score buffers of 64 columns
   // two of P as bfloat16 pairs, 32 columns each; O, up to 256 columns (PAIR: 128)
