@@ -20,9 +20,10 @@
 // bits of a half) as its ratio to a reference scale, which the accumulators follow when the ratio leaves [1/8, 8].
 // Scores, soft cap, maxima, sums and accumulators are 32-bit.
 //
-// 64 requests of about 2,200 keys, 16 heads in 8 groups of 256: 581 MB of codes in 101 us = 5.75 TB/s, 0.88 of a copy's
-// rate; one request of 2,000 keys 9.4 us, nearly all of it round trips (where a block begins, its pages' numbers, scales, the
-// pages, the meeting of the parts), of which the first two pass under the kernel in front.
+// 64 requests of about 2,200 keys, 16 heads in 8 groups of 256: 581 MB of codes in 102 us = 5.7 TB/s, 0.87 of a copy's
+// rate; one request of 2,000 keys 9.5 us, nearly all of it round trips (where a block begins, its pages' numbers, scales, the
+// pages, the meeting of the parts), of which the first two pass under the kernel in front.  They do so only where the step's
+// arrays come by copies: behind a kernel that may have written them, 103 and 11.1 us.
 // Score = (q.k) * multiplier, then cap * tanh(score / cap); keys from max(0, pos - window + 1) to pos.
 //
 // No key is masked by zeroing values: codes are finite whatever bytes an unwritten row holds, and so is what

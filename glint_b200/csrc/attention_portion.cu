@@ -17,19 +17,19 @@
 // With a soft cap of up to 55 the exponentials need no running maximum at all: scores lie within +-cap (80 log2 units), and
 // probabilities relative to 2^10, between 2^-90 and 2^70, keep the precision they always have in float32 sums and as bfloat16.
 // So do their products with values of up to 2^36 (a row of 2^20 keys that all reach +cap) and down to 2^-36 (one whose
-// keys all stay at -cap); sums of larger ones that overflow are reported (status 7).  Otherwise the groups hand each row's reference from tile to tile (it follows the maximum when that
-// has grown by more than 8 log2 units, and O is rescaled then).
+// keys all stay at -cap); sums of larger ones that overflow are reported (status 7).  Otherwise the groups hand each row's
+// reference from tile to tile (it follows the maximum when that has grown by more than 8 log2 units, and O is rescaled then).
 // Where SMs would stay empty (fewer blocks than SMs, or a few blocks behind the last full round of them) the keys of a tile of
 // rows are split over several blocks, whose partial results a second kernel adds up in order.
 // Blocks are found from the portions' lengths, so that short portions beside long ones cost no empty blocks.
-// 4,096 tokens, 16 heads in 8 groups of 256: 137 GFLOP in 123 us (and 10 for the wide pages) = 1.11 PFLOP/s, 0.68 of what a
-// large product reaches (call after call 144 us: the power cap); tensor pipe and special-function unit are busy 55 % of the time.  Neither binds alone:
-// what is left is the hand-over between the warps of a tile.
-// Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx: 2^-11 of a capped score, so up to 0.02 in the exponent of
-// a score of 40, beside the 2^-8 of a probability's rounding.  The single-token kernel has its cap to 32 bits; exponential and
-// reciprocal in place of tanh.approx would be a third special-function operation a score where two of them bind.  Keys of a token at position p from
-// max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit; probabilities are rounded to bfloat16 for the
-// second product, and their sum is that of the rounded ones.
+// 4,096 tokens, 16 heads in 8 groups of 256: 137 GFLOP in 124 us (and 10 for the wide pages) = 1.11 PFLOP/s, 0.68 of what a
+// large product reaches (call after call 145 us: the power cap); tensor pipe and special-function unit are busy 55 % of the
+// time.  Neither binds alone: what is left is the hand-over between the warps of a tile.
+// Score = (q.k) * multiplier, then cap * tanh(score / cap) with tanh.approx: 2^-11 of a capped score, so up to 0.02 in the
+// exponent of a score of 40, beside the 2^-8 of a probability's rounding.  The single-token kernel has its cap to 32 bits;
+// exponential and reciprocal in place of tanh.approx would be a third special-function operation a score where two of them
+// bind.  Keys of a token at position p from max(0, p - window + 1) to p.  Sums, references and accumulators are 32-bit;
+// probabilities are rounded to bfloat16 for the second product, and their sum is that of the rounded ones.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -144,8 +144,9 @@ __device__ __forceinline__ PortionKeys portion_keys(const PortionParams& p, cons
   return k;
 }
 
-// FIXED: the soft cap spares the running maximum (4,096 tokens, 16 heads in 8 groups of 256: 134 us, 211 without; 2,282 ragged
-// ones, 32 heads in 16 groups of 128: 90 and 174, where the columns that do not fit the registers are computed twice).
+// FIXED: the soft cap spares the running maximum (with the widening, at cap 50 / without a cap / at cap 56: 4,096 tokens, 16 heads
+// in 8 groups of 256, 136 / 170 / 188 us; 2,282 ragged ones, 32 heads in 16 groups of 128, 92 / 134 / 166, where the columns that
+// do not fit the registers are computed twice).
 // PAIR: two blocks on an SM (head sizes up to 128): each has half of the tensor memory, so that P is written over the scores
 // it came from and the scores two tiles on wait for the product that reads it; one block's beginning and end pass under the
 // other's tiles (the ragged portions 90 us, 105 with one block).

@@ -33,8 +33,8 @@ struct GlintStep {
   const int* logit_rows;        // [logit rows]
   const int* block_table[GLINT_MAX_GROUPS];   // per cache group: [requests][max_pages]
   int max_pages[GLINT_MAX_GROUPS];
-  int copied;                   // 1: the device arrays came by a copy, which is over before any kernel behind it begins: kernels may
-                                // read them before they wait for the kernel in front.  0: a kernel in front may have written them
+  int copied;                   // 1: the device arrays came by a copy, which is over before any kernel behind it begins: kernels
+                                // may read them before they wait for the kernel in front.  0: that may have written them
 };
 
 // Entry points of the tensor-core library, bound at run time (a float32 process never loads it).

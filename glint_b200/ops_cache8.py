@@ -108,11 +108,12 @@ class StepArrays:
     """The arrays of a step (int32, on the device) for calls that bring their own: ``positions`` and ``token_seq`` per
     token (a request's tokens stand together, in ascending positions; requests in the order of their rows), ``seq_start``
     (tokens cached before the step) and ``cu_seqlens`` (token offsets, one more, the last of them the number of tokens) per
-    request, ``block_table`` [requests, pages].  Every token is a request's: a row of padding would be one like the others.  ``max_seq_len`` is the most tokens of a request, ``max_context`` at least the largest position
-    plus one; ``contexts``: the contexts of the requests in front that bring a single token, for planning launches.
-    A page that a step writes belongs to one of its requests; pages that are only read may be several requests'.
-    ``begin()`` starts a new step: the arrays may hold other values, and what was planned for the old ones is not used.
-    Kernels in front on the stream may write them (``positions += 1``): the calls read them behind those kernels' end."""
+    request, ``block_table`` [requests, pages].  Every token is a request's: a row of padding would be one like the others.
+    ``max_seq_len`` is the most tokens of a request, ``max_context`` at least the largest position plus one; ``contexts``:
+    the contexts of the requests in front that bring a single token, for planning launches.  A page that a step writes
+    belongs to one of its requests; pages that are only read may be several requests'.  ``begin()`` starts a new step: the
+    arrays may hold other values, and what was planned for the old ones is not used.  Kernels in front on the stream may write
+    them (``positions += 1``), also in a captured graph: the calls read them behind those kernels' end."""
 
     def __init__(self, positions, token_seq, seq_start, cu_seqlens, block_table, max_seq_len, max_context, contexts=()):
         from .engine.step import _uneven
